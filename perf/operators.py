@@ -380,17 +380,19 @@ def _run_own(s):
         s["ws"] = ops.RequestWorkspace()
         if c["op"] == "lora":
             s["adapters"] = ops.LoraAdapters(s["A"], s["B"], s["scales"], s["ranks"])
+        if c["op"] in ("append", "attend"):
+            s["layer"] = ops.KVCache(*s["cache"])
     if c["op"] == "plan":
         p = ops.page_plan(s["lens"], s["new"], s["table"], s["free"], s["count"], c["page"], s["T"], s["ws"], parents=s["parents"],
                           free_count_out=s["count_out"])
         out = [p.q_start, p.slots, p.positions, s["table"], s["count_out"]]
         return out + [p.mask] if c["tree"] else out
     if c["op"] == "append":
-        ops.rope_append(s["q"], s["k"], s["v"], s["lut"], s["positions"], s["slots"], s["cache"][0], s["cache"][1], s["ws"], q_out=s["q_out"])
+        ops.rope_append(s["q"], s["k"], s["v"], s["lut"], s["positions"], s["slots"], s["layer"], s["ws"], q_out=s["q_out"])
         return s["q_out"], s["cache"]
     if c["op"] == "attend":
-        return ops.tree_attention(s["q"], s["cache"][0], s["cache"][1], s["table"], s["lens"], s["q_start"], s["ws"], mask=s["mask"],
-                                  scale=s["scale"], out=s["out"])
+        return ops.tree_attention(s["q"], s["layer"], s["table"], s["lens"], s["q_start"], s["ws"], mask=s["mask"], scale=s["scale"],
+                                  out=s["out"])
     if c["op"] == "keep":
         ops.page_keep(s["kv"], s["table"], s["lens"], s["q_start"], s["kept"], s["free"], s["count"], s["ws"], path=s["path"],
                       lens_out=s["lens_out"], free_count_out=s["count_out"])
