@@ -444,6 +444,82 @@ int awq_b200_rope_halfsplit_bf16(const uint16_t *x, size_t x_stride, const uint1
                                  uint16_t *out, size_t out_stride, int B, int n_heads,
                                  int head_dim, awq_stream_t stream);
 
+/* ---- many requests: paged cache, drafted tokens, adapters ---------------------------------------
+ * No counterpart in the reference, whose decode loop serves one request and runs attention on the host
+ * between the QKV block and the O projection (llms/llama32_1b_int4/llama32_1b_int4_decode.py:266-275).
+ *
+ * A step works on T rows: the new tokens of R requests, one request after another, request r's rows being
+ * q_start[r] .. q_start[r + 1].  Its K and V lie in pages of page_size slots; token p of request r is in slot
+ * table[r][p / page_size] * page_size + p % page_size.  `lens` counts the tokens a request had before the step; the
+ * step's own tokens follow them.  R <= 4096, T <= 2^20, a cache has less than 2^31 slots; strides are in elements.
+ *
+ * Lengths, pages, slots and adapters live on the device, where the host cannot check them: a kernel that meets one
+ * outside its buffers skips the access and sets a bit in the workspace's error word, which awq_b200_request_check
+ * reports.  The workspace is zeroed once with awq_b200_workspace_init and left clean by every call; calls that may
+ * overlap on the GPU (two streams, two captured graphs) need one each. */
+size_t awq_b200_request_workspace_bytes(void);
+/* Synchronise `stream`; AWQ_ERR_INVALID_ARGUMENT (or AWQ_ERR_DEVICE_TIMEOUT) and a text if a call since the last check met
+ * such an index.  Clears the error word. */
+int awq_b200_request_check(void *workspace, awq_stream_t stream);
+
+/* K and V of one layer: [n_pages, page_size, n_kv_heads, head_dim], bf16 or fp16 (AWQ_ACT_*), any strides that are
+ * multiples of 8 elements, the head_dim values of a head side by side. */
+typedef struct {
+    const void *k, *v;
+    long long k_page_stride, k_slot_stride, k_head_stride, v_page_stride, v_slot_stride, v_head_stride;
+    int n_pages, page_size, n_kv_heads, head_dim, format;
+} awq_b200_kv_cache_t;
+
+/* Plan a step: pages for lens[r] + fresh[r] tokens of every request (new ones popped from the free pages, a stack of *free_count
+ * entries in an array of `pool`, request by request, topmost first; *free_count_out, which may be free_count, gets the rest), and for
+ * every row its slot, its position and, with `parents` (int32 [T]: index in the tree of the token it continues, -1: the last
+ * cached one; up to 64 tokens per request), the mask of its ancestors and itself; its position is then lens + its depth.
+ * q_start int32 [R + 1]; rows behind the last request get slot -1, position 0, mask 0.  A step that does not fit (pages,
+ * T rows, the table's width, a tree's 64 tokens) changes nothing, gets no rows, and is reported by awq_b200_request_check. */
+int awq_b200_page_plan(const int32_t *lens, const int32_t *fresh, int32_t *table, long long table_stride, int table_width,
+                       const int32_t *free_pages, int pool, const int32_t *free_count, int32_t *free_count_out,
+                       const int32_t *parents, int page_size, int32_t *q_start, int32_t *slots, int32_t *positions,
+                       long long *mask, int R, int T, void *workspace, size_t workspace_bytes, awq_stream_t stream);
+
+/* Half-split RoPE (as awq_b200_rope_halfsplit_bf16) of Q and K by row positions[t] of lut bf16 [n_positions, head_dim], K and V
+ * into slot slots[t] of the cache (-1: the row is left out).  A slot that several rows name keeps the last of them.
+ * q_out may be q.  Rows and cache share one format. */
+int awq_b200_rope_append(const void *q, long long q_row_stride, long long q_head_stride, const void *k, long long k_row_stride,
+                         long long k_head_stride, const void *v, long long v_row_stride, long long v_head_stride, const uint16_t *lut,
+                         int n_positions, const int32_t *positions, const int32_t *slots, void *q_out, long long q_out_row_stride,
+                         long long q_out_head_stride, const awq_b200_kv_cache_t *cache, int T, int n_heads, void *workspace,
+                         size_t workspace_bytes, awq_stream_t stream);
+
+/* out[t, h] = softmax over the keys row t sees of scale q[t, h] . k, times v; heads in groups of n_heads / n_kv_heads share a cache
+ * head.  A row sees its request's lens[r] cached tokens and of the step's tokens of its request token j if bit j of mask[t] is set
+ * (int64 [T], up to 64 tokens per request), or, without `mask`, those up to itself (any number).  A row that sees nothing is 0;
+ * rows behind the last request are left as they are. */
+int awq_b200_tree_attention(const void *q, long long q_row_stride, long long q_head_stride, const awq_b200_kv_cache_t *cache,
+                            const int32_t *table, long long table_stride, int table_width, const int32_t *lens, const int32_t *q_start,
+                            const long long *mask, float scale, void *out, long long out_row_stride, long long out_head_stride, int R, int T,
+                            int n_heads, void *workspace, size_t workspace_bytes, awq_stream_t stream);
+
+/* Keep kept[r] of the step's tokens of every request, in every layer of kv [layers, 2, n_pages, page_size, n_kv_heads, head_dim] (any
+ * 16-bit type): the rows path[q_start[r] + i] (ascending; NULL: the first kept[r], which lie where they belong) move to lens[r] + i,
+ * lens_out[r] = lens[r] + kept[r] (lens_out may be lens), and the pages behind that go back onto the stack of free pages.
+ * kept[r] = -1 ends the request: length 0, all pages free.  A path has up to 64 tokens.  A request whose count or path does not fit
+ * keeps nothing and is reported by awq_b200_request_check. */
+int awq_b200_page_keep(void *kv, long long layer_stride, long long kv_stride, long long page_stride, long long slot_stride,
+                       long long head_stride, int layers, int n_pages, int page_size, int n_kv_heads, int head_dim,
+                       const int32_t *table, long long table_stride, int table_width, const int32_t *lens, int32_t *lens_out,
+                       const int32_t *q_start, const int32_t *kept, const int32_t *path, int32_t *free_pages, int pool,
+                       const int32_t *free_count, int32_t *free_count_out, int R, int T, void *workspace, size_t workspace_bytes,
+                       awq_stream_t stream);
+
+/* out bf16 [T, N] = bf16(base + scales[a] (x A[a]^T) B[a]^T (+ residual)), a = idx[t] per row (-1: base alone): low-rank adapters
+ * beside a shared projection, whose f32 sums (awq_b200_gemv_f32 and the like) or bf16 output `base` is.  A bf16 [n, rank_max, K],
+ * B bf16 [n, N, rank_max], of which adapter a uses ranks[a] rows / columns (NULL: all); rank_max a multiple of 8 up to 128, K and N
+ * multiples of 8, T <= 65535.  out may be a bf16 base; base and residual are [T, N]. */
+int awq_b200_lora_bf16(const uint16_t *x, long long x_row_stride, const uint16_t *A, const uint16_t *B, const float *scales,
+                       const int32_t *ranks, int n_adapters, int rank_max, const int32_t *idx, const void *base, int base_is_f32,
+                       const uint16_t *residual, uint16_t *out, int T, int K, int N, void *workspace, size_t workspace_bytes,
+                       awq_stream_t stream);
+
 /* ---- layout converters (once per weight) ------------------------------------------------
  * Layout B is mlir-air's logical form (matvec_int4_packed.py:346-350):
  *   A_q uint8 [M, K/2] (low nibble = even k), A_s bf16 [K/gs, M], A_z uint8 [K/gs, M], M = N.

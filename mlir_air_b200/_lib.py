@@ -30,8 +30,23 @@ class AwqBackendError(Exception):
         self.status = status
 
 
+class KvCacheStruct(ctypes.Structure):
+    """awq_b200_kv_cache_t"""
+    _fields_ = [("k", c_void_p), ("v", c_void_p)] + [(n, ctypes.c_longlong) for n in (
+        "k_page_stride", "k_slot_stride", "k_head_stride", "v_page_stride", "v_slot_stride", "v_head_stride")] + \
+        [(n, c_int) for n in ("n_pages", "page_size", "n_kv_heads", "head_dim", "format")]
+
+
+MAX_ROWS = 1 << 20  # rows of a step at most
+
+
+def address_of(struct) -> int:
+    return ctypes.addressof(struct)
+
+
 # name -> (restype, argtypes); mirrors include/awq_b200.h one to one
 _P = c_void_p
+_L = ctypes.c_longlong
 SIGNATURES = {
     "awq_b200_version": (c_int, []),
     "awq_b200_last_error": (c_char_p, []),
@@ -87,6 +102,13 @@ SIGNATURES = {
     "awq_b200_ffn_layer_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
     "awq_b200_ffn_layer_decode_bf16": (c_int, [_P, _P, c_float] + [_P] * 7 + [c_int, c_int, c_int, c_int, _P, c_size_t, _P]),
     "awq_b200_gemm_decode_bf16": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P, c_size_t, _P]),
+    "awq_b200_request_workspace_bytes": (c_size_t, []),
+    "awq_b200_request_check": (c_int, [_P, _P]),
+    "awq_b200_page_plan": (c_int, [_P, _P, _P, _L, c_int, _P, c_int] + [_P] * 3 + [c_int] + [_P] * 4 + [c_int, c_int, _P, c_size_t, _P]),
+    "awq_b200_rope_append": (c_int, [_P, _L, _L] * 3 + [_P, c_int, _P, _P, _P, _L, _L, _P, c_int, c_int, _P, c_size_t, _P]),
+    "awq_b200_tree_attention": (c_int, [_P, _L, _L, _P, _P, _L, c_int, _P, _P, _P, c_float, _P, _L, _L, c_int, c_int, c_int, _P, c_size_t, _P]),
+    "awq_b200_page_keep": (c_int, [_P] + [_L] * 5 + [c_int] * 5 + [_P, _L, c_int] + [_P] * 6 + [c_int, _P, _P, c_int, c_int, _P, c_size_t, _P]),
+    "awq_b200_lora_bf16": (c_int, [_P, _L, _P, _P, _P, _P, c_int, c_int, _P, _P, c_int, _P, _P, c_int, c_int, c_int, _P, c_size_t, _P]),
     "awq_b200_repack_B_to_A": (c_int, [_P] * 6 + [c_int, c_int, c_int, _P]),
     "awq_b200_repack_A_to_B": (c_int, [_P] * 6 + [c_int, c_int, c_int, _P]),
     "awq_b200_repack_C_to_B": (c_int, [_P] * 4 + [c_int, c_int, c_int, c_int, c_int, _P]),

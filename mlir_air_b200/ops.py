@@ -504,6 +504,272 @@ def rope_halfsplit(x, lut, n_heads: int, head_dim: int, out=None):
     return out
 
 
+# ---- many requests: paged cache, drafted tokens, adapters -----------------------------------------------------------------
+def _on(t: torch.Tensor, name: str, dtype, device: int, dim: int = 1):
+    """`t` as an argument on `device`: its type, its dimensions, its values side by side."""
+    if t.dtype != dtype or t.dim() != dim or t.get_device() != device:
+        raise _lib.AwqBackendError(f"{name} must be a {dim}-dimensional {dtype} tensor on cuda:{device}, got {t.dim()} dimensions of {t.dtype} "
+                                   f"on {t.device}")
+    if not t.is_contiguous():
+        raise _lib.AwqBackendError(f"{name} must be contiguous")
+    return t.data_ptr()
+
+
+def _numel(t: torch.Tensor, name: str, n: int, at_least=False):
+    if t.numel() < n or (t.numel() > n and not at_least):
+        raise _lib.AwqBackendError(f"{name} must have {'at least ' if at_least else ''}{n} elements, got {t.numel()}")
+
+
+def _call_on(device: int, name: str, *args):
+    """The call on `device`'s current stream, whichever device is the current one."""
+    if device == _device():
+        return _lib.call(name, *args, _raw_stream(device))
+    with torch.cuda.device(device):
+        return _lib.call(name, *args, _raw_stream(device))
+
+
+class RequestWorkspace:
+    """Scratch and error word of the operators on many requests' rows (`page_plan`, `rope_append`, `tree_attention`, `page_keep`,
+    `lora`); one size serves them all.  One per stream: calls that share it must not overlap on the GPU, nor may graphs
+    captured with it."""
+
+    def __init__(self, device="cuda"):
+        self.nbytes = int(_lib.load().awq_b200_request_workspace_bytes())
+        self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
+        if not self.buf.is_cuda:
+            raise _lib.AwqBackendError("RequestWorkspace needs a CUDA device")
+        self.ptr, self.device = self.buf.data_ptr(), self.buf.get_device()
+        _call_on(self.device, "awq_b200_workspace_init", self.ptr, self.nbytes)
+
+    def check(self):
+        """Synchronise and raise if a call since the last check met a length, page, slot, path or adapter outside its buffers."""
+        _call_on(self.device, "awq_b200_request_check", self.ptr)
+
+
+class KVCache:
+    """K and V of one layer in pages: [n_pages, page_size, n_kv_heads, head_dim] each, bf16 or fp16.  Views with other strides
+    (heads in front of slots, K and V in one tensor) are fine as long as a head's values lie side by side and all strides are
+    multiples of 8 elements.  Checked once, here; keeps the tensors alive."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        for name, t in (("k", k), ("v", v)):
+            if not t.is_cuda or t.dtype not in (torch.bfloat16, torch.float16) or t.dim() != 4:
+                raise _lib.AwqBackendError(f"KVCache: {name} must be a bf16 or fp16 CUDA tensor [n_pages, page_size, n_kv_heads, head_dim]")
+            if t.numel() == 0 or t.stride(3) != 1 or any(t.stride(i) % 8 or t.stride(i) <= 0 for i in range(3) if t.shape[i] > 1):
+                raise _lib.AwqBackendError(f"KVCache: {name} needs elements, a unit stride over head_dim and positive multiples of 8 elsewhere")
+        if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device:
+            raise _lib.AwqBackendError("KVCache: k and v must have the same shape, type and device")
+        self.k, self.v, self.dtype, self.device = k, v, k.dtype, k.get_device()
+        self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = k.shape
+        if self.n_pages * self.page_size > 0x7fffffff:
+            raise _lib.AwqBackendError("KVCache: more than 2^31 - 1 slots")
+        if self.head_dim % 16 or self.head_dim > 256:
+            raise _lib.AwqBackendError(f"KVCache: head_dim must be a multiple of 16, at most 256, got {self.head_dim}")
+        if not _aligned16(k, v):
+            raise _lib.AwqBackendError("KVCache: k and v must be 16-byte aligned")
+        strides = [t.stride(i) if t.shape[i] > 1 else 0 for t in (k, v) for i in range(3)]
+        self._struct = _lib.KvCacheStruct(k.data_ptr(), v.data_ptr(), *strides, self.n_pages, self.page_size, self.n_kv_heads, self.head_dim,
+                                          ACT_F16 if k.dtype == torch.float16 else ACT_BF16)
+        self.ptr = _lib.address_of(self._struct)
+
+    def rows(self, t: torch.Tensor, name: str, n_heads=None, rows=None):
+        """Checks [T, heads, head_dim] rows that go with the cache (column slices of a wider projection are fine)."""
+        if t.dim() != 3 or t.dtype != self.dtype or t.get_device() != self.device or t.shape[2] != self.head_dim or t.stride(2) != 1:
+            raise _lib.AwqBackendError(f"{name} must be [T, heads, {self.head_dim}] of {self.dtype} on cuda:{self.device} with unit stride over head_dim, "
+                                       f"got {tuple(t.shape)} of {t.dtype} on {t.device}")
+        if (n_heads is not None and t.shape[1] != n_heads) or (rows is not None and t.shape[0] != rows):
+            raise _lib.AwqBackendError(f"{name} must be [{rows}, {n_heads}, {self.head_dim}], got {tuple(t.shape)}")
+        # the stride of a dimension of one is arbitrary and never used
+        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
+
+
+@dataclass
+class StepPlan:
+    """The rows of one step, from `page_plan`: q_start int32 [R + 1], slots and positions int32 [T], mask int64 [T] or None."""
+    q_start: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    mask: Optional[torch.Tensor] = None
+
+
+def _table(table: torch.Tensor, R: int, device: int):
+    if table.dtype != torch.int32 or table.dim() != 2 or table.get_device() != device or table.shape[0] != R or \
+            (table.shape[1] > 1 and table.stride(1) != 1):
+        raise _lib.AwqBackendError(f"table must be int32 [{R}, width] on cuda:{device} with unit column stride, got {tuple(table.shape)} of {table.dtype}")
+    return table.data_ptr(), table.stride(0) if R > 1 else table.shape[1], table.shape[1]
+
+
+def page_plan(lens, new, table, free_pages, free_count, page_size: int, T: int, ws: RequestWorkspace, parents=None, free_count_out=None,
+              out: Optional[StepPlan] = None) -> StepPlan:
+    """Plan a step of `T` rows: every request r has lens[r] tokens in the cache and brings new[r] more.  Pages for them are popped
+    from `free_pages` (a stack of free_count[0] page numbers) into `table` int32 [R, width], request by request; the plan says
+    each row's request, slot and position and, with `parents` (int32, per row the index in its tree of the token it continues,
+    -1: the last cached one; at most 64 per request), the mask of its ancestors.  free_count is updated in place unless
+    free_count_out is given; lens stays: `page_keep` moves it on.  A step that does not fit changes nothing, has no rows, and
+    ws.check() says so; rows behind the last request get slot -1."""
+    dev, R = ws.device, lens.numel()
+    lens_p, new_p = _on(lens, "lens", torch.int32, dev), _on(new, "new", torch.int32, dev)
+    _numel(new, "new", R)
+    table_p, stride, width = _table(table, R, dev)
+    free_p, count_p = _on(free_pages, "free_pages", torch.int32, dev), _on(free_count, "free_count", torch.int32, dev)
+    _numel(free_count, "free_count", 1)
+    count_out = free_count if free_count_out is None else free_count_out
+    count_out_p = _on(count_out, "free_count_out", torch.int32, dev)
+    _numel(count_out, "free_count_out", 1)
+    if out is None:
+        i32 = dict(dtype=torch.int32, device=lens.device)
+        out = StepPlan(torch.empty(R + 1, **i32), torch.empty(T, **i32), torch.empty(T, **i32),
+                       None if parents is None else torch.empty(T, dtype=torch.int64, device=lens.device))
+    parents_p = mask_p = None
+    if parents is not None:
+        parents_p = _on(parents, "parents", torch.int32, dev)
+        _numel(parents, "parents", T)
+        if out.mask is None:
+            raise _lib.AwqBackendError("page_plan: parents need a mask in `out`")
+        mask_p = _on(out.mask, "out.mask", torch.int64, dev)
+        _numel(out.mask, "out.mask", T)
+    elif out.mask is not None:
+        raise _lib.AwqBackendError("page_plan: a mask in `out` needs parents")
+    start_p, slots_p, pos_p = (_on(t, n, torch.int32, dev) for t, n in (
+        (out.q_start, "out.q_start"), (out.slots, "out.slots"), (out.positions, "out.positions")))
+    _numel(out.q_start, "out.q_start", R + 1)
+    _numel(out.slots, "out.slots", T)
+    _numel(out.positions, "out.positions", T)
+    _call_on(dev, "awq_b200_page_plan", lens_p, new_p, table_p, stride, width, free_p, free_pages.numel(), count_p, count_out_p, parents_p,
+             int(page_size), start_p, slots_p, pos_p, mask_p, R, T, ws.ptr, ws.nbytes)
+    return out
+
+
+def rope_append(q, k, v, lut, positions, slots, cache: KVCache, ws: RequestWorkspace, q_out=None):
+    """Half-split RoPE of q [T, n_heads, head_dim] (in place, or into q_out) and k [T, n_kv_heads, head_dim] by the rows
+    positions[t] of lut bf16 [n_positions, head_dim] ([cos | sin], as for `rope_halfsplit`), and k and v written to slot
+    slots[t] of the cache: one launch.  A row with slot -1 is left out; of rows that name one slot the last one stays there."""
+    dev = cache.device
+    if ws.device != dev:
+        raise _lib.AwqBackendError("rope_append: workspace and cache must be on one device")
+    T = q.shape[0]
+    qp, qr, qh = cache.rows(q, "q")
+    H = q.shape[1]
+    kp, kr, kh = cache.rows(k, "k", cache.n_kv_heads, T)
+    vp, vr, vh = cache.rows(v, "v", cache.n_kv_heads, T)
+    op, orow, oh = (qp, qr, qh) if q_out is None else cache.rows(q_out, "q_out", H, T)
+    lut_p = _on(lut, "lut", torch.bfloat16, dev, 2)
+    if lut.shape[1] != cache.head_dim or lut.shape[0] == 0:
+        raise _lib.AwqBackendError(f"lut must be [positions, {cache.head_dim}], got {tuple(lut.shape)}")
+    pos_p, slots_p = _on(positions, "positions", torch.int32, dev), _on(slots, "slots", torch.int32, dev)
+    _numel(positions, "positions", T)
+    _numel(slots, "slots", T)
+    _call_on(dev, "awq_b200_rope_append", qp, qr, qh, kp, kr, kh, vp, vr, vh, lut_p, lut.shape[0], pos_p, slots_p, op, orow, oh, cache.ptr, T, H,
+             ws.ptr, ws.nbytes)
+    return q if q_out is None else q_out
+
+
+def tree_attention(q, cache: KVCache, table, lens, q_start, ws: RequestWorkspace, mask=None, scale: Optional[float] = None, out=None):
+    """out [T, n_heads, head_dim]: the step's rows q against their requests' cached tokens and the step's own (whose K and V
+    are in the cache already: `rope_append`).  Row t of request r sees its lens[r] cached tokens and token j of the step if bit
+    j of mask[t] (int64) is set, or without `mask` the tokens up to itself.  A row that sees nothing is 0.  Rows behind
+    q_start[R] are left as they are in a given `out`, 0 in a new one.  scale: head_dim ** -0.5 unless given."""
+    dev = cache.device
+    if ws.device != dev:
+        raise _lib.AwqBackendError("tree_attention: workspace and cache must be on one device")
+    qp, qr, qh = cache.rows(q, "q")
+    T, H = q.shape[0], q.shape[1]
+    if out is None:
+        out = torch.zeros((T, H, cache.head_dim), dtype=cache.dtype, device=q.device)
+    op, orow, oh = cache.rows(out, "out", H, T)
+    R = lens.numel()
+    lens_p, start_p = _on(lens, "lens", torch.int32, dev), _on(q_start, "q_start", torch.int32, dev)
+    _numel(q_start, "q_start", R + 1)
+    table_p, stride, width = _table(table, R, dev)
+    mask_p = None
+    if mask is not None:
+        mask_p = _on(mask, "mask", torch.int64, dev)
+        _numel(mask, "mask", T)
+    _call_on(dev, "awq_b200_tree_attention", qp, qr, qh, cache.ptr, table_p, stride, width, lens_p, start_p, mask_p,
+             cache.head_dim ** -0.5 if scale is None else float(scale), op, orow, oh, R, T, H, ws.ptr, ws.nbytes)
+    return out
+
+
+def page_keep(kv, table, lens, q_start, kept, free_pages, free_count, ws: RequestWorkspace, path=None, lens_out=None, free_count_out=None):
+    """After a step: keep kept[r] of request r's tokens.  In every layer of kv [layers, 2, n_pages, page_size, n_kv_heads, head_dim] the
+    rows path[q_start[r] + i] (indices in its tree, ascending; without `path` the first kept[r]) move to lens[r] + i; lens grows
+    by kept and the pages behind it go back to `free_pages` (in place unless lens_out / free_count_out are given).
+    kept[r] = -1 ends the request: length 0, all its pages free."""
+    dev, R = ws.device, lens.numel()
+    if kv.dim() != 6 or kv.shape[1] != 2 or kv.element_size() != 2 or kv.get_device() != dev or kv.numel() == 0:
+        raise _lib.AwqBackendError(f"kv must be [layers, 2, n_pages, page_size, n_kv_heads, head_dim] of 16-bit values on cuda:{dev}, got "
+                                   f"{tuple(kv.shape)} of {kv.dtype} on {kv.device}")
+    strides = [kv.stride(i) if kv.shape[i] > 1 else 0 for i in range(5)]
+    if kv.stride(5) != 1 or any(s % 8 or (s <= 0 and kv.shape[i] > 1) for i, s in enumerate(strides)):
+        raise _lib.AwqBackendError("kv needs a unit stride over head_dim and positive multiples of 8 elsewhere")
+    table_p, stride, width = _table(table, R, dev)
+    lens_out = lens if lens_out is None else lens_out
+    count_out = free_count if free_count_out is None else free_count_out
+    lens_p, lens_out_p, start_p, kept_p, free_p, count_p, count_out_p = (_on(t, n, torch.int32, dev) for t, n in (
+        (lens, "lens"), (lens_out, "lens_out"), (q_start, "q_start"), (kept, "kept"), (free_pages, "free_pages"), (free_count, "free_count"),
+        (count_out, "free_count_out")))
+    for t, n, k in ((lens_out, "lens_out", R), (q_start, "q_start", R + 1), (kept, "kept", R), (free_count, "free_count", 1),
+                    (count_out, "free_count_out", 1)):
+        _numel(t, n, k)
+    path_p, T = None, _lib.MAX_ROWS
+    if path is not None:
+        path_p, T = _on(path, "path", torch.int32, dev), path.numel()
+    _call_on(dev, "awq_b200_page_keep", kv.data_ptr(), *strides, kv.shape[0], kv.shape[2], kv.shape[3], kv.shape[4], kv.shape[5], table_p, stride,
+             width, lens_p, lens_out_p, start_p, kept_p, path_p, free_p, free_pages.numel(), count_p, count_out_p, R, T, ws.ptr, ws.nbytes)
+    return lens_out
+
+
+class LoraAdapters:
+    """Low-rank adapters of one projection [K, N], resident: A bf16 [n, rank_max, K], B bf16 [n, N, rank_max] (the two matrices of
+    each adapter as they are trained), scales f32 [n], ranks int32 [n] or None: how many rows of A and columns of B an
+    adapter has; what lies behind them is not read."""
+
+    def __init__(self, A: torch.Tensor, B: torch.Tensor, scales: torch.Tensor, ranks: Optional[torch.Tensor] = None):
+        if not A.is_cuda or A.dim() != 3 or B.dim() != 3:
+            raise _lib.AwqBackendError("LoraAdapters: A [n, rank_max, K] and B [n, N, rank_max] must be CUDA tensors")
+        self.device = A.get_device()
+        self.n, self.rank_max, self.K = A.shape
+        self.N = B.shape[1]
+        if tuple(B.shape) != (self.n, self.N, self.rank_max):
+            raise _lib.AwqBackendError(f"LoraAdapters: B must be [{self.n}, N, {self.rank_max}], got {tuple(B.shape)}")
+        if self.rank_max % 8 or not 0 < self.rank_max <= 128 or self.K % 8 or self.N % 8:
+            raise _lib.AwqBackendError(f"LoraAdapters: rank_max must be a multiple of 8 up to 128, K and N multiples of 8, got {self.rank_max}, {self.K}, "
+                                       f"{self.N}")
+        self.A, self.B, self.scales, self.ranks = A, B, scales, ranks
+        self._ptrs = (_on(A, "A", torch.bfloat16, self.device, 3), _on(B, "B", torch.bfloat16, self.device, 3),
+                      _on(scales, "scales", torch.float32, self.device), None if ranks is None else _on(ranks, "ranks", torch.int32, self.device))
+        _numel(scales, "scales", self.n)
+        if ranks is not None:
+            _numel(ranks, "ranks", self.n)
+        if not _aligned16(A, B):
+            raise _lib.AwqBackendError("LoraAdapters: A and B must be 16-byte aligned")
+
+
+def lora(x, adapters: LoraAdapters, idx, base, ws: RequestWorkspace, out=None, residual=None):
+    """out bf16 [T, N] = bf16(base + scale (x A^T) B^T (+ residual)) with adapter idx[t] for row t of x bf16 [T, K], -1: none.  base is
+    the shared projection's output, f32 sums (`gemv(..., f32_out=True)`) or bf16; out may be a bf16 base."""
+    dev = ws.device
+    if adapters.device != dev:
+        raise _lib.AwqBackendError("lora: workspace and adapters must be on one device")
+    if x.dtype != torch.bfloat16 or x.dim() != 2 or x.get_device() != dev or x.shape[1] != adapters.K or x.stride(1) != 1:
+        raise _lib.AwqBackendError(f"x must be bf16 [T, {adapters.K}] on cuda:{dev} with unit column stride, got {tuple(x.shape)} of {x.dtype} on {x.device}")
+    T = x.shape[0]
+    shape = (T, adapters.N)
+    idx_p = _on(idx, "idx", torch.int32, dev)
+    _numel(idx, "idx", T)
+    f32 = base.dtype == torch.float32
+    base_p = _on(base, "base", torch.float32 if f32 else torch.bfloat16, dev, 2)
+    if out is None:
+        out = torch.empty(shape, dtype=torch.bfloat16, device=x.device)
+    out_p = _on(out, "out", torch.bfloat16, dev, 2)
+    res_p = None if residual is None else _on(residual, "residual", torch.bfloat16, dev, 2)
+    if base.shape != shape or out.shape != shape or (residual is not None and residual.shape != shape):
+        raise _lib.AwqBackendError(f"base, out and residual must be {list(shape)}")
+    _call_on(dev, "awq_b200_lora_bf16", x.data_ptr(), x.stride(0) if T > 1 else 0, *adapters._ptrs, adapters.n, adapters.rank_max, idx_p, base_p,
+             1 if f32 else 0, res_p, out_p, T, adapters.K, adapters.N, ws.ptr, ws.nbytes)
+    return out
+
+
 def linear_bf16(x, W, out=None):
     """y [M, N] = x [M, K] @ W[N, K]^T with un-quantised bf16 weights (the bf16 sibling path)."""
     _want(x, torch.bfloat16, "x")
