@@ -62,7 +62,7 @@ struct PlanArgs {
     const int32_t *free_pages, *count, *parents;
     int32_t *count_out, *q_start, *slots, *positions;
     long long *mask;
-    int R, T, table_width, pool, page;
+    int R, T, table_width, pool, page, max_pages;  // max_pages: as many as int32 slots can number
     RequestHeader *header;
 };
 
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(PlanArgs a) {
     for (int k = me; k < (int)all_need; k += step) {
         const int r = request_of_row(first, a.R, k);
         int page = a.free_pages[count - 1 - k];
-        if ((unsigned)page >= (unsigned)a.pool) {
+        if ((unsigned)page >= (unsigned)a.max_pages) {
             req_error(&a.header->error, REQ_ERR_PAGE);
             page = -1;
         }
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(PlanArgs a) {
         const int at = len + j, block = at / a.page, held = (len + a.page - 1) / a.page;
         // a new page is not read from the table, which another CTA may not have written yet
         int page = block < held ? a.table[r * a.table_stride + block] : a.free_pages[count - 1 - (first[r] + block - held)];
-        if ((unsigned)page >= (unsigned)a.pool) {
+        if ((unsigned)page >= (unsigned)a.max_pages) {
             req_error(&a.header->error, REQ_ERR_PAGE);
             page = -1;
         }
@@ -429,7 +429,7 @@ extern "C" int awq_b200_page_plan(const int32_t *lens, const int32_t *fresh, int
     AWQ_REQUIRE((parents == nullptr) == (mask == nullptr), "page_plan: parents and mask go together");
     AWQ_REQUIRE_REQUEST_WORKSPACE("page_plan", workspace, workspace_bytes);
     PlanArgs a{lens, fresh, table, table_stride, free_pages, free_count, parents, free_count_out, q_start, slots, positions, mask, R, T,
-               table_width, pool, page_size, request_workspace(workspace).header};
+               table_width, pool, page_size, 0x7fffffff / page_size, request_workspace(workspace).header};
     const int grid = max(1, min((T + PLAN_THREADS - 1) / PLAN_THREADS, device_sm_count()));
     return check_cuda(launch_pdl(page_plan_kernel, dim3(grid), dim3(PLAN_THREADS), (size_t)(2 * R + 2) * 4, as_stream(stream), a), "page_plan launch");
 }

@@ -115,7 +115,402 @@ __global__ void __launch_bounds__(128) tree_attention_any_kernel(AttendArgs a) {
     }
 }
 
-size_t tree_attention_scratch_bytes() { return 0; }
+// =====================================================================================
+// Few rows per cache head (one token, small trees): bound by the cache's bytes.
+//
+// A unit of work is a tile of keys of a segment = (request, cache head, 16 rows); rows are (token, head of the group) pairs,
+// padded to the 16 rows of one mma.sync.  The CTAs split the units of all segments evenly (stream-K), whatever the lengths;
+// a segment that several CTAs share is joined by the last of them to finish, in the order of its keys, so no CTA waits and
+// results do not depend on timing.
+//
+// Inside a tile every warp has 16 keys of its own and keeps its own running maximum and sum.  K and V go from global memory to
+// the registers in which mma.sync wants them, without shared memory:
+//   scores: the order of the products over the head is free, so a lane's 16 bytes of a key are its operands of two k-steps
+//           if the rows of Q are taken in the same order;
+//   output: a lane loads 16 bytes of four keys (its k-indices) and pairs them up with byte permutes; column n of block j is
+//           then head element 8 n + j, so that a lane's results are 16 neighbours.
+// Weights are multiplied as two 16-bit pieces, p = hi + lo: the tensor cores have time to spare, and the result keeps the
+// accuracy of f32 weights.
+// =====================================================================================
+constexpr int AR_WARPS = 4, AR_TILE = AR_WARPS * 16, AR_PER_SM = 3, AR_ROWS = 16;
+constexpr int AR_MAX_CTAS = 192 * AR_PER_SM;
+
+__device__ __forceinline__ uint4 ldg_stream(const uint16_t *p, bool on) {
+    uint4 v;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+        "@p ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+        : "l"(p), "r"((int)on));
+    return v;
+}
+template <bool F16>
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if (F16)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        mma_bf16_16816(d, a0, a1, a2, a3, b0, b1);
+}
+template <bool F16>
+__device__ __forceinline__ bool not_finite16x2(uint32_t v) {
+    constexpr uint32_t e = F16 ? 0x7c00u : 0x7f80u;
+    return (v & e) == e || ((v >> 16) & e) == e;
+}
+
+// Tiles of all requests before each one, in shared memory; returns their number.  Requests that do not fit are reported by
+// CTA 0 and have what attend_request leaves of them.
+template <int THREADS>
+__device__ __forceinline__ long long scan_units(const AttendArgs &a, long long *cum, int rows_per_segment, int tile) {
+    __shared__ long long sums[THREADS / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = a.n_heads / a.cache.n_kv;
+    const int per = (a.R + THREADS - 1) / THREADS, r0 = min(tid * per, a.R), r1 = min(r0 + per, a.R);
+    long long mine = 0;
+    for (int r = r0; r < r1; ++r) {
+        const AttendRequest q = attend_request(a, r);
+        if (q.bad && blockIdx.x == 0) req_error(&a.header->error, REQ_ERR_REQUEST);
+        const long long units = (((long long)q.n * group + rows_per_segment - 1) / rows_per_segment) * a.cache.n_kv * ((q.len + q.n + tile - 1) / tile);
+        cum[r] = units;
+        mine += units;
+    }
+    long long incl = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += u;
+    }
+    if (lane == 31) sums[warp] = incl;
+    __syncthreads();
+    long long base = incl - mine, total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) base += sums[w];
+        total += sums[w];
+    }
+    for (int r = r0; r < r1; ++r) {
+        const long long u = cum[r];
+        cum[r] = base;
+        base += u;
+    }
+    if (tid == 0) cum[a.R] = total;
+    __syncthreads();
+    return total;
+}
+__device__ __forceinline__ int request_of_unit(const long long *cum, int n, long long x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (cum[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+
+// Shared memory: cum | Q in operand order | key offsets | the warps' results
+template <int D>
+constexpr int AR_SMEM = D * 32 + AR_WARPS * 2 * 16 * 16 + AR_WARPS * AR_ROWS * (D + 2) * 4;
+
+template <bool F16, int D>
+__global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_kernel(AttendArgs a, int min_units) {
+    constexpr int THREADS = AR_WARPS * 32, QC = D / 32, VC = D / 64;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    uint4 *qs = reinterpret_cast<uint4 *>(smem);                                     // [QC][2][32]
+    longlong2 *offs = reinterpret_cast<longlong2 *>(smem + D * 32) + warp * 32;       // [2][16] of this warp
+    float *ow = reinterpret_cast<float *>(smem + D * 32 + AR_WARPS * 512);            // [WARPS][16][D]
+    float *mw = ow + AR_WARPS * AR_ROWS * D, *lw = mw + AR_WARPS * AR_ROWS;            // [WARPS][16]
+    long long *cum = reinterpret_cast<long long *>(smem + AR_SMEM<D>);
+    __shared__ int s_last;
+    pdl_wait();
+    pdl_launch_dependents();
+    const long long units = scan_units<THREADS>(a, cum, AR_ROWS, AR_TILE);
+    const long long per = max((units + gridDim.x - 1) / gridDim.x, (long long)min_units);
+    long long x = blockIdx.x * per;
+    const long long end = min(x + per, units);
+    const int group = a.n_heads / a.cache.n_kv, page_size = a.cache.page_size;
+    float *parts = reinterpret_cast<float *>(a.scratch + 4 * AR_MAX_CTAS);
+    int *counters = reinterpret_cast<int *>(a.scratch);
+    constexpr int PART = AR_ROWS * (D + 2);
+
+    while (x < end) {
+        const int r = request_of_unit(cum, a.R, x);
+        const AttendRequest rq = attend_request(a, r);
+        const int total = rq.len + rq.n, n_tiles = (total + AR_TILE - 1) / AR_TILE, m_tiles = (rq.n * group + AR_ROWS - 1) / AR_ROWS;
+        const long long rem = x - cum[r];
+        const int seg = (int)(rem / n_tiles), tile0 = (int)(rem % n_tiles), hk = seg / m_tiles, row0 = (seg % m_tiles) * AR_ROWS;
+        const long long seg_start = x - tile0, seg_end = seg_start + n_tiles;
+        const int tiles = (int)(min(end, seg_end) - x);
+        const int32_t *table = a.table + r * a.table_stride;
+        const uint16_t *kbase = a.cache.k + hk * a.cache.k_head, *vbase = a.cache.v + hk * a.cache.v_head;
+        // this lane's rows, g and g + 8: token and mask
+        int j[2];
+        unsigned long long bits[2];
+        const uint16_t *qrow[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = row0 + g + 8 * i;
+            j[i] = row < rq.n * group ? row / group : -1;
+            bits[i] = a.mask && j[i] >= 0 ? (unsigned long long)a.mask[rq.q0 + j[i]] : 0;
+            qrow[i] = a.q + (long long)(rq.q0 + max(j[i], 0)) * a.q_row + (long long)(hk * group + row % group) * a.q_head;
+        }
+        __syncthreads();  // the previous segment's readers of shared memory are done
+        for (int c = warp; c < QC; c += AR_WARPS)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                qs[(c * 2 + i) * 32 + lane] = j[i] >= 0 ? *reinterpret_cast<const uint4 *>(qrow[i] + 32 * c + 8 * t4) : make_uint4(0, 0, 0, 0);
+        __syncthreads();
+
+        float acc[VC][8][4];
+#pragma unroll
+        for (int c = 0; c < VC; ++c)
+#pragma unroll
+            for (int b = 0; b < 8; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[c][b][e] = 0.f;
+        float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+
+        // lane l < 16 looks after key l of a block: its page, then its place in K and V
+        const int first = tile0 * AR_TILE + warp * 16;
+        auto page_of = [&](int i) {
+            const int key = first + i * AR_TILE + lane;
+            return lane < 16 && i < tiles && key < total ? __ldg(table + key / page_size) : -1;
+        };
+        auto place = [&](int i, int page) {  // returns the block's valid keys
+            const int key = first + i * AR_TILE + lane;
+            bool ok = false;
+            if (lane < 16) {
+                const int off = key % page_size;
+                ok = (unsigned)page < (unsigned)a.cache.n_pages;
+                if (!ok && i < tiles && key < total) req_error(&a.header->error, REQ_ERR_PAGE);
+                offs[(i & 1) * 16 + lane] = ok ? make_longlong2(page * a.cache.k_page + off * a.cache.k_slot, page * a.cache.v_page + off * a.cache.v_slot)
+                                               : make_longlong2(-1, -1);
+            }
+            __syncwarp();
+            return __ballot_sync(0xffffffffu, ok) & 0xffffu;
+        };
+        uint4 kr[2][QC], vr[VC][4];
+        auto load_k = [&](int i) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const long long o = offs[(i & 1) * 16 + 8 * b + g].x;
+#pragma unroll
+                for (int c = 0; c < QC; ++c) kr[b][c] = ldg_stream(kbase + o + 32 * c + 8 * t4, o >= 0);
+            }
+        };
+        auto load_v = [&](int i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const long long o = offs[(i & 1) * 16 + 2 * t4 + (e & 1) + 8 * (e >> 1)].y;
+#pragma unroll
+                for (int c = 0; c < VC; ++c) vr[c][e] = ldg_stream(vbase + o + 64 * c + 8 * g, o >= 0);
+            }
+        };
+        uint32_t valid = place(0, page_of(0));
+        load_k(0);
+        load_v(0);
+        int next_page = page_of(1);
+        for (int i = 0; i < tiles; ++i) {
+            const int page2 = page_of(i + 2);
+            float s[2][4] = {};
+#pragma unroll
+            for (int c = 0; c < QC; ++c) {
+                const uint4 q0 = qs[(c * 2) * 32 + lane], q1 = qs[(c * 2 + 1) * 32 + lane];
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    mma16<F16>(s[b], q0.x, q1.x, q0.y, q1.y, kr[b][c].x, kr[b][c].y);
+                    mma16<F16>(s[b], q0.z, q1.z, q0.w, q1.w, kr[b][c].z, kr[b][c].w);
+                }
+            }
+            const uint32_t valid_next = place(i + 1, next_page);
+            next_page = page2;
+            load_k(i + 1);
+            const int key0 = first + i * AR_TILE;
+            const bool partly = key0 + 16 > rq.len || valid != 0xffffu;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[b][e] *= a.scale_log2;
+                    if (partly) {
+                        const int c = 8 * b + 2 * t4 + (e & 1), d = key0 + c - rq.len;
+                        const bool seen = (valid >> c & 1) && (d < 0 || (a.mask ? d < 64 && (bits[e >> 1] >> d & 1) : d <= j[e >> 1]));
+                        if (!seen) s[b][e] = -INFINITY;
+                    }
+                }
+            float p[2][4];
+#pragma unroll
+            for (int i2 = 0; i2 < 2; ++i2) {
+                float m = fmaxf(fmaxf(s[0][2 * i2], s[0][2 * i2 + 1]), fmaxf(s[1][2 * i2], s[1][2 * i2 + 1]));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                m = fmaxf(m, top[i2]);
+                const float ref = m == -INFINITY ? 0.f : m, keep = exp2f(top[i2] - ref);
+                top[i2] = m;
+                float add = 0.f;
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) add += p[b][2 * i2 + e] = exp2f(s[b][2 * i2 + e] - ref);
+                sum[i2] = sum[i2] * keep + add;
+                if (__any_sync(0xffffffffu, keep != 1.f)) {
+#pragma unroll
+                    for (int c = 0; c < VC; ++c)
+#pragma unroll
+                        for (int b = 0; b < 8; ++b) acc[c][b][2 * i2] *= keep, acc[c][b][2 * i2 + 1] *= keep;
+                }
+            }
+            // a value that some rows do not see must not reach them as 0 times infinity or NaN
+            if (partly) {
+                bool odd = false;
+#pragma unroll
+                for (int c = 0; c < VC; ++c)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        odd = odd || not_finite16x2<F16>(vr[c][e].x) || not_finite16x2<F16>(vr[c][e].y) || not_finite16x2<F16>(vr[c][e].z) ||
+                              not_finite16x2<F16>(vr[c][e].w);
+                if (__any_sync(0xffffffffu, odd)) {
+                    for (int key = 0; key < 16; ++key) {
+                        const long long o = offs[(i & 1) * 16 + key].y;
+                        if (o < 0) continue;  // (loaded as zero)
+                        // the weights of rows g and g + 8 for this key
+                        float w[2];
+#pragma unroll
+                        for (int i2 = 0; i2 < 2; ++i2) {
+                            const float w0 = __shfl_sync(0xffffffffu, p[0][2 * i2], (lane & 28) + ((key & 7) >> 1)), w1 = __shfl_sync(0xffffffffu, p[0][2 * i2 + 1], (lane & 28) + ((key & 7) >> 1));
+                            const float w2 = __shfl_sync(0xffffffffu, p[1][2 * i2], (lane & 28) + ((key & 7) >> 1)), w3 = __shfl_sync(0xffffffffu, p[1][2 * i2 + 1], (lane & 28) + ((key & 7) >> 1));
+                            w[i2] = key < 8 ? (key & 1 ? w1 : w0) : (key & 1 ? w3 : w2);
+                        }
+#pragma unroll
+                        for (int c = 0; c < VC; ++c)
+                            for (int d = 0; d < 16; ++d) {
+                                const uint32_t bitsv = (vbase + o)[64 * c + 16 * t4 + d];
+                                if (!not_finite16x2<F16>(bitsv)) continue;
+                                const float v = unpack16x2<F16>(bitsv).x;
+#pragma unroll
+                                for (int b = 0; b < 8; ++b)
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e)
+                                        if (d == 8 * (e & 1) + b && w[e >> 1] != 0.f) acc[c][b][e] += w[e >> 1] * v;
+                            }
+                    }
+                    auto clean = [](uint32_t v) {
+                        if (not_finite16x2<F16>(v & 0xffffu)) v &= 0xffff0000u;
+                        if (not_finite16x2<F16>(v >> 16)) v &= 0xffffu;
+                        return v;
+                    };
+#pragma unroll
+                    for (int c = 0; c < VC; ++c)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            vr[c][e] = make_uint4(clean(vr[c][e].x), clean(vr[c][e].y), clean(vr[c][e].z), clean(vr[c][e].w));
+                }
+            }
+            uint32_t hi[4], lo[4];  // rows g, g + 8 of keys 0-7, then of keys 8-15
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int i2 = 0; i2 < 2; ++i2) {
+                    const float p0 = p[b][2 * i2], p1 = p[b][2 * i2 + 1];
+                    hi[2 * b + i2] = pack16x2<F16>(p0, p1);
+                    const float2 h = unpack16x2<F16>(hi[2 * b + i2]);
+                    lo[2 * b + i2] = pack16x2<F16>(p0 - h.x, p1 - h.y);
+                }
+#pragma unroll
+            for (int c = 0; c < VC; ++c) {
+                const uint32_t v[4][4] = {{vr[c][0].x, vr[c][0].y, vr[c][0].z, vr[c][0].w}, {vr[c][1].x, vr[c][1].y, vr[c][1].z, vr[c][1].w},
+                                          {vr[c][2].x, vr[c][2].y, vr[c][2].z, vr[c][2].w}, {vr[c][3].x, vr[c][3].y, vr[c][3].z, vr[c][3].w}};
+#pragma unroll
+                for (int b = 0; b < 8; ++b) {
+                    const uint32_t sel = b & 1 ? 0x7632u : 0x5410u;
+                    const uint32_t b0 = __byte_perm(v[0][b >> 1], v[1][b >> 1], sel), b1 = __byte_perm(v[2][b >> 1], v[3][b >> 1], sel);
+                    mma16<F16>(acc[c][b], hi[0], hi[1], hi[2], hi[3], b0, b1);
+                    mma16<F16>(acc[c][b], lo[0], lo[1], lo[2], lo[3], b0, b1);
+                }
+            }
+            load_v(i + 1);
+            valid = valid_next;
+        }
+        // ---- join the warps ----
+#pragma unroll
+        for (int i2 = 0; i2 < 2; ++i2) {
+            sum[i2] += __shfl_xor_sync(0xffffffffu, sum[i2], 1);
+            sum[i2] += __shfl_xor_sync(0xffffffffu, sum[i2], 2);
+            const int row = g + 8 * i2;
+            if (t4 == 0) mw[warp * 16 + row] = top[i2], lw[warp * 16 + row] = sum[i2];
+#pragma unroll
+            for (int c = 0; c < VC; ++c)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float *o = ow + (warp * 16 + row) * D + 64 * c + 16 * t4 + 8 * e;
+                    *reinterpret_cast<float4 *>(o) = make_float4(acc[c][0][2 * i2 + e], acc[c][1][2 * i2 + e], acc[c][2][2 * i2 + e], acc[c][3][2 * i2 + e]);
+                    *reinterpret_cast<float4 *>(o + 4) = make_float4(acc[c][4][2 * i2 + e], acc[c][5][2 * i2 + e], acc[c][6][2 * i2 + e], acc[c][7][2 * i2 + e]);
+                }
+        }
+        __syncthreads();
+        const int c0 = (int)(seg_start / per), c1 = (int)((seg_end - 1) / per), rows = min(AR_ROWS, rq.n * group - row0);
+        const bool whole = c0 == c1;
+        float *part = parts + (long long)(2 * blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0)) * PART;
+        auto store = [&](int row, int d, const float (&o)[8], float total_w) {
+            const float inv = total_w == 0.f ? 0.f : 1.f / total_w;
+            uint16_t *dst = a.out + (long long)(rq.q0 + (row0 + row) / group) * a.o_row + (long long)(hk * group + (row0 + row) % group) * a.o_head + d;
+            *reinterpret_cast<uint4 *>(dst) = make_uint4(pack16x2<F16>(o[0] * inv, o[1] * inv), pack16x2<F16>(o[2] * inv, o[3] * inv),
+                                                         pack16x2<F16>(o[4] * inv, o[5] * inv), pack16x2<F16>(o[6] * inv, o[7] * inv));
+        };
+        for (int i = tid; i < rows * (D / 8); i += THREADS) {
+            const int row = i / (D / 8), d = 8 * (i % (D / 8));
+            float m = -INFINITY, l = 0.f, o[8] = {};
+#pragma unroll
+            for (int w = 0; w < AR_WARPS; ++w) m = fmaxf(m, mw[w * 16 + row]);
+#pragma unroll
+            for (int w = 0; w < AR_WARPS; ++w) {
+                const float mm = mw[w * 16 + row], f = mm == -INFINITY ? 0.f : exp2f(mm - m);
+                l += f * lw[w * 16 + row];
+                if (f == 0.f) continue;
+                const float4 u = *reinterpret_cast<const float4 *>(ow + (w * 16 + row) * D + d), v = *reinterpret_cast<const float4 *>(ow + (w * 16 + row) * D + d + 4);
+                o[0] += f * u.x, o[1] += f * u.y, o[2] += f * u.z, o[3] += f * u.w;
+                o[4] += f * v.x, o[5] += f * v.y, o[6] += f * v.z, o[7] += f * v.w;
+            }
+            if (whole) {
+                store(row, d, o, l);
+            } else {
+                *reinterpret_cast<float4 *>(part + row * D + d) = make_float4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<float4 *>(part + row * D + d + 4) = make_float4(o[4], o[5], o[6], o[7]);
+                if (d == 0) part[AR_ROWS * D + row] = m, part[AR_ROWS * D + AR_ROWS + row] = l;
+            }
+        }
+        if (!whole) {
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) s_last = atomicAdd(counters + c0, 1) == c1 - c0;
+            __syncthreads();
+            if (s_last) {
+                __threadfence();
+                for (int i = tid; i < rows * (D / 8); i += THREADS) {
+                    const int row = i / (D / 8), d = 8 * (i % (D / 8));
+                    float m = -INFINITY, l = 0.f, o[8] = {};
+                    for (int c = c0; c <= c1; ++c) {
+                        const float *src = parts + (long long)(2 * c + (c == c0 ? 1 : 0)) * PART;
+                        const float mc = __ldcg(src + AR_ROWS * D + row), lc = __ldcg(src + AR_ROWS * D + AR_ROWS + row);
+                        const float4 u = __ldcg(reinterpret_cast<const float4 *>(src + row * D + d)), v = __ldcg(reinterpret_cast<const float4 *>(src + row * D + d + 4));
+                        const float m2 = fmaxf(m, mc);
+                        if (m2 == -INFINITY) continue;
+                        const float f = exp2f(m - m2), fc = exp2f(mc - m2);
+                        m = m2;
+                        l = l * f + lc * fc;
+                        const float add[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) o[e] = o[e] * f + (fc == 0.f ? 0.f : add[e] * fc);
+                    }
+                    store(row, d, o, l);
+                }
+                if (tid == 0) counters[c0] = 0;
+            }
+        }
+        x += tiles;
+    }
+}
+
+size_t tree_attention_scratch_bytes() { return 4 * AR_MAX_CTAS + (size_t)2 * AR_MAX_CTAS * AR_ROWS * (128 + 2) * 4; }
 
 }  // namespace awq
 
@@ -143,6 +538,15 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
     const RequestWorkspaceView w = request_workspace(workspace);
     AttendArgs a{reinterpret_cast<const uint16_t *>(q), s[0], s[1], view, table, table_stride, lens, q_start, mask,
                  reinterpret_cast<uint16_t *>(out), s[2], s[3], scale * 1.4426950408889634f, R, T, n_heads, table_width, w.header, w.attention};
+    if (view.head_dim == 64 || view.head_dim == 128) {
+        const bool f16 = cache->format == ACT_F16;
+        auto kernel = view.head_dim == 64 ? (f16 ? tree_attention_rows_kernel<true, 64> : tree_attention_rows_kernel<false, 64>)
+                                          : (f16 ? tree_attention_rows_kernel<true, 128> : tree_attention_rows_kernel<false, 128>);
+        const int smem = (view.head_dim == 64 ? AR_SMEM<64> : AR_SMEM<128>) + (R + 1) * 8;
+        if ((rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "tree_attention shared memory"))) return rc;
+        const int grid = min(device_sm_count() * AR_PER_SM, AR_MAX_CTAS);
+        return check_cuda(launch_pdl(kernel, dim3(grid), dim3(AR_WARPS * 32), smem, as_stream(stream), a, 1), "tree_attention launch");
+    }
     const long long items = (long long)T * n_heads;
     AWQ_REQUIRE((items + 3) / 4 <= 0x7fffffffLL, "tree_attention: too many rows and heads");
     auto kernel = cache->format == ACT_F16 ? tree_attention_any_kernel<true> : tree_attention_any_kernel<false>;

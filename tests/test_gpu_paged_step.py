@@ -116,7 +116,7 @@ def test_plan_reports_parents_and_pages_it_cannot_use():
         assert p.slots.tolist() == [3, 4, 5]
         with pytest.raises(AwqBackendError, match="parent"):
             ws.check()
-    for page in (-1, 2, 2 ** 31 - 1):
+    for page in (-1, 2 ** 27, 2 ** 31 - 1):  # 2^27 pages of 16 have no int32 slots
         p = ops.page_plan(i32([0]), i32([3]), i32([[-1, -1]]), i32([page, page]), i32([2]), 16, 3, ws)
         assert p.slots.tolist() == [-1] * 3
         with pytest.raises(AwqBackendError, match="page outside"):
