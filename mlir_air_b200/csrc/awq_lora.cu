@@ -3,11 +3,23 @@
 //   out[t] = bf16(base[t] + scale[a] (x[t] A[a]^T) B[a]^T (+ residual[t])),   a = idx[t], -1: none.
 //
 // A [n, rank_max, K] and B [n, N, rank_max] hold rank[a] rows / columns of each adapter; what lies behind them is not read.
+//
+// Rows are put together by adapter into tiles, so that an adapter is read once per tile and multiplied on the tensor cores
+// (mma.sync: the products are small, the bytes of x, base, out and the adapters are what takes time).  A row's result does not
+// depend on its tile or its place in it.  Operands go from global memory to registers in 16-byte pieces: the order of the
+// products along K (or the rank) is free as long as both operands have the same one, so eight neighbours of a row are a lane's
+// operands of two k-steps.  x A^T stays at f32's accuracy between the products: it is summed in f32 and multiplied as two
+// bf16 pieces (hi + lo, 2^-17).
 #include "awq_request.cuh"
 
+#include <cooperative_groups.h>
 #include <math.h>
 
 namespace awq {
+
+namespace cg = cooperative_groups;
+
+constexpr int LORA_MAX_ROWS = 65535, LORA_MAX_RANK = 128, LORA_MAX_ADAPTERS = 4096;
 
 struct LoraArgs {
     const uint16_t *x, *A, *B;
@@ -18,53 +30,444 @@ struct LoraArgs {
     uint16_t *out;
     long long x_row;
     int base_f32, T, K, N, n, rank_max;
-    float *low;  // [T, rank_max] x A^T
+    int splits;  // clusters that share a tile's columns (few rows)
     RequestHeader *header;
+    int32_t *order;   // [T] rows by adapter
+    int4 *tiles;      // adapter, first of `order`, rows, -
+    int32_t *n_tiles;
+    uint16_t *low;    // [T][2][rank_max up to 32] scale x A^T in the order of `order`, hi and lo
 };
 
-__global__ void __launch_bounds__(128) lora_down_kernel(LoraArgs a) {
-    pdl_wait();
-    pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int t = (int)(item / a.rank_max), r = (int)(item % a.rank_max);
-    if (t >= a.T) return;
+__device__ __forceinline__ int lora_rank(const LoraArgs &a, int ad) {
+    if (ad >= a.n) return 0;
+    return a.ranks ? min(max(a.ranks[ad], 0), a.rank_max) : a.rank_max;
+}
+// The adapter of a row; a.n: none.
+__device__ __forceinline__ int lora_adapter(const LoraArgs &a, int t, bool report) {
     const int ad = a.idx[t];
-    if (ad < 0 || ad >= a.n) {
-        if (ad >= a.n && lane == 0) req_error(&a.header->error, REQ_ERR_ADAPTER);
-        return;
-    }
-    const int rank = a.ranks ? min(max(a.ranks[ad], 0), a.rank_max) : a.rank_max;
-    if (r >= rank) return;
-    const uint16_t *x = a.x + t * a.x_row, *A = a.A + ((long long)ad * a.rank_max + r) * a.K;
-    float s = 0.f;
-    for (int k = lane; k < a.K; k += 32) s = fmaf(bf16_bits_to_f32(x[k]), bf16_bits_to_f32(A[k]), s);
+    if (ad >= a.n && report) req_error(&a.header->error, REQ_ERR_ADAPTER);
+    return (unsigned)ad < (unsigned)a.n ? ad : a.n;
+}
+__device__ __forceinline__ uint4 ldg16(const uint16_t *p, bool on) {
+    return on ? __ldg(reinterpret_cast<const uint4 *>(p)) : make_uint4(0, 0, 0, 0);
+}
+
+// acc[m][b] += x rows x (rank rows of A)^T over chunks first, first + step, ... < last of 32 columns of K.
+template <int MT, int NB>
+__device__ __forceinline__ void lora_down(float (&acc)[MT][NB][4], const uint16_t *const (&x)[MT][2], const uint16_t *A, int K, int rank, int r0,
+                                          int first, int last, int step, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll 2
+    for (int c = first; c < last; c += step) {
+        const int k = 32 * c + 8 * t;
+        uint4 xv[MT][2], av[NB];
 #pragma unroll
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    if (lane == 0) a.low[(long long)t * a.rank_max + r] = s * a.scales[ad];
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) xv[m][i] = ldg16(x[m][i] + k, x[m][i] != nullptr && k < K);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) av[b] = ldg16(A + (long long)(r0 + 8 * b + g) * K + k, r0 + 8 * b + g < rank && k < K);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
+                mma_bf16_16816(acc[m][b], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, av[b].x, av[b].y);
+                mma_bf16_16816(acc[m][b], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, av[b].z, av[b].w);
+            }
+    }
 }
 
-__global__ void __launch_bounds__(128) lora_up_kernel(LoraArgs a) {
+// Eight columns of B from rank column r on; columns from `rank` on are zero whatever is stored there.
+__device__ __forceinline__ uint4 lora_b_piece(const uint16_t *B, int r, int rank, bool on) {
+    uint4 v = ldg16(B + r, on && r < rank);
+    const int left = rank - r;
+    if (left < 8) {
+        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] &= left > 2 * i + 1 ? 0xffffffffu : left > 2 * i ? 0xffffu : 0u;
+        v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return v;
+}
+// 32 columns of B as operands: column n of block b is column 8 (n / 2) + 2 b + n % 2, so that a lane's results are 8 neighbours.
+template <int RC>
+__device__ __forceinline__ void lora_load_b(uint4 (&bv)[4][RC], const LoraArgs &a, int ad, int rank, int n0, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const int col = n0 + 8 * (g >> 1) + 2 * b + (g & 1);
+#pragma unroll
+        for (int c = 0; c < RC; ++c) bv[b][c] = lora_b_piece(a.B + ((long long)ad * a.N + col) * a.rank_max, 32 * c + 8 * t, rank, col < a.N);
+    }
+}
+// Eight neighbours of a row of base (+ residual), in f32.
+struct Base8 {
+    float v[8];
+};
+__device__ __forceinline__ Base8 lora_base(const LoraArgs &a, long long at, bool on) {
+    Base8 o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o.v[i] = 0.f;
+    if (!on) return o;
+    if (a.base_f32) {
+        const float4 *p = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(a.base) + at);
+        const float4 u = p[0], w = p[1];
+        o.v[0] = u.x, o.v[1] = u.y, o.v[2] = u.z, o.v[3] = u.w, o.v[4] = w.x, o.v[5] = w.y, o.v[6] = w.z, o.v[7] = w.w;
+    } else {
+        const uint4 u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.base) + at);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o.v[2 * i] = bf16x2_lo(w[i]), o.v[2 * i + 1] = bf16x2_hi(w[i]);
+    }
+    return o;
+}
+__device__ __forceinline__ void lora_store(const LoraArgs &a, long long at, const Base8 &base, const float (&up)[8]) {
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = base.v[i] + up[i];
+    if (a.residual) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(a.residual + at);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[2 * i] += bf16x2_lo(w[i]), s[2 * i + 1] += bf16x2_hi(w[i]);
+    }
+    *reinterpret_cast<uint4 *>(a.out + at) = make_uint4(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]), pack_bf16x2(s[4], s[5]), pack_bf16x2(s[6], s[7]));
+}
+
+// =====================================================================================
+// Up to LORA_FEW rows: one launch.  A cluster of eight CTAs takes a tile of 16 rows: each an eighth of K, its warps a share of
+// that; the partial sums meet in distributed shared memory, and each CTA goes on with its share of the columns of B, whose
+// first pieces are on their way before the sums meet.  Every CTA puts the rows in order for itself (a few hundred comparisons a
+// thread), which is cheaper than a launch in front.  Where the tiles are few, several clusters share a tile's columns and each
+// forms x A^T for itself.
+// =====================================================================================
+constexpr int LORA_FEW = 128, LF_WARPS = 8, LF_CLUSTER = 8;
+
+template <int RC>  // rank_max up to 32 RC
+__global__ void __cluster_dims__(LF_CLUSTER, 1, 1) __launch_bounds__(LF_WARPS * 32) lora_few_kernel(LoraArgs a) {
+    constexpr int NB = 4 * RC, RP = 32 * RC, THREADS = LF_WARPS * 32;
+    extern __shared__ __align__(16) float lf_smem[];
+    float(*red)[16][RP + 4] = reinterpret_cast<float(*)[16][RP + 4]>(lf_smem);  // [WARPS / 2]
+    __shared__ __align__(16) float part[16][RP + 4];
+    __shared__ uint4 frag[RC][2][2][32];  // chunk, hi / lo, rows g / g + 8, lane
+    __shared__ int key[LORA_FEW], start[LORA_FEW], rows[16], s_tile[2];
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int rank_in = blockIdx.x % LF_CLUSTER, tile = blockIdx.x / LF_CLUSTER / a.splits, split = blockIdx.x / LF_CLUSTER % a.splits;
     pdl_wait();
     pdl_launch_dependents();
-    const int t = blockIdx.y, n = blockIdx.x * 128 + threadIdx.x;
-    if (n >= a.N) return;
-    const int ad = a.idx[t];
-    const long long at = (long long)t * a.N + n;
-    float s = a.base_f32 ? reinterpret_cast<const float *>(a.base)[at] : bf16_bits_to_f32(reinterpret_cast<const uint16_t *>(a.base)[at]);
-    float up = 0.f;
-    if (ad >= 0 && ad < a.n) {
-        const int rank = a.ranks ? min(max(a.ranks[ad], 0), a.rank_max) : a.rank_max;
-        const uint16_t *B = a.B + ((long long)ad * a.N + n) * a.rank_max;
-        for (int r = 0; r < rank; ++r) up = fmaf(a.low[(long long)t * a.rank_max + r], bf16_bits_to_f32(B[r]), up);
+    // ---- the tile: the rows of one adapter, 16 at a time, adapters in order ----
+    if (tid < a.T) key[tid] = lora_adapter(a, tid, blockIdx.x == 0);
+    if (tid < 16) rows[tid] = -1;
+    if (tid == 0) s_tile[0] = -1;
+    __syncthreads();
+    int mine = -1, pos = 0;
+    if (tid < a.T) {
+        mine = key[tid];
+        for (int u = 0; u < tid; ++u) pos += key[u] == mine;
+        start[tid] = pos % 16 == 0 ? mine : -1;
     }
-    s += up;
-    if (a.residual) s += bf16_bits_to_f32(a.residual[at]);
-    a.out[at] = f32_to_bf16_bits(s);
+    __syncthreads();
+    if (tid < a.T) {
+        int before = pos / 16;  // tiles of smaller adapters, and this one's earlier ones
+        for (int u = 0; u < a.T; ++u) before += start[u] >= 0 && start[u] < mine;
+        if (before == tile) {
+            rows[pos % 16] = tid;
+            if (pos % 16 == 0) s_tile[0] = mine;
+        }
+    }
+    __syncthreads();
+    const int ad = s_tile[0];
+    if (ad < 0) return;  // (the whole cluster)
+    const int rank = lora_rank(a, ad), r_lo = rows[g], r_hi = rows[g + 8];
+    // ---- x A^T ----
+    if (rank > 0) {
+        const int chunks = (a.K + 31) / 32, c0 = chunks * rank_in / LF_CLUSTER, c1 = chunks * (rank_in + 1) / LF_CLUSTER;
+        const uint16_t *x[1][2] = {{r_lo >= 0 ? a.x + r_lo * a.x_row : nullptr, r_hi >= 0 ? a.x + r_hi * a.x_row : nullptr}};
+        float acc[1][NB][4] = {};
+        lora_down<1, NB>(acc, x, a.A + (long long)ad * a.rank_max * a.K, a.K, rank, 0, c0 + warp, c1, LF_WARPS, lane);
+#pragma unroll
+        for (int half = 1; half >= 0; --half) {
+            if (warp / (LF_WARPS / 2) == half)
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float &d = red[warp % (LF_WARPS / 2)][g + 8 * (e >> 1)][8 * b + 2 * t4 + (e & 1)];
+                        d = half ? acc[0][b][e] : d + acc[0][b][e];
+                    }
+            __syncthreads();
+        }
+        for (int i = tid; i < 16 * RP; i += THREADS) {
+            float s = 0.f;
+#pragma unroll
+            for (int w = 0; w < LF_WARPS / 2; ++w) s += red[w][i / RP][i % RP];
+            part[i / RP][i % RP] = s;
+        }
+    }
+    // ---- this warp's first columns, before the sums meet ----
+    const int blocks = (a.N + 31) / 32, stride = LF_CLUSTER * a.splits * LF_WARPS;
+    int cb = (split * LF_CLUSTER + rank_in) * LF_WARPS + warp;
+    uint4 bv[4][RC];
+    Base8 base[2];
+    auto fetch = [&]() {
+        const int n0 = 32 * cb, col = n0 + 8 * t4;
+        lora_load_b<RC>(bv, a, ad, cb < blocks ? rank : 0, n0, lane);
+        base[0] = lora_base(a, (long long)r_lo * a.N + col, r_lo >= 0 && cb < blocks && col < a.N);
+        base[1] = lora_base(a, (long long)r_hi * a.N + col, r_hi >= 0 && cb < blocks && col < a.N);
+    };
+    fetch();
+    if (rank > 0) {
+        cluster.sync();
+        const float scale = a.scales[ad];
+        for (int i = tid; i < 16 * RP / 2; i += THREADS) {
+            const int row = i / (RP / 2), r = 2 * (i % (RP / 2));
+            float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < LF_CLUSTER; ++c) {
+                const float2 v = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(&part[row][r], c));
+                s.x += v.x, s.y += v.y;
+            }
+            s.x *= scale, s.y *= scale;
+            const uint32_t hi = pack_bf16x2(s.x, s.y), lo = pack_bf16x2(s.x - bf16x2_lo(hi), s.y - bf16x2_hi(hi));
+            // element r of the row: chunk, the lane's eight, the word in it
+            const int c = r / 32, l = (row % 8) * 4 + r % 32 / 8, w = r % 8 / 2;
+            reinterpret_cast<uint32_t *>(&frag[c][0][row / 8][l])[w] = hi;
+            reinterpret_cast<uint32_t *>(&frag[c][1][row / 8][l])[w] = lo;
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // done with the other CTAs' sums
+        __syncthreads();
+    }
+    while (cb < blocks) {
+        float acc[4][4] = {};
+        if (rank > 0) {
+#pragma unroll
+            for (int c = 0; c < RC; ++c)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const uint4 u = frag[c][p][0][lane], v = frag[c][p][1][lane];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        mma_bf16_16816(acc[b], u.x, v.x, u.y, v.y, bv[b][c].x, bv[b][c].y);
+                        mma_bf16_16816(acc[b], u.z, v.z, u.w, v.w, bv[b][c].z, bv[b][c].w);
+                    }
+                }
+        }
+        const int col = 32 * cb + 8 * t4;
+        const Base8 b0 = base[0], b1 = base[1];
+        cb += stride;
+        fetch();
+        if (col < a.N) {
+            const float u[8] = {acc[0][0], acc[0][1], acc[1][0], acc[1][1], acc[2][0], acc[2][1], acc[3][0], acc[3][1]};
+            const float v[8] = {acc[0][2], acc[0][3], acc[1][2], acc[1][3], acc[2][2], acc[2][3], acc[3][2], acc[3][3]};
+            if (r_lo >= 0) lora_store(a, (long long)r_lo * a.N + col, b0, u);
+            if (r_hi >= 0) lora_store(a, (long long)r_hi * a.N + col, b1, v);
+        }
+    }
+    if (rank > 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-constexpr int LORA_MAX_ROWS = 65535, LORA_MAX_RANK = 128;
-size_t lora_scratch_bytes() { return (size_t)LORA_MAX_ROWS * LORA_MAX_RANK * 4; }
+// =====================================================================================
+// Many rows, three launches: rows by adapter into tiles of 64; x A^T of a tile by a cluster of eight CTAs (an eighth of K each,
+// the sums meeting in distributed shared memory); and the columns of B, 64 rows x 256 columns a CTA, which is where the bytes
+// of base and out go by.
+// =====================================================================================
+constexpr int LM_ROWS = 64, LM_MT = LM_ROWS / 16, LG_THREADS = 1024, LD_WARPS = 4, LD_CLUSTER = 8, LU_WARPS = 8;
+constexpr int LORA_MAX_TILES = (LORA_MAX_ROWS + LM_ROWS - 1) / LM_ROWS + LORA_MAX_ADAPTERS + 1;
+
+__global__ void __launch_bounds__(LG_THREADS) lora_group_kernel(LoraArgs a) {
+    extern __shared__ int lora_smem[];
+    int *count = lora_smem, *first = lora_smem + a.n + 1;  // [n + 1] each; adapter n: none
+    __shared__ int sums[LG_THREADS / 32][2];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int i = tid; i <= a.n; i += LG_THREADS) count[i] = 0;
+    pdl_wait();
+    pdl_launch_dependents();
+    __syncthreads();
+    // (rows of one adapter are counted together: a prompt's rows would otherwise queue for one counter)
+    for (int base = 0; base < a.T; base += LG_THREADS) {
+        const int t = base + tid, ad = t < a.T ? lora_adapter(a, t, true) : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, ad);
+        if (ad >= 0 && lane == __ffs(same) - 1) atomicAdd(&count[ad], __popc(same));
+    }
+    __syncthreads();
+    const int per = (a.n + LG_THREADS) / LG_THREADS, a0 = min(tid * per, a.n + 1), a1 = min(a0 + per, a.n + 1);
+    int r = 0, w = 0;  // rows and tiles
+    for (int i = a0; i < a1; ++i) r += count[i], w += (count[i] + LM_ROWS - 1) / LM_ROWS;
+    int ir = r, iw = w;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int ur = __shfl_up_sync(0xffffffffu, ir, d), uw = __shfl_up_sync(0xffffffffu, iw, d);
+        if (lane >= d) ir += ur, iw += uw;
+    }
+    if (lane == 31) sums[warp][0] = ir, sums[warp][1] = iw;
+    __syncthreads();
+    int br = ir - r, bw = iw - w, all = 0;
+    for (int i = 0; i < LG_THREADS / 32; ++i) {
+        if (i < warp) br += sums[i][0], bw += sums[i][1];
+        all += sums[i][1];
+    }
+    for (int i = a0; i < a1; ++i) {
+        const int c = count[i];
+        first[i] = br;
+        for (int k = 0; k < c; k += LM_ROWS) a.tiles[bw++] = make_int4(i, br + k, min(LM_ROWS, c - k), 0);
+        br += c;
+    }
+    if (tid == 0) *a.n_tiles = all;
+    __syncthreads();
+    for (int base = 0; base < a.T; base += LG_THREADS) {
+        const int t = base + tid, ad = t < a.T ? lora_adapter(a, t, false) : -1;
+        const unsigned same = __match_any_sync(0xffffffffu, ad);
+        int at = 0;
+        if (ad >= 0 && lane == __ffs(same) - 1) at = atomicAdd(&first[ad], __popc(same));
+        at = __shfl_sync(0xffffffffu, at, __ffs(same) - 1) + __popc(same & ((1u << lane) - 1));
+        if (ad >= 0) a.order[at] = t;
+    }
+}
+
+template <int NB>  // blocks of eight ranks at a time
+__global__ void __cluster_dims__(LD_CLUSTER, 1, 1) __launch_bounds__(LD_WARPS * 32) lora_down_kernel(LoraArgs a) {
+    constexpr int RP = 8 * NB, THREADS = LD_WARPS * 32;
+    extern __shared__ __align__(16) float ld_smem[];  // [WARPS][64][RP + 4]; the first is the CTA's sum
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    const int tile = blockIdx.x / LD_CLUSTER, rank_in = blockIdx.x % LD_CLUSTER;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (tile >= *a.n_tiles) return;  // (the whole cluster)
+    const int4 w = a.tiles[tile];
+    const int rank = lora_rank(a, w.x), wide = (a.rank_max + 31) / 32 * 32;
+    if (rank == 0) return;
+    const float scale = a.scales[w.x];
+    const uint16_t *x[LM_MT][2];
+#pragma unroll
+    for (int m = 0; m < LM_MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = 16 * m + 8 * i + g;
+            x[m][i] = row < w.z ? a.x + a.order[w.y + row] * a.x_row : nullptr;
+        }
+    const int chunks = (a.K + 31) / 32, c0 = chunks * rank_in / LD_CLUSTER, c1 = chunks * (rank_in + 1) / LD_CLUSTER;
+    for (int r0 = 0; r0 < rank; r0 += RP) {
+        float acc[LM_MT][NB][4] = {};
+        lora_down<LM_MT, NB>(acc, x, a.A + (long long)w.x * a.rank_max * a.K, a.K, rank, r0, c0 + warp, c1, LD_WARPS, lane);
+        float *mine = ld_smem + warp * LM_ROWS * (RP + 4);
+#pragma unroll
+        for (int m = 0; m < LM_MT; ++m)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    *reinterpret_cast<float2 *>(mine + (16 * m + 8 * e + g) * (RP + 4) + 8 * b + 2 * t4) = make_float2(acc[m][b][2 * e], acc[m][b][2 * e + 1]);
+        __syncthreads();
+        for (int i = tid; i < LM_ROWS * RP / 4; i += THREADS) {
+            float4 *p = reinterpret_cast<float4 *>(ld_smem + (i / (RP / 4)) * (RP + 4)) + i % (RP / 4);
+            float4 s = *p;
+#pragma unroll
+            for (int k = 1; k < LD_WARPS; ++k) {
+                const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + k * LM_ROWS * (RP + 4));
+                s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+            }
+            *p = s;
+        }
+        cluster.sync();
+        // eight rows a CTA
+        for (int i = tid; i < LM_ROWS / LD_CLUSTER * RP / 4; i += THREADS) {
+            const int row = LM_ROWS / LD_CLUSTER * rank_in + i / (RP / 4), r = 4 * (i % (RP / 4));
+            if (row >= w.z || r0 + r >= wide) continue;
+            float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < LD_CLUSTER; ++c) {
+                const float4 v = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(ld_smem + row * (RP + 4) + r, c));
+                s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+            }
+            s.x *= scale, s.y *= scale, s.z *= scale, s.w *= scale;
+            const uint2 hi = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+            const uint2 lo = make_uint2(pack_bf16x2(s.x - bf16x2_lo(hi.x), s.y - bf16x2_hi(hi.x)), pack_bf16x2(s.z - bf16x2_lo(hi.y), s.w - bf16x2_hi(hi.y)));
+            uint16_t *d = a.low + (long long)(w.y + row) * 2 * wide + r0 + r;
+            *reinterpret_cast<uint2 *>(d) = hi;
+            *reinterpret_cast<uint2 *>(d + wide) = lo;
+        }
+        cluster.sync();
+    }
+}
+
+template <int RC>
+__global__ void __launch_bounds__(LU_WARPS * 32) lora_up_kernel(LoraArgs a) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    pdl_wait();
+    pdl_launch_dependents();
+    if ((int)blockIdx.y >= *a.n_tiles) return;
+    const int4 w = a.tiles[blockIdx.y];
+    const int rank = lora_rank(a, w.x), wide = (a.rank_max + 31) / 32 * 32, n0 = (blockIdx.x * LU_WARPS + warp) * 32, col = n0 + 8 * t4;
+    if (n0 >= a.N) return;
+    uint4 bv[4][RC];
+    lora_load_b<RC>(bv, a, w.x, rank, n0, lane);
+#pragma unroll
+    for (int m = 0; m < LM_MT; ++m) {
+        if (16 * m >= w.z) break;
+        const int lo_row = 16 * m + g, hi_row = lo_row + 8;
+        const long long t_lo = lo_row < w.z ? a.order[w.y + lo_row] : -1, t_hi = hi_row < w.z ? a.order[w.y + hi_row] : -1;
+        const Base8 b0 = lora_base(a, t_lo * a.N + col, t_lo >= 0 && col < a.N), b1 = lora_base(a, t_hi * a.N + col, t_hi >= 0 && col < a.N);
+        float acc[4][4] = {};
+#pragma unroll
+        for (int c = 0; c < RC; ++c)
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                const bool on = 32 * c + 8 * t4 < rank;  // (columns behind it need not have been written)
+                const uint16_t *l = a.low + (long long)(w.y + lo_row) * 2 * wide + p * wide + 32 * c + 8 * t4;
+                const uint4 u = ldg16(l, on && t_lo >= 0), v = ldg16(l + 16 * wide, on && t_hi >= 0);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    mma_bf16_16816(acc[b], u.x, v.x, u.y, v.y, bv[b][c].x, bv[b][c].y);
+                    mma_bf16_16816(acc[b], u.z, v.z, u.w, v.w, bv[b][c].z, bv[b][c].w);
+                }
+            }
+        if (col < a.N) {
+            const float u[8] = {acc[0][0], acc[0][1], acc[1][0], acc[1][1], acc[2][0], acc[2][1], acc[3][0], acc[3][1]};
+            const float v[8] = {acc[0][2], acc[0][3], acc[1][2], acc[1][3], acc[2][2], acc[2][3], acc[3][2], acc[3][3]};
+            if (t_lo >= 0) lora_store(a, t_lo * a.N + col, b0, u);
+            if (t_hi >= 0) lora_store(a, t_hi * a.N + col, b1, v);
+        }
+    }
+}
+
+size_t lora_scratch_bytes() {
+    return 256 + (size_t)LORA_MAX_TILES * 16 + ((size_t)LORA_MAX_ROWS + 1) * 4 + ((size_t)LORA_MAX_ROWS + 1) * LORA_MAX_RANK * 4;
+}
+
+template <int NB>
+static int launch_lora_down(const LoraArgs &a, int tiles, cudaStream_t stream) {
+    const int smem = LD_WARPS * LM_ROWS * (8 * NB + 4) * 4;
+    int rc = check_cuda(cudaFuncSetAttribute(lora_down_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "lora shared memory");
+    if (rc) return rc;
+    return check_cuda(launch_pdl(lora_down_kernel<NB>, dim3(tiles * LD_CLUSTER), dim3(LD_WARPS * 32), smem, stream, a), "lora down launch");
+}
+
+static int launch_lora(LoraArgs a, cudaStream_t stream) {
+    const int rc32 = (a.rank_max + 31) / 32;
+    if (a.T <= LORA_FEW) {
+        // Columns a warp would have with one cluster per tile, counted in blocks of 32: share them while SMs would idle.
+        const int tiles = (a.T + 15) / 16, blocks = (a.N + 31) / 32;
+        a.splits = max(1, min(2 * device_sm_count() / (LF_CLUSTER * tiles), blocks / (LF_CLUSTER * LF_WARPS)));
+        const dim3 grid(LF_CLUSTER * a.splits * min(a.T, tiles + a.n + 1)), block(LF_WARPS * 32);
+        auto kernel = rc32 == 1 ? lora_few_kernel<1> : rc32 == 2 ? lora_few_kernel<2> : lora_few_kernel<4>;
+        const int smem = LF_WARPS / 2 * 16 * ((rc32 == 3 ? 4 : rc32) * 32 + 4) * 4;
+        int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "lora shared memory");
+        if (rc) return rc;
+        return check_cuda(launch_pdl(kernel, grid, block, smem, stream, a), "lora launch");
+    }
+    const int tiles = min(a.T, (a.T + LM_ROWS - 1) / LM_ROWS + a.n + 1);
+    const int smem = 2 * (a.n + 1) * 4;
+    int rc = check_cuda(launch_pdl(lora_group_kernel, dim3(1), dim3(LG_THREADS), smem, stream, a), "lora group launch");
+    if (rc) return rc;
+    if (a.n > 0) {
+        rc = a.rank_max <= 16 ? launch_lora_down<2>(a, tiles, stream) : a.rank_max <= 32 ? launch_lora_down<4>(a, tiles, stream) : launch_lora_down<8>(a, tiles, stream);
+        if (rc) return rc;
+    }
+    auto up = rc32 == 1 ? lora_up_kernel<1> : rc32 == 2 ? lora_up_kernel<2> : lora_up_kernel<4>;
+    return check_cuda(launch_pdl(up, dim3((a.N + 32 * LU_WARPS - 1) / (32 * LU_WARPS), tiles), dim3(LU_WARPS * 32), 0, stream, a), "lora up launch");
+}
 
 }  // namespace awq
 
@@ -74,7 +477,8 @@ extern "C" int awq_b200_lora_bf16(const uint16_t *x, long long x_row_stride, con
                                   const int32_t *ranks, int n_adapters, int rank_max, const int32_t *idx, const void *base, int base_is_f32,
                                   const uint16_t *residual, uint16_t *out, int T, int K, int N, void *workspace, size_t workspace_bytes,
                                   awq_stream_t stream) {
-    AWQ_REQUIRE(T >= 0 && T <= LORA_MAX_ROWS && K > 0 && N >= 0 && n_adapters >= 0, "lora: bad size (at most %d rows)", LORA_MAX_ROWS);
+    AWQ_REQUIRE(T >= 0 && T <= LORA_MAX_ROWS && K > 0 && N >= 0 && n_adapters >= 0 && n_adapters <= LORA_MAX_ADAPTERS,
+                "lora: bad size (at most %d rows and %d adapters)", LORA_MAX_ROWS, LORA_MAX_ADAPTERS);
     AWQ_REQUIRE(rank_max > 0 && rank_max <= LORA_MAX_RANK && rank_max % 8 == 0, "lora: rank_max (%d) must be a multiple of 8, at most %d", rank_max,
                 LORA_MAX_RANK);
     AWQ_REQUIRE(K % 8 == 0 && N % 8 == 0, "lora: K (%d) and N (%d) must be multiples of 8", K, N);
@@ -86,10 +490,14 @@ extern "C" int awq_b200_lora_bf16(const uint16_t *x, long long x_row_stride, con
                 "lora: pointers must be 16-byte aligned");
     AWQ_REQUIRE_REQUEST_WORKSPACE("lora", workspace, workspace_bytes);
     const RequestWorkspaceView w = request_workspace(workspace);
-    LoraArgs a{x, A, B, scales, ranks, idx, base, residual, out, x_row_stride, base_is_f32, T, K, N, n_adapters, rank_max,
-               reinterpret_cast<float *>(w.lora), w.header};
-    const long long items = (long long)T * rank_max;
-    int rc = check_cuda(launch_pdl(lora_down_kernel, dim3((unsigned)((items + 3) / 4)), dim3(128), 0, as_stream(stream), a), "lora down launch");
-    if (rc) return rc;
-    return check_cuda(launch_pdl(lora_up_kernel, dim3((N + 127) / 128, T), dim3(128), 0, as_stream(stream), a), "lora up launch");
+    LoraArgs a{};
+    a.x = x, a.A = A, a.B = B, a.scales = scales, a.ranks = ranks, a.idx = idx, a.base = base, a.residual = residual, a.out = out;
+    a.x_row = x_row_stride, a.base_f32 = base_is_f32, a.T = T, a.K = K, a.N = N, a.n = n_adapters, a.rank_max = rank_max, a.splits = 1;
+    a.header = w.header;
+    uint8_t *p = w.lora;
+    a.n_tiles = reinterpret_cast<int32_t *>(p), p += 256;
+    a.tiles = reinterpret_cast<int4 *>(p), p += (size_t)LORA_MAX_TILES * 16;
+    a.order = reinterpret_cast<int32_t *>(p), p += ((size_t)LORA_MAX_ROWS + 1) * 4;
+    a.low = reinterpret_cast<uint16_t *>(p);
+    return launch_lora(a, as_stream(stream));
 }
