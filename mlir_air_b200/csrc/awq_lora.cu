@@ -13,6 +13,7 @@
 #include "awq_request.cuh"
 
 #include <cooperative_groups.h>
+#include <cuda_fp16.h>
 #include <math.h>
 
 namespace awq {
@@ -33,7 +34,7 @@ struct LoraArgs {
     int splits;  // clusters that share a tile's columns (few rows)
     RequestHeader *header;
     int32_t *order;   // [T] rows by adapter
-    int4 *tiles;      // adapter, first of `order`, rows, -
+    int4 *tiles;      // adapter, first of `order`, rows, rank
     int32_t *n_tiles;
     uint16_t *low;    // [T][2][rank_max up to 32] scale x A^T in the order of `order`, hi and lo
 };
@@ -77,17 +78,16 @@ __device__ __forceinline__ void lora_down(float (&acc)[MT][NB][4], const uint16_
     }
 }
 
-// Eight columns of B from rank column r on; columns from `rank` on are zero whatever is stored there.
-__device__ __forceinline__ uint4 lora_b_piece(const uint16_t *B, int r, int rank, bool on) {
-    uint4 v = ldg16(B + r, on && r < rank);
-    const int left = rank - r;
-    if (left < 8) {
-        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// The first `left` of eight columns of B, the others zero, whatever is stored there.
+__device__ __forceinline__ uint4 lora_mask_rank(uint4 v, int left) {
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] &= left > 2 * i + 1 ? 0xffffffffu : left > 2 * i ? 0xffffu : 0u;
-        v = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    return v;
+    for (int i = 0; i < 4; ++i) w[i] &= left > 2 * i + 1 ? 0xffffffffu : left > 2 * i ? 0xffffu : 0u;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 lora_b_piece(const uint16_t *B, int r, int rank, bool on) {
+    const uint4 v = ldg16(B + r, on && r < rank);
+    return rank & 7 ? lora_mask_rank(v, rank - r) : v;
 }
 // 32 columns of B as operands: column n of block b is column 8 (n / 2) + 2 b + n % 2, so that a lane's results are 8 neighbours.
 template <int RC>
@@ -131,7 +131,7 @@ __device__ __forceinline__ void lora_store(const LoraArgs &a, long long at, cons
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[2 * i] += bf16x2_lo(w[i]), s[2 * i + 1] += bf16x2_hi(w[i]);
     }
-    *reinterpret_cast<uint4 *>(a.out + at) = make_uint4(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]), pack_bf16x2(s[4], s[5]), pack_bf16x2(s[6], s[7]));
+    *reinterpret_cast<uint4 *>(a.out + at) = make_uint4(pack16x2<false>(s[0], s[1]), pack16x2<false>(s[2], s[3]), pack16x2<false>(s[4], s[5]), pack16x2<false>(s[6], s[7]));
 }
 
 // =====================================================================================
@@ -229,7 +229,7 @@ __global__ void __cluster_dims__(LF_CLUSTER, 1, 1) __launch_bounds__(LF_WARPS * 
                 s.x += v.x, s.y += v.y;
             }
             s.x *= scale, s.y *= scale;
-            const uint32_t hi = pack_bf16x2(s.x, s.y), lo = pack_bf16x2(s.x - bf16x2_lo(hi), s.y - bf16x2_hi(hi));
+            const uint32_t hi = pack16x2<false>(s.x, s.y), lo = pack16x2<false>(s.x - bf16x2_lo(hi), s.y - bf16x2_hi(hi));
             // element r of the row: chunk, the lane's eight, the word in it
             const int c = r / 32, l = (row % 8) * 4 + r % 32 / 8, w = r % 8 / 2;
             reinterpret_cast<uint32_t *>(&frag[c][0][row / 8][l])[w] = hi;
@@ -272,12 +272,13 @@ __global__ void __cluster_dims__(LF_CLUSTER, 1, 1) __launch_bounds__(LF_WARPS * 
 // the sums meeting in distributed shared memory); and the columns of B, 64 rows x 256 columns a CTA, which is where the bytes
 // of base and out go by.
 // =====================================================================================
-constexpr int LM_ROWS = 64, LM_MT = LM_ROWS / 16, LG_THREADS = 1024, LD_WARPS = 4, LD_CLUSTER = 8, LU_WARPS = 8;
+constexpr int LM_ROWS = 64, LM_MT = LM_ROWS / 16, LG_THREADS = 1024, LD_WARPS = 8, LU_WARPS = 4;
 constexpr int LORA_MAX_TILES = (LORA_MAX_ROWS + LM_ROWS - 1) / LM_ROWS + LORA_MAX_ADAPTERS + 1;
 
 __global__ void __launch_bounds__(LG_THREADS) lora_group_kernel(LoraArgs a) {
     extern __shared__ int lora_smem[];
     int *count = lora_smem, *first = lora_smem + a.n + 1;  // [n + 1] each; adapter n: none
+    int *place = reinterpret_cast<int *>(a.low);           // [T] a row's place among its adapter's (`low` is not in use yet)
     __shared__ int sums[LG_THREADS / 32][2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     for (int i = tid; i <= a.n; i += LG_THREADS) count[i] = 0;
@@ -285,10 +286,14 @@ __global__ void __launch_bounds__(LG_THREADS) lora_group_kernel(LoraArgs a) {
     pdl_launch_dependents();
     __syncthreads();
     // (rows of one adapter are counted together: a prompt's rows would otherwise queue for one counter)
+#pragma unroll 4
     for (int base = 0; base < a.T; base += LG_THREADS) {
         const int t = base + tid, ad = t < a.T ? lora_adapter(a, t, true) : -1;
         const unsigned same = __match_any_sync(0xffffffffu, ad);
-        if (ad >= 0 && lane == __ffs(same) - 1) atomicAdd(&count[ad], __popc(same));
+        int at = 0;
+        if (ad >= 0 && lane == __ffs(same) - 1) at = atomicAdd(&count[ad], __popc(same));
+        at = __shfl_sync(0xffffffffu, at, __ffs(same) - 1) + __popc(same & ((1u << lane) - 1));
+        if (ad >= 0) place[t] = at;
     }
     __syncthreads();
     const int per = (a.n + LG_THREADS) / LG_THREADS, a0 = min(tid * per, a.n + 1), a1 = min(a0 + per, a.n + 1);
@@ -308,50 +313,85 @@ __global__ void __launch_bounds__(LG_THREADS) lora_group_kernel(LoraArgs a) {
         all += sums[i][1];
     }
     for (int i = a0; i < a1; ++i) {
-        const int c = count[i];
+        const int c = count[i], rank = c ? lora_rank(a, i) : 0;
         first[i] = br;
-        for (int k = 0; k < c; k += LM_ROWS) a.tiles[bw++] = make_int4(i, br + k, min(LM_ROWS, c - k), 0);
+        for (int k = 0; k < c; k += LM_ROWS) a.tiles[bw++] = make_int4(i, br + k, min(LM_ROWS, c - k), rank);
         br += c;
     }
     if (tid == 0) *a.n_tiles = all;
     __syncthreads();
-    for (int base = 0; base < a.T; base += LG_THREADS) {
-        const int t = base + tid, ad = t < a.T ? lora_adapter(a, t, false) : -1;
-        const unsigned same = __match_any_sync(0xffffffffu, ad);
-        int at = 0;
-        if (ad >= 0 && lane == __ffs(same) - 1) at = atomicAdd(&first[ad], __popc(same));
-        at = __shfl_sync(0xffffffffu, at, __ffs(same) - 1) + __popc(same & ((1u << lane) - 1));
-        if (ad >= 0) a.order[at] = t;
-    }
+#pragma unroll 4
+    for (int t = tid; t < a.T; t += LG_THREADS) a.order[first[lora_adapter(a, t, false)] + place[t]] = t;
 }
 
-template <int NB>  // blocks of eight ranks at a time
-__global__ void __cluster_dims__(LD_CLUSTER, 1, 1) __launch_bounds__(LD_WARPS * 32) lora_down_kernel(LoraArgs a) {
-    constexpr int RP = 8 * NB, THREADS = LD_WARPS * 32;
-    extern __shared__ __align__(16) float ld_smem[];  // [WARPS][64][RP + 4]; the first is the CTA's sum
+// x A^T of a tile of 64 rows by a cluster of 1 to 8 CTAs, each with a share of K, which it runs through in stages of 128: x and A
+// come in by 16-byte asynchronous copies, three stages deep, so that the memory has 64 KB per CTA to fetch whatever the warps
+// do; a warp multiplies a quarter of a stage by half the ranks.  Rows in shared memory are 256 bytes with their two halves
+// swapped in odd rows: a quarter warp's 16-byte reads then touch every bank once.
+constexpr int LD_STAGE = 128, LD_STAGES = 3;
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool on) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+
+template <int NB>  // blocks of eight ranks a warp has; a CTA has twice that at a time
+__global__ void __launch_bounds__(LD_WARPS * 32, 2) lora_down_kernel(LoraArgs a) {
+    constexpr int RP = 16 * NB, THREADS = LD_WARPS * 32, PARTS = LD_WARPS / 2, ROWS = LM_ROWS + RP, BYTES = ROWS * 2 * LD_STAGE;
+    extern __shared__ __align__(128) uint8_t ld_smem[];  // [STAGES][64 rows of x, RP of A][256]; then [PARTS][64][RP + 4] f32
     const cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-    const int tile = blockIdx.x / LD_CLUSTER, rank_in = blockIdx.x % LD_CLUSTER;
+    const int n_ctas = (int)cluster.num_blocks(), rank_in = (int)cluster.block_rank(), tile = blockIdx.x / n_ctas;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3, half = warp & 1, part = warp >> 1;
     pdl_wait();
     pdl_launch_dependents();
+    const int4 w = a.tiles[tile];  // (behind the last tile: not looked at)
     if (tile >= *a.n_tiles) return;  // (the whole cluster)
-    const int4 w = a.tiles[tile];
-    const int rank = lora_rank(a, w.x), wide = (a.rank_max + 31) / 32 * 32;
+    const int rank = w.w, wide = (a.rank_max + 31) / 32 * 32;
     if (rank == 0) return;
     const float scale = a.scales[w.x];
-    const uint16_t *x[LM_MT][2];
+    const int all = (a.K + LD_STAGE - 1) / LD_STAGE, s0 = all * rank_in / n_ctas, s1 = all * (rank_in + 1) / n_ctas;
+    // a thread copies piece tid % 16 of rows tid / 16 + 16 i
+    const int piece = tid & 15, r16 = tid >> 4, swapped = piece ^ ((r16 & 1) << 2);
+    const uint16_t *src[ROWS / 16];
 #pragma unroll
-    for (int m = 0; m < LM_MT; ++m)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int row = 16 * m + 8 * i + g;
-            x[m][i] = row < w.z ? a.x + a.order[w.y + row] * a.x_row : nullptr;
-        }
-    const int chunks = (a.K + 31) / 32, c0 = chunks * rank_in / LD_CLUSTER, c1 = chunks * (rank_in + 1) / LD_CLUSTER;
+    for (int i = 0; i < LM_ROWS / 16; ++i) src[i] = r16 + 16 * i < w.z ? a.x + a.order[w.y + r16 + 16 * i] * a.x_row : nullptr;
+    const uint32_t smem = smem_u32(ld_smem), dst = smem + r16 * 256 + swapped * 16;
+    float *sums = reinterpret_cast<float *>(ld_smem);
     for (int r0 = 0; r0 < rank; r0 += RP) {
+#pragma unroll
+        for (int i = 0; i < RP / 16; ++i)
+            src[LM_ROWS / 16 + i] = r0 + r16 + 16 * i < rank ? a.A + ((long long)w.x * a.rank_max + r0 + r16 + 16 * i) * a.K : nullptr;
+        auto load = [&](int s) {
+            const int k = s * LD_STAGE + 8 * piece;
+            if (s < s1)
+#pragma unroll
+                for (int i = 0; i < ROWS / 16; ++i) {
+                    const bool on = src[i] != nullptr && k < a.K;
+                    cp_async16(dst + (s - s0) % LD_STAGES * BYTES + i * 16 * 256, on ? src[i] + k : a.A, on);
+                }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        for (int s = 0; s < LD_STAGES - 1; ++s) load(s0 + s);
         float acc[LM_MT][NB][4] = {};
-        lora_down<LM_MT, NB>(acc, x, a.A + (long long)w.x * a.rank_max * a.K, a.K, rank, r0, c0 + warp, c1, LD_WARPS, lane);
-        float *mine = ld_smem + warp * LM_ROWS * (RP + 4);
+        for (int s = s0; s < s1; ++s) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(LD_STAGES - 2) : "memory");
+            __syncthreads();
+            load(s + LD_STAGES - 1);
+            const uint32_t at = smem + (s - s0) % LD_STAGES * BYTES + g * 256 + ((4 * part + t4) ^ ((g & 1) << 2)) * 16;
+            uint4 av[NB];
+#pragma unroll
+            for (int b = 0; b < NB; ++b) av[b] = lds128(at + (LM_ROWS + 8 * (NB * half + b)) * 256);
+#pragma unroll
+            for (int m = 0; m < LM_MT; ++m) {
+                if (r0 + 8 * NB * half >= rank) break;  // (no ranks for this warp)
+                const uint4 x0 = lds128(at + 16 * m * 256), x1 = lds128(at + (16 * m + 8) * 256);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    mma_bf16_16816(acc[m][b], x0.x, x1.x, x0.y, x1.y, av[b].x, av[b].y);
+                    mma_bf16_16816(acc[m][b], x0.z, x1.z, x0.w, x1.w, av[b].z, av[b].w);
+                }
+            }
+        }
+        __syncthreads();  // (the copies still pending are empty groups)
+        float *mine = sums + part * LM_ROWS * (RP + 4) + half * 8 * NB;
 #pragma unroll
         for (int m = 0; m < LM_MT; ++m)
 #pragma unroll
@@ -361,29 +401,28 @@ __global__ void __cluster_dims__(LD_CLUSTER, 1, 1) __launch_bounds__(LD_WARPS * 
                     *reinterpret_cast<float2 *>(mine + (16 * m + 8 * e + g) * (RP + 4) + 8 * b + 2 * t4) = make_float2(acc[m][b][2 * e], acc[m][b][2 * e + 1]);
         __syncthreads();
         for (int i = tid; i < LM_ROWS * RP / 4; i += THREADS) {
-            float4 *p = reinterpret_cast<float4 *>(ld_smem + (i / (RP / 4)) * (RP + 4)) + i % (RP / 4);
+            float4 *p = reinterpret_cast<float4 *>(sums + (i / (RP / 4)) * (RP + 4)) + i % (RP / 4);
             float4 s = *p;
 #pragma unroll
-            for (int k = 1; k < LD_WARPS; ++k) {
+            for (int k = 1; k < PARTS; ++k) {
                 const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + k * LM_ROWS * (RP + 4));
                 s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
             }
             *p = s;
         }
         cluster.sync();
-        // eight rows a CTA
-        for (int i = tid; i < LM_ROWS / LD_CLUSTER * RP / 4; i += THREADS) {
-            const int row = LM_ROWS / LD_CLUSTER * rank_in + i / (RP / 4), r = 4 * (i % (RP / 4));
+        // 64 / n_ctas rows a CTA
+        for (int i = tid; i < LM_ROWS / n_ctas * (RP / 4); i += THREADS) {
+            const int row = LM_ROWS / n_ctas * rank_in + i / (RP / 4), r = 4 * (i % (RP / 4));
             if (row >= w.z || r0 + r >= wide) continue;
             float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int c = 0; c < LD_CLUSTER; ++c) {
-                const float4 v = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(ld_smem + row * (RP + 4) + r, c));
+            for (int c = 0; c < n_ctas; ++c) {
+                const float4 v = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(sums + row * (RP + 4) + r, c));
                 s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
             }
             s.x *= scale, s.y *= scale, s.z *= scale, s.w *= scale;
-            const uint2 hi = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
-            const uint2 lo = make_uint2(pack_bf16x2(s.x - bf16x2_lo(hi.x), s.y - bf16x2_hi(hi.x)), pack_bf16x2(s.z - bf16x2_lo(hi.y), s.w - bf16x2_hi(hi.y)));
+            const uint2 hi = make_uint2(pack16x2<false>(s.x, s.y), pack16x2<false>(s.z, s.w));
+            const uint2 lo = make_uint2(pack16x2<false>(s.x - bf16x2_lo(hi.x), s.y - bf16x2_hi(hi.x)), pack16x2<false>(s.z - bf16x2_lo(hi.y), s.w - bf16x2_hi(hi.y)));
             uint16_t *d = a.low + (long long)(w.y + row) * 2 * wide + r0 + r;
             *reinterpret_cast<uint2 *>(d) = hi;
             *reinterpret_cast<uint2 *>(d + wide) = lo;
@@ -392,42 +431,96 @@ __global__ void __cluster_dims__(LD_CLUSTER, 1, 1) __launch_bounds__(LD_WARPS * 
     }
 }
 
-template <int RC>
-__global__ void __launch_bounds__(LU_WARPS * 32) lora_up_kernel(LoraArgs a) {
+// A CTA has a tile's x A^T in shared memory, in the order of mma operands, and goes through `loops` times 32 columns per warp; the
+// base of the next columns is on its way while these are multiplied, and the products are summed on top of it.  Lanes without
+// a row or column of their own read some other one's and store nothing.
+template <int RC, bool F32>
+__global__ void __launch_bounds__(LU_WARPS * 32, RC == 4 ? 2 : F32 ? 3 : 4) lora_up_kernel(LoraArgs a, int loops) {
+    extern __shared__ __align__(16) uint4 lu_frag[];  // [MT][RC][hi / lo][rows g / g + 8][32]
+    __shared__ int rows[LM_ROWS];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     pdl_wait();
     pdl_launch_dependents();
-    if ((int)blockIdx.y >= *a.n_tiles) return;
     const int4 w = a.tiles[blockIdx.y];
-    const int rank = lora_rank(a, w.x), wide = (a.rank_max + 31) / 32 * 32, n0 = (blockIdx.x * LU_WARPS + warp) * 32, col = n0 + 8 * t4;
-    if (n0 >= a.N) return;
-    uint4 bv[4][RC];
-    lora_load_b<RC>(bv, a, w.x, rank, n0, lane);
+    if ((int)blockIdx.y >= *a.n_tiles) return;
+    const int rank = w.w, wide = (a.rank_max + 31) / 32 * 32, used = (rank + 31) / 32;
+    if (tid < LM_ROWS) rows[tid] = a.order[w.y + min(tid, w.z - 1)];
+    for (int i = tid; i < LM_MT * RC * 128; i += LU_WARPS * 32) {
+        const int l = i & 31, row = 16 * (i / (128 * RC)) + 8 * (i >> 5 & 1) + (l >> 2), r = 32 * (i / 128 % RC) + 8 * (l & 3);
+        // (columns behind the rank need not have been written)
+        lu_frag[i] = ldg16(a.low + ((long long)(w.y + row) * 2 + (i >> 6 & 1)) * wide + r, row < w.z && r < rank);
+    }
+    __syncthreads();
+    int n0 = (blockIdx.x * loops * LU_WARPS + warp) * 32, col = min(n0 + 8 * t4, a.N - 8);
+    long long at[LM_MT][2];  // the lane's rows
 #pragma unroll
-    for (int m = 0; m < LM_MT; ++m) {
-        if (16 * m >= w.z) break;
-        const int lo_row = 16 * m + g, hi_row = lo_row + 8;
-        const long long t_lo = lo_row < w.z ? a.order[w.y + lo_row] : -1, t_hi = hi_row < w.z ? a.order[w.y + hi_row] : -1;
-        const Base8 b0 = lora_base(a, t_lo * a.N + col, t_lo >= 0 && col < a.N), b1 = lora_base(a, t_hi * a.N + col, t_hi >= 0 && col < a.N);
-        float acc[4][4] = {};
+    for (int m = 0; m < LM_MT; ++m)
 #pragma unroll
-        for (int c = 0; c < RC; ++c)
+        for (int i = 0; i < 2; ++i) at[m][i] = (long long)rows[16 * m + 8 * i + g] * a.N;
+    const int parts = (w.z + 15) / 16;
+    uint4 raw[LM_MT][2][F32 ? 2 : 1];
+    auto fetch = [&](int m, int c) {
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                const bool on = 32 * c + 8 * t4 < rank;  // (columns behind it need not have been written)
-                const uint16_t *l = a.low + (long long)(w.y + lo_row) * 2 * wide + p * wide + 32 * c + 8 * t4;
-                const uint4 u = ldg16(l, on && t_lo >= 0), v = ldg16(l + 16 * wide, on && t_hi >= 0);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int k = 0; k < (F32 ? 2 : 1); ++k)
+                raw[m][i][k] = F32 ? reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(a.base) + at[m][i] + c)[k]
+                                   : *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.base) + at[m][i] + c);
+    };
+#pragma unroll
+    for (int m = 0; m < LM_MT; ++m)
+        if (m < parts) fetch(m, col);
+    for (int l = 0; l < loops && n0 < a.N; ++l) {
+        uint4 bv[4][RC];
+        lora_load_b<RC>(bv, a, w.x, rank, n0, lane);
+        const bool here = n0 + 8 * t4 < a.N;
+        const int this_col = col;
+        n0 += 32 * LU_WARPS;
+        const bool more = l + 1 < loops && n0 < a.N;
+        if (more) col = min(n0 + 8 * t4, a.N - 8);
+#pragma unroll
+        for (int m = 0; m < LM_MT; ++m) {
+            if (m >= parts) break;
+            float acc[4][4];  // base, then the sums
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
-                    mma_bf16_16816(acc[b], u.x, v.x, u.y, v.y, bv[b][c].x, bv[b][c].y);
-                    mma_bf16_16816(acc[b], u.z, v.z, u.w, v.w, bv[b][c].z, bv[b][c].w);
+                    const uint4 u = raw[m][i][F32 ? b >> 1 : 0];
+                    if (F32) {
+                        acc[b][2 * i] = __uint_as_float(b & 1 ? u.z : u.x), acc[b][2 * i + 1] = __uint_as_float(b & 1 ? u.w : u.y);
+                    } else {
+                        const uint32_t e = b == 0 ? u.x : b == 1 ? u.y : b == 2 ? u.z : u.w;
+                        acc[b][2 * i] = bf16x2_lo(e), acc[b][2 * i + 1] = bf16x2_hi(e);
+                    }
+                }
+            if (more) fetch(m, col);
+#pragma unroll
+            for (int c = 0; c < RC; ++c) {
+                if (c >= used) break;
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const uint4 u = lu_frag[((m * RC + c) * 2 + p) * 64 + lane], v = lu_frag[((m * RC + c) * 2 + p) * 64 + 32 + lane];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        mma_bf16_16816(acc[b], u.x, v.x, u.y, v.y, bv[b][c].x, bv[b][c].y);
+                        mma_bf16_16816(acc[b], u.z, v.z, u.w, v.w, bv[b][c].z, bv[b][c].w);
+                    }
                 }
             }
-        if (col < a.N) {
-            const float u[8] = {acc[0][0], acc[0][1], acc[1][0], acc[1][1], acc[2][0], acc[2][1], acc[3][0], acc[3][1]};
-            const float v[8] = {acc[0][2], acc[0][3], acc[1][2], acc[1][3], acc[2][2], acc[2][3], acc[3][2], acc[3][3]};
-            if (t_lo >= 0) lora_store(a, t_lo * a.N + col, b0, u);
-            if (t_hi >= 0) lora_store(a, t_hi * a.N + col, b1, v);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (!here || 16 * m + 8 * i + g >= w.z) continue;
+                const long long o = at[m][i] + this_col;
+                if (a.residual) {
+                    const uint4 u = *reinterpret_cast<const uint4 *>(a.residual + o);
+                    const uint32_t e[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) acc[b][2 * i] += bf16x2_lo(e[b]), acc[b][2 * i + 1] += bf16x2_hi(e[b]);
+                }
+                *reinterpret_cast<uint4 *>(a.out + o) = make_uint4(pack16x2<false>(acc[0][2 * i], acc[0][2 * i + 1]), pack16x2<false>(acc[1][2 * i], acc[1][2 * i + 1]),
+                                                                   pack16x2<false>(acc[2][2 * i], acc[2][2 * i + 1]), pack16x2<false>(acc[3][2 * i], acc[3][2 * i + 1]));
+            }
         }
     }
 }
@@ -438,10 +531,35 @@ size_t lora_scratch_bytes() {
 
 template <int NB>
 static int launch_lora_down(const LoraArgs &a, int tiles, cudaStream_t stream) {
-    const int smem = LD_WARPS * LM_ROWS * (8 * NB + 4) * 4;
+    constexpr int stages = LD_STAGES * (LM_ROWS + 16 * NB) * 2 * LD_STAGE, sums = LD_WARPS / 2 * LM_ROWS * (16 * NB + 4) * 4, smem = stages > sums ? stages : sums;
     int rc = check_cuda(cudaFuncSetAttribute(lora_down_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "lora shared memory");
     if (rc) return rc;
-    return check_cuda(launch_pdl(lora_down_kernel<NB>, dim3(tiles * LD_CLUSTER), dim3(LD_WARPS * 32), smem, stream, a), "lora down launch");
+    // as many shares of K as let every CTA be resident at once
+    const int busy = (a.T + LM_ROWS - 1) / LM_ROWS, most = 2 * device_sm_count();
+    const int n_ctas = busy * 8 <= most ? 8 : busy * 4 <= most ? 4 : busy * 2 <= most ? 2 : 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(tiles * n_ctas);
+    cfg.blockDim = dim3(LD_WARPS * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim = {(unsigned)n_ctas, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return check_cuda(cudaLaunchKernelEx(&cfg, lora_down_kernel<NB>, a), "lora down launch");
+}
+template <int RC>
+static int launch_lora_up(const LoraArgs &a, int tiles, cudaStream_t stream) {
+    // as many columns a CTA as leave four CTAs to each of the four places on an SM
+    const int blocks = (a.N + 32 * LU_WARPS - 1) / (32 * LU_WARPS), busy = (a.T + LM_ROWS - 1) / LM_ROWS;
+    const int loops = max(1, min(16, (int)((long long)blocks * busy / (16 * device_sm_count()))));
+    const dim3 grid((blocks + loops - 1) / loops, tiles), block(LU_WARPS * 32);
+    const int smem = LM_MT * RC * 128 * 16;
+    auto kernel = a.base_f32 ? lora_up_kernel<RC, true> : lora_up_kernel<RC, false>;
+    return check_cuda(launch_pdl(kernel, grid, block, smem, stream, a, loops), "lora up launch");
 }
 
 static int launch_lora(LoraArgs a, cudaStream_t stream) {
@@ -462,11 +580,10 @@ static int launch_lora(LoraArgs a, cudaStream_t stream) {
     int rc = check_cuda(launch_pdl(lora_group_kernel, dim3(1), dim3(LG_THREADS), smem, stream, a), "lora group launch");
     if (rc) return rc;
     if (a.n > 0) {
-        rc = a.rank_max <= 16 ? launch_lora_down<2>(a, tiles, stream) : a.rank_max <= 32 ? launch_lora_down<4>(a, tiles, stream) : launch_lora_down<8>(a, tiles, stream);
+        rc = a.rank_max <= 16 ? launch_lora_down<1>(a, tiles, stream) : a.rank_max <= 32 ? launch_lora_down<2>(a, tiles, stream) : launch_lora_down<4>(a, tiles, stream);
         if (rc) return rc;
     }
-    auto up = rc32 == 1 ? lora_up_kernel<1> : rc32 == 2 ? lora_up_kernel<2> : lora_up_kernel<4>;
-    return check_cuda(launch_pdl(up, dim3((a.N + 32 * LU_WARPS - 1) / (32 * LU_WARPS), tiles), dim3(LU_WARPS * 32), 0, stream, a), "lora up launch");
+    return rc32 == 1 ? launch_lora_up<1>(a, tiles, stream) : rc32 == 2 ? launch_lora_up<2>(a, tiles, stream) : launch_lora_up<4>(a, tiles, stream);
 }
 
 }  // namespace awq
