@@ -22,6 +22,7 @@ struct AttendArgs {
     long long o_row, o_head;
     float scale_log2;  // scale / ln 2: the exponentials are powers of two
     int R, T, n_heads, table_width;
+    int page_shift;    // log2 of the page size, -1: not a power of two
     RequestHeader *header;
     uint8_t *scratch;
 };
@@ -42,6 +43,13 @@ __device__ __forceinline__ AttendRequest attend_request(const AttendArgs &a, int
     if (q.n > capacity) q.n = 0;
     return q;
 }
+
+__device__ __forceinline__ float exp2_fast(float x) {  // 2 units in the last place
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ int page_index(const AttendArgs &a, int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / a.cache.page_size; }
 
 // Any head size: a warp per row and head, one key after another.  Head sizes that have no tensor-core kernel.
 template <bool F16>
@@ -123,26 +131,31 @@ __global__ void __launch_bounds__(128) tree_attention_any_kernel(AttendArgs a) {
 // a segment that several CTAs share is joined by the last of them to finish, in the order of its keys, so no CTA waits and
 // results do not depend on timing.
 //
-// Inside a tile every warp has 16 keys of its own and keeps its own running maximum and sum.  K and V go from global memory to
-// the registers in which mma.sync wants them, without shared memory:
-//   scores: the order of the products over the head is free, so a lane's 16 bytes of a key are its operands of two k-steps
-//           if the rows of Q are taken in the same order;
-//   output: a lane loads 16 bytes of four keys (its k-indices) and pairs them up with byte permutes; column n of block j is
-//           then head element 8 n + j, so that a lane's results are 16 neighbours.
+// Inside a tile every warp has 16 keys of its own and keeps its own running maximum and sum.  K and V come in by asynchronous
+// copies into shared memory of the warp's own, two blocks ahead, so that 12 warps an SM have up to 190 KB on their way.  Eight
+// lanes fetch 128 bytes of a key at once: requests of half a line, which a lane's own pieces would be, are what the L2's tags
+// run out of first.  In shared memory the pieces lie where mma.sync's lanes find them without bank conflicts:
+//   scores: the order of the products over the head is free, so 16 bytes of a key are a lane's operands of two k-steps if the
+//           rows of Q are taken in the same order; odd keys have the halves of their lines swapped;
+//   output: a lane has 16 bytes of four keys (its k-indices) and pairs them up with byte permutes; column n of block j is then
+//           head element 8 n + j, so that a lane's results are 16 neighbours; pieces are shifted by pairs of keys.
 // Weights are multiplied as two 16-bit pieces, p = hi + lo: the tensor cores have time to spare, and the result keeps the
 // accuracy of f32 weights.
 // =====================================================================================
 constexpr int AR_WARPS = 4, AR_TILE = AR_WARPS * 16, AR_PER_SM = 3, AR_ROWS = 16;
 constexpr int AR_MAX_CTAS = 192 * AR_PER_SM;
 
-__device__ __forceinline__ uint4 ldg_stream(const uint16_t *p, bool on) {
-    uint4 v;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
-        "@p ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
-        : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
-        : "l"(p), "r"((int)on));
-    return v;
+template <int TO, int FROM>  // at fixed distances (bytes) from dst and src; zeros where bytes is 0, not 16
+__device__ __forceinline__ void copy16(uint32_t dst, const uint16_t *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %4], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(TO), "n"(FROM) : "memory");
+}
+// N copies, the i-th at i TO and i FROM.
+template <int N, int TO, int FROM, int I = 0>
+__device__ __forceinline__ void copies16(uint32_t dst, const uint16_t *src, int bytes) {
+    if constexpr (I < N) {
+        copy16<I * TO, I * FROM>(dst, src, bytes);
+        copies16<N, TO, FROM, I + 1>(dst, src, bytes);
+    }
 }
 template <bool F16>
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -206,19 +219,32 @@ __device__ __forceinline__ int request_of_unit(const long long *cum, int n, long
     return lo;
 }
 
-// Shared memory: cum | Q in operand order | key offsets | the warps' results
+// Shared memory: Q in operand order | places of the keys | K and V, later the warps' results | tiles before each request
+constexpr int AR_PLACES = 4 * 16 * 16 + 64;  // of a warp: four blocks of 16 keys, and which of them there are (stages start on 128 bytes)
 template <int D>
-constexpr int AR_SMEM = D * 32 + AR_WARPS * 2 * 16 * 16 + AR_WARPS * AR_ROWS * (D + 2) * 4;
+constexpr int AR_STAGE = 16 * D * 4;  // K and V of a warp's block
+template <int D>
+constexpr int AR_STAGES = AR_WARPS * (2 * AR_STAGE<D> > AR_ROWS * (D + 2) * 4 ? 2 * AR_STAGE<D> : AR_ROWS * (D + 2) * 4);
+template <int D>
+constexpr int AR_SMEM = D * 32 + AR_WARPS * AR_PLACES + AR_STAGES<D>;
 
 template <bool F16, int D>
 __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_kernel(AttendArgs a, int min_units) {
     constexpr int THREADS = AR_WARPS * 32, QC = D / 32, VC = D / 64;
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-    uint4 *qs = reinterpret_cast<uint4 *>(smem);                                     // [QC][2][32]
-    longlong2 *offs = reinterpret_cast<longlong2 *>(smem + D * 32) + warp * 32;       // [2][16] of this warp
-    float *ow = reinterpret_cast<float *>(smem + D * 32 + AR_WARPS * 512);            // [WARPS][16][D]
-    float *mw = ow + AR_WARPS * AR_ROWS * D, *lw = mw + AR_WARPS * AR_ROWS;            // [WARPS][16]
+    uint4 *qs = reinterpret_cast<uint4 *>(smem);  // [QC][2][32]
+    longlong2 *places = reinterpret_cast<longlong2 *>(smem + D * 32 + warp * AR_PLACES);
+    uint32_t *there = reinterpret_cast<uint32_t *>(places + 64);
+    uint8_t *stages = smem + D * 32 + AR_WARPS * AR_PLACES;
+    uint8_t *mine = stages + warp * 2 * AR_STAGE<D>;  // [2][K [16][D], V [16][D]]
+    // copies: lane l brings pieces l % 8 (and l % 8 + 8) of keys l / 8 + 4 i
+    const int ck = lane >> 3, cp = lane & 7;
+    const uint32_t copy_k = smem_u32(mine) + ck * 2 * D + (cp ^ ((ck & 1) << 2)) * 16;
+    const uint32_t copy_v = smem_u32(mine) + 32 * D + ck * 2 * D;  // + the piece, in its place for even and odd i
+    const uint32_t piece_v[2] = {(uint32_t)(cp ^ (ck & 2)) * 16, (uint32_t)(cp ^ (ck & 2) ^ 4) * 16};
+    float *ow = reinterpret_cast<float *>(stages);                           // [WARPS][16][D]
+    float *mw = ow + AR_WARPS * AR_ROWS * D, *lw = mw + AR_WARPS * AR_ROWS;   // [WARPS][16]
     long long *cum = reinterpret_cast<long long *>(smem + AR_SMEM<D>);
     __shared__ int s_last;
     pdl_wait();
@@ -241,7 +267,48 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
         const long long seg_start = x - tile0, seg_end = seg_start + n_tiles;
         const int tiles = (int)(min(end, seg_end) - x);
         const int32_t *table = a.table + r * a.table_stride;
-        const uint16_t *kbase = a.cache.k + hk * a.cache.k_head, *vbase = a.cache.v + hk * a.cache.v_head;
+        const uint16_t *kbase = a.cache.k + hk * a.cache.k_head + 8 * cp, *vbase = a.cache.v + hk * a.cache.v_head + 8 * cp;
+
+        // a lane looks after one key of two blocks: its page, then its place in K and V (negative: none)
+        const int first = tile0 * AR_TILE + warp * 16;
+        auto page_of = [&](int i) {
+            const int key = first + (i + (lane >> 4)) * AR_TILE + (lane & 15);
+            return i + (lane >> 4) < tiles && key < total ? __ldg(table + page_index(a, key)) : -2;
+        };
+        auto place = [&](int i, int page) {  // i even
+            const int key = first + (i + (lane >> 4)) * AR_TILE + (lane & 15), off = key - page_index(a, key) * page_size;
+            const bool ok = (unsigned)page < (unsigned)a.cache.n_pages;
+            if (!ok && page != -2) req_error(&a.header->error, REQ_ERR_PAGE);
+            if (page == -2 && i + (lane >> 4) < tiles && key < total) req_error(&a.header->error, REQ_ERR_PAGE);
+            places[(i & 2) * 16 + lane] =
+                ok ? make_longlong2(page * a.cache.k_page + off * a.cache.k_slot, page * a.cache.v_page + off * a.cache.v_slot) : make_longlong2(-8, -8);
+            const uint32_t b = __ballot_sync(0xffffffffu, ok);
+            if (lane == 0) there[(i & 2) >> 1] = b;
+            __syncwarp();
+        };
+        auto load_k = [&](int i) {
+            __syncwarp();  // the block that was here has been read
+            if (i < tiles)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const long long o = places[(i & 3) * 16 + 4 * q + ck].x;
+                    copies16<D / 64, 128, 128>(copy_k + (i & 1) * AR_STAGE<D> + q * 8 * D, kbase + o, o < 0 ? 0 : 16);
+                }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        auto load_v = [&](int i) {
+            __syncwarp();
+            if (i < tiles)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const long long o = places[(i & 3) * 16 + 4 * q + ck].y;
+                    copies16<D / 64, 128, 128>(copy_v + piece_v[q & 1] + (i & 1) * AR_STAGE<D> + q * 8 * D, vbase + o, o < 0 ? 0 : 16);
+                }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        __syncthreads();  // the previous segment's readers of shared memory are done
+        const int page0 = page_of(0);
+        int next_page = page_of(2);
         // this lane's rows, g and g + 8: token and mask
         int j[2];
         unsigned long long bits[2];
@@ -253,11 +320,15 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
             bits[i] = a.mask && j[i] >= 0 ? (unsigned long long)a.mask[rq.q0 + j[i]] : 0;
             qrow[i] = a.q + (long long)(rq.q0 + max(j[i], 0)) * a.q_row + (long long)(hk * group + row % group) * a.q_head;
         }
-        __syncthreads();  // the previous segment's readers of shared memory are done
         for (int c = warp; c < QC; c += AR_WARPS)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 qs[(c * 2 + i) * 32 + lane] = j[i] >= 0 ? *reinterpret_cast<const uint4 *>(qrow[i] + 32 * c + 8 * t4) : make_uint4(0, 0, 0, 0);
+        place(0, page0);
+        load_k(0);
+        load_v(0);
+        load_k(1);
+        load_v(1);
         __syncthreads();
 
         float acc[VC][8][4];
@@ -268,142 +339,66 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[c][b][e] = 0.f;
         float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
-
-        // lane l < 16 looks after key l of a block: its page, then its place in K and V
-        const int first = tile0 * AR_TILE + warp * 16;
-        auto page_of = [&](int i) {
-            const int key = first + i * AR_TILE + lane;
-            return lane < 16 && i < tiles && key < total ? __ldg(table + key / page_size) : -1;
-        };
-        auto place = [&](int i, int page) {  // returns the block's valid keys
-            const int key = first + i * AR_TILE + lane;
-            bool ok = false;
-            if (lane < 16) {
-                const int off = key % page_size;
-                ok = (unsigned)page < (unsigned)a.cache.n_pages;
-                if (!ok && i < tiles && key < total) req_error(&a.header->error, REQ_ERR_PAGE);
-                offs[(i & 1) * 16 + lane] = ok ? make_longlong2(page * a.cache.k_page + off * a.cache.k_slot, page * a.cache.v_page + off * a.cache.v_slot)
-                                               : make_longlong2(-1, -1);
-            }
-            __syncwarp();
-            return __ballot_sync(0xffffffffu, ok) & 0xffffu;
-        };
-        uint4 kr[2][QC], vr[VC][4];
-        auto load_k = [&](int i) {
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const long long o = offs[(i & 1) * 16 + 8 * b + g].x;
-#pragma unroll
-                for (int c = 0; c < QC; ++c) kr[b][c] = ldg_stream(kbase + o + 32 * c + 8 * t4, o >= 0);
-            }
-        };
-        auto load_v = [&](int i) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const long long o = offs[(i & 1) * 16 + 2 * t4 + (e & 1) + 8 * (e >> 1)].y;
-#pragma unroll
-                for (int c = 0; c < VC; ++c) vr[c][e] = ldg_stream(vbase + o + 64 * c + 8 * g, o >= 0);
-            }
-        };
-        uint32_t valid = place(0, page_of(0));
-        load_k(0);
-        load_v(0);
-        int next_page = page_of(1);
         for (int i = 0; i < tiles; ++i) {
-            const int page2 = page_of(i + 2);
+            if ((i & 1) == 0) {
+                place(i + 2, next_page);
+                next_page = page_of(i + 4);
+            }
+            const uint8_t *stage = mine + (i & 1) * AR_STAGE<D>;
+            const uint8_t *ks = stage + g * 2 * D + t4 * 16, *vs = stage + 32 * D + 4 * D * t4 + (g ^ (2 * t4)) * 16;
+            const int swap = (g & 1) * 64;
+            asm volatile("cp.async.wait_group 3;" ::: "memory");
+            __syncwarp();
             float s[2][4] = {};
 #pragma unroll
             for (int c = 0; c < QC; ++c) {
                 const uint4 q0 = qs[(c * 2) * 32 + lane], q1 = qs[(c * 2 + 1) * 32 + lane];
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
-                    mma16<F16>(s[b], q0.x, q1.x, q0.y, q1.y, kr[b][c].x, kr[b][c].y);
-                    mma16<F16>(s[b], q0.z, q1.z, q0.w, q1.w, kr[b][c].z, kr[b][c].w);
+                    const uint4 k = *reinterpret_cast<const uint4 *>(ks + 16 * D * b + (64 * c ^ swap));
+                    mma16<F16>(s[b], q0.x, q1.x, q0.y, q1.y, k.x, k.y);
+                    mma16<F16>(s[b], q0.z, q1.z, q0.w, q1.w, k.z, k.w);
                 }
             }
-            const uint32_t valid_next = place(i + 1, next_page);
-            next_page = page2;
-            load_k(i + 1);
+            load_k(i + 2);
             const int key0 = first + i * AR_TILE;
+            const uint32_t valid = there[(i & 2) >> 1] >> (16 * (i & 1)) & 0xffffu;
             const bool partly = key0 + 16 > rq.len || valid != 0xffffu;
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    s[b][e] *= a.scale_log2;
-                    if (partly) {
+                for (int e = 0; e < 4; ++e) s[b][e] *= a.scale_log2;
+            if (partly) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
                         const int c = 8 * b + 2 * t4 + (e & 1), d = key0 + c - rq.len;
                         const bool seen = (valid >> c & 1) && (d < 0 || (a.mask ? d < 64 && (bits[e >> 1] >> d & 1) : d <= j[e >> 1]));
                         if (!seen) s[b][e] = -INFINITY;
                     }
-                }
+            }
+            // The weights refer to a maximum that may lie 8 behind: they stay below 2^8, and the sums are rarely rescaled.
             float p[2][4];
 #pragma unroll
             for (int i2 = 0; i2 < 2; ++i2) {
                 float m = fmaxf(fmaxf(s[0][2 * i2], s[0][2 * i2 + 1]), fmaxf(s[1][2 * i2], s[1][2 * i2 + 1]));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                m = fmaxf(m, top[i2]);
-                const float ref = m == -INFINITY ? 0.f : m, keep = exp2f(top[i2] - ref);
-                top[i2] = m;
-                float add = 0.f;
-#pragma unroll
-                for (int b = 0; b < 2; ++b)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) add += p[b][2 * i2 + e] = exp2f(s[b][2 * i2 + e] - ref);
-                sum[i2] = sum[i2] * keep + add;
-                if (__any_sync(0xffffffffu, keep != 1.f)) {
+                if (__any_sync(0xffffffffu, m > top[i2] + 8.f)) {
+                    const float to = fmaxf(m, top[i2]), keep = to == -INFINITY ? 1.f : exp2_fast(top[i2] - to);
+                    top[i2] = to;
+                    sum[i2] *= keep;
 #pragma unroll
                     for (int c = 0; c < VC; ++c)
 #pragma unroll
                         for (int b = 0; b < 8; ++b) acc[c][b][2 * i2] *= keep, acc[c][b][2 * i2 + 1] *= keep;
                 }
-            }
-            // a value that some rows do not see must not reach them as 0 times infinity or NaN
-            if (partly) {
-                bool odd = false;
+                const float ref = top[i2] == -INFINITY ? 0.f : top[i2];
 #pragma unroll
-                for (int c = 0; c < VC; ++c)
+                for (int b = 0; b < 2; ++b)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        odd = odd || not_finite16x2<F16>(vr[c][e].x) || not_finite16x2<F16>(vr[c][e].y) || not_finite16x2<F16>(vr[c][e].z) ||
-                              not_finite16x2<F16>(vr[c][e].w);
-                if (__any_sync(0xffffffffu, odd)) {
-                    for (int key = 0; key < 16; ++key) {
-                        const long long o = offs[(i & 1) * 16 + key].y;
-                        if (o < 0) continue;  // (loaded as zero)
-                        // the weights of rows g and g + 8 for this key
-                        float w[2];
-#pragma unroll
-                        for (int i2 = 0; i2 < 2; ++i2) {
-                            const float w0 = __shfl_sync(0xffffffffu, p[0][2 * i2], (lane & 28) + ((key & 7) >> 1)), w1 = __shfl_sync(0xffffffffu, p[0][2 * i2 + 1], (lane & 28) + ((key & 7) >> 1));
-                            const float w2 = __shfl_sync(0xffffffffu, p[1][2 * i2], (lane & 28) + ((key & 7) >> 1)), w3 = __shfl_sync(0xffffffffu, p[1][2 * i2 + 1], (lane & 28) + ((key & 7) >> 1));
-                            w[i2] = key < 8 ? (key & 1 ? w1 : w0) : (key & 1 ? w3 : w2);
-                        }
-#pragma unroll
-                        for (int c = 0; c < VC; ++c)
-                            for (int d = 0; d < 16; ++d) {
-                                const uint32_t bitsv = (vbase + o)[64 * c + 16 * t4 + d];
-                                if (!not_finite16x2<F16>(bitsv)) continue;
-                                const float v = unpack16x2<F16>(bitsv).x;
-#pragma unroll
-                                for (int b = 0; b < 8; ++b)
-#pragma unroll
-                                    for (int e = 0; e < 4; ++e)
-                                        if (d == 8 * (e & 1) + b && w[e >> 1] != 0.f) acc[c][b][e] += w[e >> 1] * v;
-                            }
-                    }
-                    auto clean = [](uint32_t v) {
-                        if (not_finite16x2<F16>(v & 0xffffu)) v &= 0xffff0000u;
-                        if (not_finite16x2<F16>(v >> 16)) v &= 0xffffu;
-                        return v;
-                    };
-#pragma unroll
-                    for (int c = 0; c < VC; ++c)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            vr[c][e] = make_uint4(clean(vr[c][e].x), clean(vr[c][e].y), clean(vr[c][e].z), clean(vr[c][e].w));
-                }
+                    for (int e = 0; e < 2; ++e) sum[i2] += p[b][2 * i2 + e] = exp2_fast(s[b][2 * i2 + e] - ref);
             }
             uint32_t hi[4], lo[4];  // rows g, g + 8 of keys 0-7, then of keys 8-15
 #pragma unroll
@@ -415,10 +410,26 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
                     const float2 h = unpack16x2<F16>(hi[2 * b + i2]);
                     lo[2 * b + i2] = pack16x2<F16>(p0 - h.x, p1 - h.y);
                 }
+            asm volatile("cp.async.wait_group 3;" ::: "memory");
+            __syncwarp();
+            bool odd = false;
+            if (partly) {  // a value that some rows do not see must not reach them as 0 times infinity or NaN
+#pragma unroll 1
+                for (int w = 0; w < 16 * VC; ++w) {  // (the pieces this lane reads below)
+                    uint32_t &u = reinterpret_cast<uint32_t *>(const_cast<uint8_t *>(vs) + (w >> 2 & 1) * 2 * D + (w >> 3 & 1) * 16 * D + (w >> 4) * 128)[w & 3];
+                    if (!not_finite16x2<F16>(u)) continue;
+                    odd = true;
+                    u &= (not_finite16x2<F16>(u & 0xffffu) ? 0xffff0000u : 0xffffffffu) & (not_finite16x2<F16>(u >> 16) ? 0xffffu : 0xffffffffu);
+                }
+            }
 #pragma unroll
             for (int c = 0; c < VC; ++c) {
-                const uint32_t v[4][4] = {{vr[c][0].x, vr[c][0].y, vr[c][0].z, vr[c][0].w}, {vr[c][1].x, vr[c][1].y, vr[c][1].z, vr[c][1].w},
-                                          {vr[c][2].x, vr[c][2].y, vr[c][2].z, vr[c][2].w}, {vr[c][3].x, vr[c][3].y, vr[c][3].z, vr[c][3].w}};
+                uint32_t v[4][4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint4 u = *reinterpret_cast<const uint4 *>(vs + (e & 1) * 2 * D + (e >> 1) * 16 * D + c * 128);
+                    v[e][0] = u.x, v[e][1] = u.y, v[e][2] = u.z, v[e][3] = u.w;
+                }
 #pragma unroll
                 for (int b = 0; b < 8; ++b) {
                     const uint32_t sel = b & 1 ? 0x7632u : 0x5410u;
@@ -427,9 +438,35 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
                     mma16<F16>(acc[c][b], lo[0], lo[1], lo[2], lo[3], b0, b1);
                 }
             }
-            load_v(i + 1);
-            valid = valid_next;
+            if (partly && __any_sync(0xffffffffu, odd)) {  // the rows that do see it, key by key
+                for (int key = 0; key < 16; ++key) {
+                    const long long o = places[(i & 3) * 16 + key].y;
+                    const int from = (lane & 28) + ((key & 7) >> 1);
+                    float w[2];  // the weights of rows g and g + 8
+#pragma unroll
+                    for (int i2 = 0; i2 < 2; ++i2) {
+                        const float w0 = __shfl_sync(0xffffffffu, p[0][2 * i2], from), w1 = __shfl_sync(0xffffffffu, p[0][2 * i2 + 1], from);
+                        const float w2 = __shfl_sync(0xffffffffu, p[1][2 * i2], from), w3 = __shfl_sync(0xffffffffu, p[1][2 * i2 + 1], from);
+                        w[i2] = key < 8 ? (key & 1 ? w1 : w0) : (key & 1 ? w3 : w2);
+                    }
+                    if (o < 0) continue;  // (zeros)
+#pragma unroll
+                    for (int c = 0; c < VC; ++c)
+#pragma unroll
+                        for (int d = 0; d < 16; ++d) {
+                            const uint32_t bitsv = (vbase - 8 * cp + o)[64 * c + 16 * t4 + d];
+                            if (!not_finite16x2<F16>(bitsv)) continue;
+                            const float v = unpack16x2<F16>(bitsv).x;
+#pragma unroll
+                            for (int i2 = 0; i2 < 2; ++i2)
+                                if (w[i2] != 0.f) acc[c][d & 7][2 * i2 + (d >> 3)] += w[i2] * v;
+                        }
+                }
+            }
+            load_v(i + 2);
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();  // the warps' results take the stages' place
         // ---- join the warps ----
 #pragma unroll
         for (int i2 = 0; i2 < 2; ++i2) {
@@ -450,31 +487,28 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
         const int c0 = (int)(seg_start / per), c1 = (int)((seg_end - 1) / per), rows = min(AR_ROWS, rq.n * group - row0);
         const bool whole = c0 == c1;
         float *part = parts + (long long)(2 * blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0)) * PART;
-        auto store = [&](int row, int d, const float (&o)[8], float total_w) {
+        auto store = [&](int row, int d, const float (&o)[4], float total_w) {
             const float inv = total_w == 0.f ? 0.f : 1.f / total_w;
             uint16_t *dst = a.out + (long long)(rq.q0 + (row0 + row) / group) * a.o_row + (long long)(hk * group + (row0 + row) % group) * a.o_head + d;
-            *reinterpret_cast<uint4 *>(dst) = make_uint4(pack16x2<F16>(o[0] * inv, o[1] * inv), pack16x2<F16>(o[2] * inv, o[3] * inv),
-                                                         pack16x2<F16>(o[4] * inv, o[5] * inv), pack16x2<F16>(o[6] * inv, o[7] * inv));
+            *reinterpret_cast<uint2 *>(dst) = make_uint2(pack16x2<F16>(o[0] * inv, o[1] * inv), pack16x2<F16>(o[2] * inv, o[3] * inv));
         };
-        for (int i = tid; i < rows * (D / 8); i += THREADS) {
-            const int row = i / (D / 8), d = 8 * (i % (D / 8));
-            float m = -INFINITY, l = 0.f, o[8] = {};
+        for (int i = tid; i < rows * (D / 4); i += THREADS) {
+            const int row = i / (D / 4), d = 4 * (i % (D / 4));
+            float m = -INFINITY, l = 0.f, o[4] = {};
 #pragma unroll
             for (int w = 0; w < AR_WARPS; ++w) m = fmaxf(m, mw[w * 16 + row]);
 #pragma unroll
             for (int w = 0; w < AR_WARPS; ++w) {
-                const float mm = mw[w * 16 + row], f = mm == -INFINITY ? 0.f : exp2f(mm - m);
+                const float mm = mw[w * 16 + row], f = mm == -INFINITY ? 0.f : exp2_fast(mm - m);
                 l += f * lw[w * 16 + row];
                 if (f == 0.f) continue;
-                const float4 u = *reinterpret_cast<const float4 *>(ow + (w * 16 + row) * D + d), v = *reinterpret_cast<const float4 *>(ow + (w * 16 + row) * D + d + 4);
+                const float4 u = *reinterpret_cast<const float4 *>(ow + (w * 16 + row) * D + d);
                 o[0] += f * u.x, o[1] += f * u.y, o[2] += f * u.z, o[3] += f * u.w;
-                o[4] += f * v.x, o[5] += f * v.y, o[6] += f * v.z, o[7] += f * v.w;
             }
             if (whole) {
                 store(row, d, o, l);
             } else {
                 *reinterpret_cast<float4 *>(part + row * D + d) = make_float4(o[0], o[1], o[2], o[3]);
-                *reinterpret_cast<float4 *>(part + row * D + d + 4) = make_float4(o[4], o[5], o[6], o[7]);
                 if (d == 0) part[AR_ROWS * D + row] = m, part[AR_ROWS * D + AR_ROWS + row] = l;
             }
         }
@@ -485,21 +519,20 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
             __syncthreads();
             if (s_last) {
                 __threadfence();
-                for (int i = tid; i < rows * (D / 8); i += THREADS) {
-                    const int row = i / (D / 8), d = 8 * (i % (D / 8));
-                    float m = -INFINITY, l = 0.f, o[8] = {};
+                for (int i = tid; i < rows * (D / 4); i += THREADS) {
+                    const int row = i / (D / 4), d = 4 * (i % (D / 4));
+                    float m = -INFINITY, l = 0.f, o[4] = {};
+#pragma unroll 8
                     for (int c = c0; c <= c1; ++c) {
                         const float *src = parts + (long long)(2 * c + (c == c0 ? 1 : 0)) * PART;
                         const float mc = __ldcg(src + AR_ROWS * D + row), lc = __ldcg(src + AR_ROWS * D + AR_ROWS + row);
-                        const float4 u = __ldcg(reinterpret_cast<const float4 *>(src + row * D + d)), v = __ldcg(reinterpret_cast<const float4 *>(src + row * D + d + 4));
-                        const float m2 = fmaxf(m, mc);
-                        if (m2 == -INFINITY) continue;
-                        const float f = exp2f(m - m2), fc = exp2f(mc - m2);
+                        const float4 u = __ldcg(reinterpret_cast<const float4 *>(src + row * D + d));
+                        const float m2 = fmaxf(m, mc), ref = m2 == -INFINITY ? 0.f : m2, f = exp2_fast(m - ref), fc = exp2_fast(mc - ref);
                         m = m2;
                         l = l * f + lc * fc;
-                        const float add[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+                        const float add[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) o[e] = o[e] * f + (fc == 0.f ? 0.f : add[e] * fc);
+                        for (int e = 0; e < 4; ++e) o[e] = (f == 0.f ? 0.f : o[e] * f) + (fc == 0.f ? 0.f : add[e] * fc);
                     }
                     store(row, d, o, l);
                 }
@@ -537,7 +570,8 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
     AWQ_REQUIRE_REQUEST_WORKSPACE("tree_attention", workspace, workspace_bytes);
     const RequestWorkspaceView w = request_workspace(workspace);
     AttendArgs a{reinterpret_cast<const uint16_t *>(q), s[0], s[1], view, table, table_stride, lens, q_start, mask,
-                 reinterpret_cast<uint16_t *>(out), s[2], s[3], scale * 1.4426950408889634f, R, T, n_heads, table_width, w.header, w.attention};
+                 reinterpret_cast<uint16_t *>(out), s[2], s[3], scale * 1.4426950408889634f, R, T, n_heads, table_width,
+                 view.page_size & (view.page_size - 1) ? -1 : __builtin_ctz(view.page_size), w.header, w.attention};
     if (view.head_dim == 64 || view.head_dim == 128) {
         const bool f16 = cache->format == ACT_F16;
         auto kernel = view.head_dim == 64 ? (f16 ? tree_attention_rows_kernel<true, 64> : tree_attention_rows_kernel<false, 64>)
