@@ -8,6 +8,8 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include "awq_tcgen05.cuh"
+
 namespace awq {
 
 struct AttendArgs {
@@ -172,18 +174,18 @@ __device__ __forceinline__ bool not_finite16x2(uint32_t v) {
     return (v & e) == e || ((v >> 16) & e) == e;
 }
 
-// Tiles of all requests before each one, in shared memory; returns their number.  Requests that do not fit are reported by
+// Units of all requests before each one, in shared memory; returns their number.  Requests that do not fit are reported by
 // CTA 0 and have what attend_request leaves of them.
-template <int THREADS>
-__device__ __forceinline__ long long scan_units(const AttendArgs &a, long long *cum, int rows_per_segment, int tile) {
+template <int THREADS, typename F>
+__device__ __forceinline__ long long scan_units(const AttendArgs &a, long long *cum, F units_of) {
     __shared__ long long sums[THREADS / 32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, group = a.n_heads / a.cache.n_kv;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (a.R + THREADS - 1) / THREADS, r0 = min(tid * per, a.R), r1 = min(r0 + per, a.R);
     long long mine = 0;
     for (int r = r0; r < r1; ++r) {
         const AttendRequest q = attend_request(a, r);
         if (q.bad && blockIdx.x == 0) req_error(&a.header->error, REQ_ERR_REQUEST);
-        const long long units = (((long long)q.n * group + rows_per_segment - 1) / rows_per_segment) * a.cache.n_kv * ((q.len + q.n + tile - 1) / tile);
+        const long long units = q.n ? units_of(q) : 0;
         cum[r] = units;
         mine += units;
     }
@@ -249,11 +251,14 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
     __shared__ int s_last;
     pdl_wait();
     pdl_launch_dependents();
-    const long long units = scan_units<THREADS>(a, cum, AR_ROWS, AR_TILE);
+    const int group = a.n_heads / a.cache.n_kv;
+    const long long units = scan_units<THREADS>(a, cum, [&](const AttendRequest &q) {
+        return (((long long)q.n * group + AR_ROWS - 1) / AR_ROWS) * a.cache.n_kv * ((q.len + q.n + AR_TILE - 1) / AR_TILE);
+    });
     const long long per = max((units + gridDim.x - 1) / gridDim.x, (long long)min_units);
     long long x = blockIdx.x * per;
     const long long end = min(x + per, units);
-    const int group = a.n_heads / a.cache.n_kv, page_size = a.cache.page_size;
+    const int page_size = a.cache.page_size;
     float *parts = reinterpret_cast<float *>(a.scratch + 4 * AR_MAX_CTAS);
     int *counters = reinterpret_cast<int *>(a.scratch);
     constexpr int PART = AR_ROWS * (D + 2);
@@ -543,7 +548,423 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
     }
 }
 
-size_t tree_attention_scratch_bytes() { return 4 * AR_MAX_CTAS + (size_t)2 * AR_MAX_CTAS * AR_ROWS * (128 + 2) * 4; }
+// =====================================================================================
+// Many rows per cache head (trees, prompts): tcgen05, 128 rows at a time.
+//
+// A unit of work is 128 keys of a segment = (request, cache head, 128 rows), split over the CTAs and joined as above.  Two CTAs an SM;
+// in each
+//   2 warps  copy K and V (16-byte asynchronous copies, whole lines) into the 128-byte swizzle, one each;
+//   1 warp   issues the products: S = Q K^T into 128 columns of tensor memory, O += P V into D others;
+//   4 warps  hold a row per thread: maximum, weights, and P as 16-bit pairs over S's own columns, from where the tensor cores take
+//            it as the left operand of the next product.
+// K and V are held once: K of the next tile is fetched while the weights of this one are formed, V while the scores are.  What
+// one CTA leaves idle (the tensor cores during its softmax, the exponentials during its products) is the other one's.  O stays in
+// tensor memory; it is rescaled only when a maximum has grown by more than 8 (powers of two), by the warp that finds it.
+// Weights are rounded to the rows' 16-bit type for the product, as they have to be for one tensor-core operand (their sum is
+// not): half a step per weight, independent from key to key.
+// =====================================================================================
+constexpr int AT_ROWS = 128, AT_TILE = 128, AT_THREADS = 7 * 32, AT_PER_SM = 2, AT_MAX_CTAS = 192 * AT_PER_SM, AT_COLS = 256;
+static_assert(AT_MAX_CTAS <= AR_MAX_CTAS, "the counters of both kernels share their place");
+struct AttendTilesShared {
+    uint64_t k_full, v_full, scored, added, weighed, q_full, summed;  // mbarriers: K, V there; QK^T, PV done; P there; Q there, O done (segment)
+    uint32_t tmem;
+    int last, odd[2];
+    uint32_t valid[2][4];         // of a tile: which of its keys there are
+    long long places[2][128];     // of a copying warp: the keys of its tile
+};
+template <int D>
+constexpr int AT_OPERAND = AT_TILE * D * 2;
+template <int D>
+constexpr int AT_SMEM = 3 * AT_OPERAND<D> + 1024 + (int)sizeof(AttendTilesShared);
+
+// Keys that some of rows [128 m, 128 m + 128) see, from the front on.
+__device__ __forceinline__ int at_tiles(const AttendArgs &a, const AttendRequest &q, int group, int m) {
+    const int seen = a.mask ? q.n : (int)min((long long)q.n, ((long long)(m + 1) * AT_ROWS - 1) / group + 1);
+    return (q.len + seen + AT_TILE - 1) / AT_TILE;
+}
+// 128-byte swizzle, columns of the operand side by side (MN-major): blocks of 64 columns `block` bytes apart, groups of eight k 1024.
+__device__ __forceinline__ uint64_t at_desc_mn(uint32_t smem_addr, uint32_t block) {
+    return (dg_desc_sw128(smem_addr) & ~((uint64_t)0x3fff << 16)) | (uint64_t)(block >> 4) << 16;
+}
+__device__ __forceinline__ void at_tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+        "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+// A CTA's walk over its part of the units, segment by segment; every warp role walks for itself.
+struct AttendSegment {
+    AttendRequest rq;
+    int r, hk, m, tile0, tiles, n_tiles;
+    long long start;  // its first unit
+};
+template <int D>
+struct AttendWalk {
+    const AttendArgs &a;
+    const long long *cum;
+    long long x, end;
+    int group;
+    __device__ __forceinline__ bool next(AttendSegment &s) {
+        if (x >= end) return false;
+        s.r = request_of_unit(cum, a.R, x);
+        s.rq = attend_request(a, s.r);
+        const long long rem = x - cum[s.r], per_head = (cum[s.r + 1] - cum[s.r]) / a.cache.n_kv;
+        s.hk = (int)(rem / per_head);
+        long long left = rem % per_head;
+        s.m = 0;
+        while (left >= (s.n_tiles = at_tiles(a, s.rq, group, s.m))) left -= s.n_tiles, ++s.m;
+        s.tile0 = (int)left;
+        s.start = x - left;
+        s.tiles = (int)min(end - x, (long long)s.n_tiles - left);
+        x += s.tiles;
+        return true;
+    }
+};
+
+template <bool F16, int D>
+__global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_kernel(AttendArgs a, int min_units, long long limit) {
+    constexpr uint32_t IDESC = (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(AT_ROWS >> 4) << 24);
+    constexpr uint32_t IDESC_QK = IDESC | ((uint32_t)(AT_TILE >> 3) << 17), IDESC_PV = IDESC | (1u << 16) | ((uint32_t)(D >> 3) << 17);
+    constexpr int HALF = AT_TILE * 128;  // bytes of 64 columns of an operand
+    constexpr int PART = AT_ROWS * (D + 2);
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t *qs = smem, *ks = smem + AT_OPERAND<D>, *vs = smem + 2 * AT_OPERAND<D>;
+    AttendTilesShared &sh = *reinterpret_cast<AttendTilesShared *>(smem + 3 * AT_OPERAND<D>);
+    long long *cum = reinterpret_cast<long long *>(&sh + 1);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int group = a.n_heads / a.cache.n_kv, page_size = a.cache.page_size;
+    const uint32_t k_full = smem_u32(&sh.k_full), v_full = smem_u32(&sh.v_full), scored = smem_u32(&sh.scored), added = smem_u32(&sh.added),
+                   weighed = smem_u32(&sh.weighed), q_full = smem_u32(&sh.q_full), summed = smem_u32(&sh.summed);
+    if (tid == 0) {
+        mbar_init(k_full, 32);
+        mbar_init(v_full, 32);
+        mbar_init(scored, 1);
+        mbar_init(added, 1);
+        mbar_init(weighed, 128);
+        mbar_init(q_full, 128);
+        mbar_init(summed, 1);
+        mbar_fence_init();
+        sh.odd[0] = sh.odd[1] = 0;
+    }
+    pdl_wait();
+    pdl_launch_dependents();
+    if (warp == 6) {
+        dg_tmem_alloc(smem_u32(&sh.tmem), AT_COLS);
+        dg_tmem_relinquish();
+    }
+    const long long units = scan_units<AT_THREADS>(a, cum, [&](const AttendRequest &q) {
+        const int m_tiles = (int)(((long long)q.n * group + AT_ROWS - 1) / AT_ROWS);
+        long long tiles = 0;
+        if (a.mask) tiles = (long long)m_tiles * at_tiles(a, q, group, 0);
+        else for (int m = 0; m < m_tiles; ++m) tiles += at_tiles(a, q, group, m);
+        return tiles * a.cache.n_kv;
+    });
+    dg_fence_before();
+    __syncthreads();
+    dg_fence_after();
+    const uint32_t tmem = sh.tmem, tmem_o = tmem + AT_TILE;
+    const long long per = max((units + gridDim.x - 1) / gridDim.x, (long long)min_units);
+    AttendWalk<D> walk{a, cum, blockIdx.x * per, min((blockIdx.x + 1) * per, units), group};
+    AttendSegment g;
+    bool ok = true;
+    int n = 0;  // tiles so far
+
+    if (warp == 4 || warp == 5) {
+        // ---- copies: warp 4 K, warp 5 V ----
+        const bool is_v = warp == 5;
+        const int ck = lane >> 3, cp = lane & 7;
+        const uint32_t full = is_v ? v_full : k_full, freed = is_v ? added : scored, to = smem_u32(is_v ? vs : ks) + ck * 128;
+        long long *places = sh.places[warp - 4];
+        for (int seg = 0; ok && walk.next(g); ++seg) {
+            const int total = g.rq.len + g.rq.n;
+            const int32_t *table = a.table + g.r * a.table_stride;
+            const uint16_t *base = (is_v ? a.cache.v + g.hk * a.cache.v_head : a.cache.k + g.hk * a.cache.k_head) + 8 * cp;
+            const long long s_page = is_v ? a.cache.v_page : a.cache.k_page, s_slot = is_v ? a.cache.v_slot : a.cache.k_slot;
+            auto page_of = [&](int i, int k) {  // key k of the lane's four
+                const int key = (g.tile0 + i) * AT_TILE + 32 * k + lane;
+                return i < g.tiles && key < total ? __ldg(table + page_index(a, key)) : -2;
+            };
+            int page[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) page[k] = page_of(0, k);
+            for (int i = 0; i < g.tiles; ++i, ++n) {
+                const int key0 = (g.tile0 + i) * AT_TILE;
+                uint32_t valid[4];
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int key = key0 + 32 * k + lane;
+                    const bool there = (unsigned)page[k] < (unsigned)a.cache.n_pages && key < total;
+                    if (key < total && !there) req_error(&a.header->error, REQ_ERR_PAGE);
+                    places[32 * k + lane] = there ? page[k] * s_page + (key - page_index(a, key) * page_size) * s_slot : -8;
+                    valid[k] = __ballot_sync(0xffffffffu, there);
+                    page[k] = page_of(i + 1, k);
+                }
+                __syncwarp();
+                if (n > 0 && !(ok = mbar_wait_bounded_warp(freed, (n - 1) & 1, limit))) break;
+                // (scores of the last tile: the tile before it, which had this place for its valid keys, has been weighed)
+                if (!is_v && lane == 0)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) sh.valid[n & 1][k] = valid[k];
+#pragma unroll 8
+                for (int q = 0; q < AT_TILE / 4; ++q) {  // keys 4 q + ck
+                    const long long o = places[4 * q + ck];
+                    copies16<D / 64, HALF, 128>(to + q * 512 + (cp ^ ((4 * q + ck) & 7)) * 16, base + o, o < 0 ? 0 : 16);
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                if (is_v && key0 + AT_TILE > g.rq.len) {
+                    // new tokens that some rows do not see: what is not finite is taken out here and added where it is seen, at the end
+#pragma unroll 1
+                    for (int q = 0; q < AT_TILE / 4; ++q) {
+                        if (key0 + 4 * q + ck < g.rq.len) continue;
+#pragma unroll 1
+                        for (int w = 0; w < 4 * (D / 64); ++w) {
+                            uint32_t &v = reinterpret_cast<uint32_t *>(vs + (w >> 2) * HALF + (4 * q + ck) * 128 + (cp ^ ((4 * q + ck) & 7)) * 16)[w & 3];
+                            if (!not_finite16x2<F16>(v)) continue;
+                            sh.odd[seg & 1] = 1;
+                            v &= (not_finite16x2<F16>(v & 0xffffu) ? 0xffff0000u : 0xffffffffu) & (not_finite16x2<F16>(v >> 16) ? 0xffffu : 0xffffffffu);
+                        }
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(full);
+            }
+        }
+    } else if (warp == 6) {
+        // ---- products ----
+        const uint64_t q_desc = dg_desc_sw128(smem_u32(qs)), k_desc = dg_desc_sw128(smem_u32(ks)), v_desc = at_desc_mn(smem_u32(vs), HALF);
+        for (int seg = 0; ok && walk.next(g); ++seg) {
+            if (!(ok = mbar_wait_bounded_warp(q_full, seg & 1, limit))) break;
+            for (int i = 0; i < g.tiles; ++i, ++n) {
+                if (!(ok = mbar_wait_bounded_warp(k_full, n & 1, limit))) break;
+                dg_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k)
+                        dg_umma_bf16(tmem, q_desc + (k >> 2) * (HALF >> 4) + 2 * (k & 3), k_desc + (k >> 2) * (HALF >> 4) + 2 * (k & 3), IDESC_QK, k > 0);
+                    dg_umma_commit(scored);
+                }
+                __syncwarp();
+                if (!(ok = mbar_wait_bounded_warp(v_full, n & 1, limit) && mbar_wait_bounded_warp(weighed, n & 1, limit))) break;
+                dg_fence_after();
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < AT_TILE / 16; ++k)
+                        dg_umma_bf16_ta(tmem_o, tmem + 8 * k, v_desc + k * (2048 >> 4), IDESC_PV, i > 0 || k > 0);
+                    dg_umma_commit(added);
+                    if (i + 1 == g.tiles) dg_umma_commit(summed);
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        // ---- a row a thread ----
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        const float scale = fabsf(a.scale_log2);  // (a negative one has turned Q's signs)
+        float *parts = reinterpret_cast<float *>(a.scratch + 4 * AR_MAX_CTAS);
+        int *counters = reinterpret_cast<int *>(a.scratch);
+        for (int seg = 0; ok && walk.next(g); ++seg) {
+            const int rows = (int)min((long long)AT_ROWS, (long long)g.rq.n * group - (long long)g.m * AT_ROWS);
+            const bool mine = tid < rows, busy = warp * 32 < rows;
+            const int row = g.m * AT_ROWS + tid, j = row / group, head = g.hk * group + row % group;
+            const unsigned long long bits = a.mask && mine ? (unsigned long long)a.mask[g.rq.q0 + j] : 0;
+            const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+            // Q, eight lanes a line
+            for (int q = tid >> 3; q < AT_ROWS; q += 16) {
+                const int rw = g.m * AT_ROWS + q;
+                const uint16_t *src = a.q + (long long)(g.rq.q0 + rw / group) * a.q_row + (long long)(g.hk * group + rw % group) * a.q_head + 8 * (tid & 7);
+#pragma unroll
+                for (int h = 0; h < D / 64; ++h) {
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (q < rows) v = *reinterpret_cast<const uint4 *>(src + 64 * h);
+                    v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
+                    *reinterpret_cast<uint4 *>(qs + h * HALF + q * 128 + ((tid & 7) ^ (q & 7)) * 16) = v;
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            dg_fence_before();
+            mbar_arrive(q_full);
+            float top = -INFINITY, sum = 0.f;
+            for (int i = 0; i < g.tiles; ++i, ++n) {
+                if (!(ok = mbar_wait_bounded_warp(scored, n & 1, limit))) break;
+                dg_fence_after();
+                if (busy) {
+                    const int key0 = (g.tile0 + i) * AT_TILE;
+                    uint32_t vis[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) vis[c] = sh.valid[n & 1][c];
+                    const bool partly = key0 + AT_TILE > g.rq.len || (vis[0] & vis[1] & vis[2] & vis[3]) != 0xffffffffu;
+                    if (partly) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const int d0 = key0 + 32 * c - g.rq.len;  // token of the step of the word's first key
+                            uint32_t see = 0xffffffffu;
+                            if (d0 > -32) {
+                                unsigned long long b;  // from token max(d0, 0) on
+                                if (a.mask) b = d0 >= 64 ? 0 : d0 > 0 ? bits >> d0 : bits;
+                                else b = j - max(d0, 0) >= 63 ? ~0ull : j < max(d0, 0) ? 0 : (2ull << (j - max(d0, 0))) - 1;
+                                see = d0 < 0 ? (uint32_t)(b << -d0) | ((1u << -d0) - 1) : (uint32_t)b;
+                            }
+                            vis[c] &= see;
+                        }
+                    }
+                    float m = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32];
+                        dg_tmem_ld_32x32b_x32(tmem + lanes + 32 * c, v);
+                        dg_tmem_ld_wait();
+                        if (partly) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v[e] = vis[c] >> e & 1 ? v[e] : 0xff800000u;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) m = fmaxf(m, __uint_as_float(v[e]));
+                    }
+                    if (m != -INFINITY) m *= scale;
+                    if (__any_sync(0xffffffffu, m > top + 8.f)) {
+                        const float to = fmaxf(m, top), keep = to == -INFINITY ? 1.f : exp2_fast(top - to);
+                        top = to;
+                        sum *= keep;
+                        if (i > 0) {  // (the last product into O is done: the scores behind it are)
+#pragma unroll
+                            for (int c = 0; c < D / 32; ++c) {
+                                uint32_t v[32];
+                                dg_tmem_ld_32x32b_x32(tmem_o + lanes + 32 * c, v);
+                                dg_tmem_ld_wait();
+                                uint32_t u[2][16];
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) u[e >> 4][e & 15] = __float_as_uint(__uint_as_float(v[e]) * keep);
+                                at_tmem_st_x16(tmem_o + lanes + 32 * c, u[0]);
+                                at_tmem_st_x16(tmem_o + lanes + 32 * c + 16, u[1]);
+                            }
+                        }
+                    }
+                    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t v[32], p[16];
+                        dg_tmem_ld_32x32b_x32(tmem + lanes + 32 * c, v);
+                        dg_tmem_ld_wait();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(fmaf(__uint_as_float(v[e]), scale, -ref));
+                        if (partly) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) v[e] = vis[c] >> e & 1 ? v[e] : 0xff800000u;
+                        }
+                        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float p0 = exp2_fast(__uint_as_float(v[2 * e])), p1 = exp2_fast(__uint_as_float(v[2 * e + 1]));
+                            s0 += p0;
+                            s1 += p1;
+                            p[e] = pack16x2<F16>(p0, p1);
+                        }
+                        sum += s0 + s1;
+                        at_tmem_st_x16(tmem + lanes + 16 * c, p);  // (over scores that have been read)
+                    }
+                    dg_tmem_st_wait();
+                }
+                dg_fence_before();
+                mbar_arrive(weighed);
+            }
+            if (!ok) break;
+            if (!(ok = mbar_wait_bounded_warp(summed, seg & 1, limit))) break;
+            dg_fence_after();
+            // ---- the segment's sums: out, or to the CTA that joins them ----
+            const int c0 = (int)(g.start / per), c1 = (int)((g.start + g.n_tiles - 1) / per);
+            const bool whole = c0 == c1;
+            const bool odd = *reinterpret_cast<volatile int *>(&sh.odd[seg & 1]) != 0;
+            float *part = parts + (long long)(2 * blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0)) * PART;  // [D + 2][128]
+            uint16_t *out = a.out + (long long)(g.rq.q0 + j) * a.o_row + (long long)head * a.o_head;
+            auto store32 = [&](int c, const float (&o)[32], float total) {
+                const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+                for (int e = 0; e < 32; e += 8)
+                    *reinterpret_cast<uint4 *>(out + 32 * c + e) =
+                        make_uint4(pack16x2<F16>(o[e] * inv, o[e + 1] * inv), pack16x2<F16>(o[e + 2] * inv, o[e + 3] * inv),
+                                   pack16x2<F16>(o[e + 4] * inv, o[e + 5] * inv), pack16x2<F16>(o[e + 6] * inv, o[e + 7] * inv));
+            };
+            if (busy) {
+#pragma unroll 1
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t v[32];
+                    float o[32];
+                    dg_tmem_ld_32x32b_x32(tmem_o + lanes + 32 * c, v);
+                    dg_tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(v[e]);
+                    if (odd && mine) {
+                        const int first = max(g.tile0 * AT_TILE - g.rq.len, 0), last = min((g.tile0 + g.tiles) * AT_TILE - g.rq.len, g.rq.n);
+                        for (int d = first; d < last; ++d) {
+                            if (!(a.mask ? d < 64 && (bits >> d & 1) : d <= j)) continue;
+                            const int key = g.rq.len + d, page = a.table[g.r * a.table_stride + page_index(a, key)];
+                            if ((unsigned)page >= (unsigned)a.cache.n_pages) continue;
+                            const uint16_t *src = a.cache.v + page * a.cache.v_page + (key - page_index(a, key) * page_size) * a.cache.v_slot + g.hk * a.cache.v_head + 32 * c;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (not_finite16x2<F16>(src[e])) o[e] += unpack16x2<F16>(src[e]).x;
+                        }
+                    }
+                    if (whole) {
+                        if (mine) store32(c, o, sum);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) part[(32 * c + e) * AT_ROWS + tid] = o[e];
+                    }
+                }
+                if (!whole) part[D * AT_ROWS + tid] = top, part[(D + 1) * AT_ROWS + tid] = sum;
+            }
+            dg_fence_before();
+            if (!whole) __threadfence();
+            named_bar_sync(1, 128);
+            if (tid == 0) sh.odd[seg & 1] = 0;
+            if (!whole) {
+                if (tid == 0) sh.last = atomicAdd(counters + c0, 1) == c1 - c0;
+                named_bar_sync(1, 128);
+                if (sh.last) {
+                    __threadfence();
+                    if (mine) {
+                        float m = -INFINITY, total = 0.f;
+                        for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(parts + (long long)(2 * c + (c == c0)) * PART + D * AT_ROWS + tid));
+                        const float ref = m == -INFINITY ? 0.f : m;
+                        for (int c = c0; c <= c1; ++c) {
+                            const float *src = parts + (long long)(2 * c + (c == c0)) * PART + D * AT_ROWS + tid;
+                            total += exp2_fast(__ldcg(src) - ref) * __ldcg(src + AT_ROWS);
+                        }
+#pragma unroll 1
+                        for (int q = 0; q < D / 32; ++q) {
+                            float o[32] = {};
+                            for (int c = c0; c <= c1; ++c) {
+                                const float *src = parts + (long long)(2 * c + (c == c0)) * PART + tid;
+                                const float f = exp2_fast(__ldcg(src + D * AT_ROWS) - ref);
+                                if (f == 0.f) continue;
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = fmaf(f, __ldcg(src + (32 * q + e) * AT_ROWS), o[e]);
+                            }
+                            store32(q, o, total);
+                        }
+                    }
+                    if (tid == 0) counters[c0] = 0;
+                }
+                named_bar_sync(1, 128);  // (`last` is one segment's at a time)
+            }
+        }
+    }
+    if (!ok && lane == 0) req_error(&a.header->error, REQ_ERR_TIMEOUT);
+    dg_fence_before();
+    __syncthreads();
+    dg_fence_after();
+    if (warp == 6) dg_tmem_dealloc(tmem, AT_COLS);
+}
+
+size_t tree_attention_scratch_bytes() {
+    const size_t rows = (size_t)2 * AR_MAX_CTAS * AR_ROWS * (128 + 2) * 4, tiles = (size_t)2 * AT_MAX_CTAS * AT_ROWS * (128 + 2) * 4;
+    return 4 * AR_MAX_CTAS + (rows > tiles ? rows : tiles);
+}
 
 }  // namespace awq
 
@@ -574,6 +995,15 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
                  view.page_size & (view.page_size - 1) ? -1 : __builtin_ctz(view.page_size), w.header, w.attention};
     if (view.head_dim == 64 || view.head_dim == 128) {
         const bool f16 = cache->format == ACT_F16;
+        // More rows than one mma.sync tile has, on average: tcgen05.
+        if ((long long)T * (n_heads / view.n_kv) > (long long)AR_ROWS * R) {
+            auto kernel = view.head_dim == 64 ? (f16 ? tree_attention_tiles_kernel<true, 64> : tree_attention_tiles_kernel<false, 64>)
+                                              : (f16 ? tree_attention_tiles_kernel<true, 128> : tree_attention_tiles_kernel<false, 128>);
+            const int smem = (view.head_dim == 64 ? AT_SMEM<64> : AT_SMEM<128>) + (R + 1) * 8;
+            if ((rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "tree_attention shared memory"))) return rc;
+            const int grid = min(device_sm_count() * AT_PER_SM, AT_MAX_CTAS);
+            return check_cuda(launch_pdl(kernel, dim3(grid), dim3(AT_THREADS), smem, as_stream(stream), a, 1, wait_limit_cycles()), "tree_attention launch");
+        }
         auto kernel = view.head_dim == 64 ? (f16 ? tree_attention_rows_kernel<true, 64> : tree_attention_rows_kernel<false, 64>)
                                           : (f16 ? tree_attention_rows_kernel<true, 128> : tree_attention_rows_kernel<false, 128>);
         const int smem = (view.head_dim == 64 ? AR_SMEM<64> : AR_SMEM<128>) + (R + 1) * 8;
