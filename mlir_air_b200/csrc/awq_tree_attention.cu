@@ -151,12 +151,12 @@ template <int TO, int FROM>  // at fixed distances (bytes) from dst and src; zer
 __device__ __forceinline__ void copy16(uint32_t dst, const uint16_t *src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0 + %3], [%1 + %4], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes), "n"(TO), "n"(FROM) : "memory");
 }
-// N copies, the i-th at i TO and i FROM.
-template <int N, int TO, int FROM, int I = 0>
+// N copies, the i-th at AT + i TO and i FROM.
+template <int N, int TO, int FROM, int AT = 0, int I = 0>
 __device__ __forceinline__ void copies16(uint32_t dst, const uint16_t *src, int bytes) {
     if constexpr (I < N) {
-        copy16<I * TO, I * FROM>(dst, src, bytes);
-        copies16<N, TO, FROM, I + 1>(dst, src, bytes);
+        copy16<AT + I * TO, I * FROM>(dst, src, bytes);
+        copies16<N, TO, FROM, AT, I + 1>(dst, src, bytes);
     }
 }
 template <bool F16>
@@ -551,31 +551,32 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
 // =====================================================================================
 // Many rows per cache head (trees, prompts): tcgen05, 128 rows at a time.
 //
-// A unit of work is 128 keys of a segment = (request, cache head, 128 rows), split over the CTAs and joined as above.  Two CTAs an SM;
+// A unit of work is 64 keys of a segment = (request, cache head, 128 rows), split over the CTAs and joined as above.  Two CTAs an SM;
 // in each
-//   2 warps  copy K and V (16-byte asynchronous copies, whole lines) into the 128-byte swizzle, one each;
-//   1 warp   issues the products: S = Q K^T into 128 columns of tensor memory, O += P V into D others;
+//   3 warps  copy K and V (16-byte asynchronous copies, whole lines) into the 128-byte swizzle, two tiles of each held;
+//   1 warp   issues the products: S = Q K^T into 64 columns of tensor memory, O += P V into D others;
 //   4 warps  hold a row per thread: maximum, weights, and P as 16-bit pairs over S's own columns, from where the tensor cores take
 //            it as the left operand of the next product.
-// K and V are held once: K of the next tile is fetched while the weights of this one are formed, V while the scores are.  What
-// one CTA leaves idle (the tensor cores during its softmax, the exponentials during its products) is the other one's.  O stays in
-// tensor memory; it is rescaled only when a maximum has grown by more than 8 (powers of two), by the warp that finds it.
+// S is held twice: the scores of a tile are formed while the one before it is weighed.  What one CTA leaves idle (the tensor
+// cores during its softmax, the exponentials during its products) is the other one's.  O stays in tensor memory; it is rescaled
+// only when a maximum has grown by more than 8 (powers of two), by the warp that finds it.
 // Weights are rounded to the rows' 16-bit type for the product, as they have to be for one tensor-core operand (their sum is
 // not): half a step per weight, independent from key to key.
 // =====================================================================================
-constexpr int AT_ROWS = 128, AT_TILE = 128, AT_THREADS = 7 * 32, AT_PER_SM = 2, AT_MAX_CTAS = 192 * AT_PER_SM, AT_COLS = 256;
+constexpr int AT_ROWS = 128, AT_TILE = 64, AT_LOADERS = 3, AT_THREADS = 8 * 32, AT_PER_SM = 2, AT_MAX_CTAS = 192 * AT_PER_SM, AT_COLS = 256;
 static_assert(AT_MAX_CTAS <= AR_MAX_CTAS, "the counters of both kernels share their place");
 struct AttendTilesShared {
-    uint64_t k_full, v_full, scored, added, weighed, q_full, summed;  // mbarriers: K, V there; QK^T, PV done; P there; Q there, O done (segment)
+    // mbarriers, of even and odd tiles: K, V there; QK^T, PV (of every fourth) done; P there.  Of a segment: Q there, O done.
+    uint64_t k_full[2], v_full[2], scored[2], added[4], weighed[2], q_full, summed;
     uint32_t tmem;
-    int last, odd[2];
-    uint32_t valid[2][4];         // of a tile: which of its keys there are
-    long long places[2][128];     // of a copying warp: the keys of its tile
+    int last, odd[2], pad;
+    uint32_t valid[4][2];                  // of a tile: which of its keys there are
+    long long places[AT_LOADERS][AT_TILE];  // of a copying warp: the keys of its tile
 };
 template <int D>
 constexpr int AT_OPERAND = AT_TILE * D * 2;
 template <int D>
-constexpr int AT_SMEM = 3 * AT_OPERAND<D> + 1024 + (int)sizeof(AttendTilesShared);
+constexpr int AT_SMEM = AT_ROWS * D * 2 + 4 * AT_OPERAND<D> + 1024 + (int)sizeof(AttendTilesShared);
 
 // Keys that some of rows [128 m, 128 m + 128) see, from the front on.
 __device__ __forceinline__ int at_tiles(const AttendArgs &a, const AttendRequest &q, int group, int m) {
@@ -592,6 +593,40 @@ __device__ __forceinline__ void at_tmem_st_x16(uint32_t taddr, const uint32_t (&
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
         "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+
+// Two f32 fused multiply-adds, and two additions onto a pair of sums, in one instruction each.
+__device__ __forceinline__ void at_fma2(float &x0, float &x1, float a0, float a1, float b, float c) {
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %4};\n\tmov.b64 c, {%5, %5};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(x0), "=f"(x1)
+        : "f"(a0), "f"(a1), "f"(b), "f"(c));
+}
+__device__ __forceinline__ void at_add2(uint64_t &sums, float x0, float x1) {
+    asm("{\n\t.reg .b64 a;\n\tmov.b64 a, {%1, %2};\n\tadd.rn.f32x2 %0, %0, a;\n\t}" : "+l"(sums) : "f"(x0), "f"(x1));
+}
+__device__ __forceinline__ float at_sum2(uint64_t sums) {
+    return __uint_as_float((uint32_t)sums) + __uint_as_float((uint32_t)(sums >> 32));
+}
+// Scores of a row against keys it does not see become -inf; vis: the keys that there are.
+__device__ __noinline__ void at_see(const AttendArgs &a, int len, int key0, int j, unsigned long long bits, uint32_t (&vis)[2]) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const int d0 = key0 + 32 * c - len;  // token of the step of the word's first key
+        if (d0 <= -32) continue;
+        unsigned long long b;  // from token max(d0, 0) on
+        if (a.mask) b = d0 >= 64 ? 0 : d0 > 0 ? bits >> d0 : bits;
+        else b = j - max(d0, 0) >= 63 ? ~0ull : j < max(d0, 0) ? 0 : (2ull << (j - max(d0, 0))) - 1;
+        vis[c] &= d0 < 0 ? (uint32_t)(b << -d0) | ((1u << -d0) - 1) : (uint32_t)b;
+    }
+}
+__device__ __forceinline__ void at_mask(const AttendArgs &a, const AttendRequest &rq, int key0, int j, unsigned long long bits, uint32_t (&vis)[2],
+                                        uint32_t (&v)[2][32]) {
+    at_see(a, rq.len, key0, j, bits, vis);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[c][e] = vis[c] >> e & 1 ? v[c][e] : 0xff800000u;
 }
 
 // A CTA's walk over its part of the units, segment by segment; every warp role walks for itself.
@@ -623,27 +658,41 @@ struct AttendWalk {
     }
 };
 
+// Keys 4 q + (the lane's of four) of a tile for q = Q .. END - 1, in lines of 128 bytes swizzled by key % 8: the lane's piece has one
+// place in keys of even q (dst0) and another one in odd (dst1).
+template <int D, int Q, int END>
+__device__ __forceinline__ void at_copy_keys(uint32_t dst0, uint32_t dst1, const uint16_t *base, const long long *places) {
+    if constexpr (Q < END) {
+        const long long o = places[4 * Q];
+        copies16<D / 64, AT_TILE * 128, 128, Q * 512>(Q & 1 ? dst1 : dst0, base + o, o < 0 ? 0 : 16);
+        at_copy_keys<D, Q + 1, END>(dst0, dst1, base, places);
+    }
+}
+
 template <bool F16, int D>
 __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_kernel(AttendArgs a, int min_units, long long limit) {
     constexpr uint32_t IDESC = (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(AT_ROWS >> 4) << 24);
     constexpr uint32_t IDESC_QK = IDESC | ((uint32_t)(AT_TILE >> 3) << 17), IDESC_PV = IDESC | (1u << 16) | ((uint32_t)(D >> 3) << 17);
-    constexpr int HALF = AT_TILE * 128;  // bytes of 64 columns of an operand
+    constexpr int HALF = AT_TILE * 128, Q_HALF = AT_ROWS * 128;  // bytes of 64 columns of an operand
     constexpr int PART = AT_ROWS * (D + 2);
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    uint8_t *qs = smem, *ks = smem + AT_OPERAND<D>, *vs = smem + 2 * AT_OPERAND<D>;
-    AttendTilesShared &sh = *reinterpret_cast<AttendTilesShared *>(smem + 3 * AT_OPERAND<D>);
+    uint8_t *qs = smem, *ks = smem + AT_ROWS * D * 2, *vs = ks + 2 * AT_OPERAND<D>;
+    AttendTilesShared &sh = *reinterpret_cast<AttendTilesShared *>(vs + 2 * AT_OPERAND<D>);
     long long *cum = reinterpret_cast<long long *>(&sh + 1);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = a.n_heads / a.cache.n_kv, page_size = a.cache.page_size;
-    const uint32_t k_full = smem_u32(&sh.k_full), v_full = smem_u32(&sh.v_full), scored = smem_u32(&sh.scored), added = smem_u32(&sh.added),
-                   weighed = smem_u32(&sh.weighed), q_full = smem_u32(&sh.q_full), summed = smem_u32(&sh.summed);
+    const uint32_t k_full = smem_u32(sh.k_full), v_full = smem_u32(sh.v_full), scored = smem_u32(sh.scored), added = smem_u32(sh.added),
+                   weighed = smem_u32(sh.weighed), q_full = smem_u32(&sh.q_full), summed = smem_u32(&sh.summed);
     if (tid == 0) {
-        mbar_init(k_full, 32);
-        mbar_init(v_full, 32);
-        mbar_init(scored, 1);
-        mbar_init(added, 1);
-        mbar_init(weighed, 128);
+        for (int b = 0; b < 16; b += 8) {
+            mbar_init(k_full + b, 32);
+            mbar_init(v_full + b, 32);
+            mbar_init(scored + b, 1);
+            mbar_init(added + b, 1);
+            mbar_init(added + 16 + b, 1);
+            mbar_init(weighed + b, 128);
+        }
         mbar_init(q_full, 128);
         mbar_init(summed, 1);
         mbar_fence_init();
@@ -651,7 +700,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
     }
     pdl_wait();
     pdl_launch_dependents();
-    if (warp == 6) {
+    if (warp == 7) {
         dg_tmem_alloc(smem_u32(&sh.tmem), AT_COLS);
         dg_tmem_relinquish();
     }
@@ -665,96 +714,106 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
     dg_fence_before();
     __syncthreads();
     dg_fence_after();
-    const uint32_t tmem = sh.tmem, tmem_o = tmem + AT_TILE;
+    const uint32_t tmem = sh.tmem, tmem_o = tmem + 2 * AT_TILE;
     const long long per = max((units + gridDim.x - 1) / gridDim.x, (long long)min_units);
     AttendWalk<D> walk{a, cum, blockIdx.x * per, min((blockIdx.x + 1) * per, units), group};
     AttendSegment g;
     bool ok = true;
-    int n = 0;  // tiles so far
+    int n = 0;  // tiles so far: tile n has place n % 2 of everything that is held twice, in phase n / 2 % 2
+    auto bar_of = [](uint32_t bar, int t) { return bar + 8 * (t & 1); };
+    auto phase_of = [](int t) { return (uint32_t)(t >> 1 & 1); };
+    auto added_of = [&](int t) { return added + 8 * (t & 3); };
+    auto added_phase = [](int t) { return (uint32_t)(t >> 2 & 1); };
 
-    if (warp == 4 || warp == 5) {
-        // ---- copies: warp 4 K, warp 5 V ----
-        const bool is_v = warp == 5;
+    if (warp >= 4 && warp < 4 + AT_LOADERS) {
+        // ---- copies: K and V of tile after tile, in turn ----
         const int ck = lane >> 3, cp = lane & 7;
-        const uint32_t full = is_v ? v_full : k_full, freed = is_v ? added : scored, to = smem_u32(is_v ? vs : ks) + ck * 128;
         long long *places = sh.places[warp - 4];
+        int turn = warp - 4;  // loads until the next one of this warp
         for (int seg = 0; ok && walk.next(g); ++seg) {
             const int total = g.rq.len + g.rq.n;
             const int32_t *table = a.table + g.r * a.table_stride;
-            const uint16_t *base = (is_v ? a.cache.v + g.hk * a.cache.v_head : a.cache.k + g.hk * a.cache.k_head) + 8 * cp;
-            const long long s_page = is_v ? a.cache.v_page : a.cache.k_page, s_slot = is_v ? a.cache.v_slot : a.cache.k_slot;
-            auto page_of = [&](int i, int k) {  // key k of the lane's four
-                const int key = (g.tile0 + i) * AT_TILE + 32 * k + lane;
-                return i < g.tiles && key < total ? __ldg(table + page_index(a, key)) : -2;
-            };
-            int page[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) page[k] = page_of(0, k);
-            for (int i = 0; i < g.tiles; ++i, ++n) {
-                const int key0 = (g.tile0 + i) * AT_TILE;
-                uint32_t valid[4];
-                __syncwarp();
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int key = key0 + 32 * k + lane;
-                    const bool there = (unsigned)page[k] < (unsigned)a.cache.n_pages && key < total;
-                    if (key < total && !there) req_error(&a.header->error, REQ_ERR_PAGE);
-                    places[32 * k + lane] = there ? page[k] * s_page + (key - page_index(a, key) * page_size) * s_slot : -8;
-                    valid[k] = __ballot_sync(0xffffffffu, there);
-                    page[k] = page_of(i + 1, k);
-                }
-                __syncwarp();
-                if (n > 0 && !(ok = mbar_wait_bounded_warp(freed, (n - 1) & 1, limit))) break;
-                // (scores of the last tile: the tile before it, which had this place for its valid keys, has been weighed)
-                if (!is_v && lane == 0)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) sh.valid[n & 1][k] = valid[k];
-#pragma unroll 8
-                for (int q = 0; q < AT_TILE / 4; ++q) {  // keys 4 q + ck
-                    const long long o = places[4 * q + ck];
-                    copies16<D / 64, HALF, 128>(to + q * 512 + (cp ^ ((4 * q + ck) & 7)) * 16, base + o, o < 0 ? 0 : 16);
-                }
-                asm volatile("cp.async.wait_all;" ::: "memory");
-                if (is_v && key0 + AT_TILE > g.rq.len) {
-                    // new tokens that some rows do not see: what is not finite is taken out here and added where it is seen, at the end
+            for (int i = 0; ok && i < g.tiles; ++i, ++n) {
 #pragma unroll 1
-                    for (int q = 0; q < AT_TILE / 4; ++q) {
-                        if (key0 + 4 * q + ck < g.rq.len) continue;
+                for (int is_v = 0; is_v < 2; ++is_v) {
+                    if (turn-- > 0) continue;
+                    turn = AT_LOADERS - 1;
+                    const int key0 = (g.tile0 + i) * AT_TILE;
+                    const uint16_t *base = (is_v ? a.cache.v + g.hk * a.cache.v_head : a.cache.k + g.hk * a.cache.k_head) + 8 * cp;
+                    const long long s_page = is_v ? a.cache.v_page : a.cache.k_page, s_slot = is_v ? a.cache.v_slot : a.cache.k_slot;
+                    uint32_t valid[2];
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int key = key0 + 32 * k + lane, block = page_index(a, key);
+                        const int page = key < total ? __ldg(table + block) : -1;
+                        const bool there = (unsigned)page < (unsigned)a.cache.n_pages;
+                        if (key < total && !there) req_error(&a.header->error, REQ_ERR_PAGE);
+                        places[32 * k + lane] = there ? page * s_page + (key - block * page_size) * s_slot : -8;
+                        valid[k] = __ballot_sync(0xffffffffu, there);
+                    }
+                    __syncwarp();
+                    // A wait tells a phase from the one before it only, so that one has to be known to be over.  For K: this warp's last
+                    // load was V of tile n - 2, behind the sum of tile n - 4.  For V, whose four barriers come round every four
+                    // tiles: it was K of tile n - 1, behind the scores of n - 3, which were asked for behind the sum of n - 5.
+                    if (n > 1 && !(ok = is_v ? mbar_wait_bounded_warp(added_of(n - 2), added_phase(n - 2), limit)
+                                             : mbar_wait_bounded_warp(bar_of(scored, n), phase_of(n - 2), limit)))
+                        break;
+                    // (scores of tile n - 2 were asked for behind the weights of tile n - 4, whose place this is)
+                    if (!is_v && lane == 0) sh.valid[n & 3][0] = valid[0], sh.valid[n & 3][1] = valid[1];
+                    const uint32_t to = smem_u32((is_v ? vs : ks) + (n & 1) * AT_OPERAND<D>) + ck * 128;
+                    at_copy_keys<D, 0, AT_TILE / 4>(to + (cp ^ ck) * 16, to + (cp ^ ck ^ 4) * 16, base, places + ck);
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    if (is_v && key0 + AT_TILE > g.rq.len) {
+                        // new tokens that some rows do not see: what is not finite is taken out here and added where it is seen, at the end
+                        uint8_t *mine = vs + (n & 1) * AT_OPERAND<D>;
 #pragma unroll 1
-                        for (int w = 0; w < 4 * (D / 64); ++w) {
-                            uint32_t &v = reinterpret_cast<uint32_t *>(vs + (w >> 2) * HALF + (4 * q + ck) * 128 + (cp ^ ((4 * q + ck) & 7)) * 16)[w & 3];
-                            if (!not_finite16x2<F16>(v)) continue;
-                            sh.odd[seg & 1] = 1;
-                            v &= (not_finite16x2<F16>(v & 0xffffu) ? 0xffff0000u : 0xffffffffu) & (not_finite16x2<F16>(v >> 16) ? 0xffffu : 0xffffffffu);
+                        for (int q = 0; q < AT_TILE / 4; ++q) {
+                            if (key0 + 4 * q + ck < g.rq.len) continue;
+#pragma unroll 1
+                            for (int w = 0; w < 4 * (D / 64); ++w) {
+                                uint32_t &v = reinterpret_cast<uint32_t *>(mine + (w >> 2) * HALF + (4 * q + ck) * 128 + (cp ^ ((4 * q + ck) & 7)) * 16)[w & 3];
+                                if (!not_finite16x2<F16>(v)) continue;
+                                sh.odd[seg & 1] = 1;
+                                v &= (not_finite16x2<F16>(v & 0xffffu) ? 0xffff0000u : 0xffffffffu) & (not_finite16x2<F16>(v >> 16) ? 0xffffu : 0xffffffffu);
+                            }
                         }
                     }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_arrive(bar_of(is_v ? v_full : k_full, n));
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(full);
             }
         }
-    } else if (warp == 6) {
-        // ---- products ----
+    } else if (warp == 7) {
+        // ---- products: the scores of a tile are asked for before the weighted sum of the one in front of it ----
         const uint64_t q_desc = dg_desc_sw128(smem_u32(qs)), k_desc = dg_desc_sw128(smem_u32(ks)), v_desc = at_desc_mn(smem_u32(vs), HALF);
+        auto score = [&](int t) {
+            ok = mbar_wait_bounded_warp(bar_of(k_full, t), phase_of(t), limit);
+            if (!ok) return;
+            dg_fence_after();
+            if (elect_one()) {
+                const uint64_t kd = k_desc + (t & 1) * (AT_OPERAND<D> >> 4);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    dg_umma_bf16(tmem + (t & 1) * AT_TILE, q_desc + (k >> 2) * (Q_HALF >> 4) + 2 * (k & 3), kd + (k >> 2) * (HALF >> 4) + 2 * (k & 3), IDESC_QK, k > 0);
+                dg_umma_commit(bar_of(scored, t));
+            }
+            __syncwarp();
+        };
         for (int seg = 0; ok && walk.next(g); ++seg) {
             if (!(ok = mbar_wait_bounded_warp(q_full, seg & 1, limit))) break;
-            for (int i = 0; i < g.tiles; ++i, ++n) {
-                if (!(ok = mbar_wait_bounded_warp(k_full, n & 1, limit))) break;
+            score(n);
+            for (int i = 0; ok && i < g.tiles; ++i, ++n) {
+                if (i + 1 < g.tiles) score(n + 1);
+                if (!ok) break;
+                if (!(ok = mbar_wait_bounded_warp(bar_of(v_full, n), phase_of(n), limit) && mbar_wait_bounded_warp(bar_of(weighed, n), phase_of(n), limit))) break;
                 dg_fence_after();
                 if (elect_one()) {
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k)
-                        dg_umma_bf16(tmem, q_desc + (k >> 2) * (HALF >> 4) + 2 * (k & 3), k_desc + (k >> 2) * (HALF >> 4) + 2 * (k & 3), IDESC_QK, k > 0);
-                    dg_umma_commit(scored);
-                }
-                __syncwarp();
-                if (!(ok = mbar_wait_bounded_warp(v_full, n & 1, limit) && mbar_wait_bounded_warp(weighed, n & 1, limit))) break;
-                dg_fence_after();
-                if (elect_one()) {
+                    const uint64_t vd = v_desc + (n & 1) * (AT_OPERAND<D> >> 4);
 #pragma unroll
                     for (int k = 0; k < AT_TILE / 16; ++k)
-                        dg_umma_bf16_ta(tmem_o, tmem + 8 * k, v_desc + k * (2048 >> 4), IDESC_PV, i > 0 || k > 0);
-                    dg_umma_commit(added);
+                        dg_umma_bf16_ta(tmem_o, tmem + (n & 1) * AT_TILE + 8 * k, vd + k * (2048 >> 4), IDESC_PV, i > 0 || k > 0);
+                    dg_umma_commit(added_of(n));
                     if (i + 1 == g.tiles) dg_umma_commit(summed);
                 }
                 __syncwarp();
@@ -763,7 +822,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
     } else {
         // ---- a row a thread ----
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-        const float scale = fabsf(a.scale_log2);  // (a negative one has turned Q's signs)
+        const float scale = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);  // (a negative one has turned Q's signs; 0 times -inf is not a number)
         float *parts = reinterpret_cast<float *>(a.scratch + 4 * AR_MAX_CTAS);
         int *counters = reinterpret_cast<int *>(a.scratch);
         for (int seg = 0; ok && walk.next(g); ++seg) {
@@ -781,7 +840,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
                     uint4 v = make_uint4(0, 0, 0, 0);
                     if (q < rows) v = *reinterpret_cast<const uint4 *>(src + 64 * h);
                     v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-                    *reinterpret_cast<uint4 *>(qs + h * HALF + q * 128 + ((tid & 7) ^ (q & 7)) * 16) = v;
+                    *reinterpret_cast<uint4 *>(qs + h * Q_HALF + q * 128 + ((tid & 7) ^ (q & 7)) * 16) = v;
                 }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -789,87 +848,60 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
             mbar_arrive(q_full);
             float top = -INFINITY, sum = 0.f;
             for (int i = 0; i < g.tiles; ++i, ++n) {
-                if (!(ok = mbar_wait_bounded_warp(scored, n & 1, limit))) break;
+                if (!(ok = mbar_wait_bounded_warp(bar_of(scored, n), phase_of(n), limit))) break;
                 dg_fence_after();
                 if (busy) {
+                    const uint32_t s_cols = tmem + lanes + (n & 1) * AT_TILE;
                     const int key0 = (g.tile0 + i) * AT_TILE;
-                    uint32_t vis[4];
+                    uint32_t v[2][32];
+                    dg_tmem_ld_32x32b_x32(s_cols, v[0]);
+                    dg_tmem_ld_32x32b_x32(s_cols + 32, v[1]);
+                    uint32_t vis[2] = {sh.valid[n & 3][0], sh.valid[n & 3][1]};
+                    dg_tmem_ld_wait();
+                    if (key0 + AT_TILE > g.rq.len || (vis[0] & vis[1]) != 0xffffffffu) at_mask(a, g.rq, key0, j, bits, vis, v);
+                    float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) vis[c] = sh.valid[n & 1][c];
-                    const bool partly = key0 + AT_TILE > g.rq.len || (vis[0] & vis[1] & vis[2] & vis[3]) != 0xffffffffu;
-                    if (partly) {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const int d0 = key0 + 32 * c - g.rq.len;  // token of the step of the word's first key
-                            uint32_t see = 0xffffffffu;
-                            if (d0 > -32) {
-                                unsigned long long b;  // from token max(d0, 0) on
-                                if (a.mask) b = d0 >= 64 ? 0 : d0 > 0 ? bits >> d0 : bits;
-                                else b = j - max(d0, 0) >= 63 ? ~0ull : j < max(d0, 0) ? 0 : (2ull << (j - max(d0, 0))) - 1;
-                                see = d0 < 0 ? (uint32_t)(b << -d0) | ((1u << -d0) - 1) : (uint32_t)b;
-                            }
-                            vis[c] &= see;
-                        }
-                    }
-                    float m = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32];
-                        dg_tmem_ld_32x32b_x32(tmem + lanes + 32 * c, v);
-                        dg_tmem_ld_wait();
-                        if (partly) {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) v[e] = vis[c] >> e & 1 ? v[e] : 0xff800000u;
-                        }
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) m = fmaxf(m, __uint_as_float(v[e]));
-                    }
+                    for (int e = 0; e < 32; ++e) m0 = fmaxf(m0, __uint_as_float(v[0][e])), m1 = fmaxf(m1, __uint_as_float(v[1][e]));
+                    float m = fmaxf(m0, m1);
                     if (m != -INFINITY) m *= scale;
                     if (__any_sync(0xffffffffu, m > top + 8.f)) {
                         const float to = fmaxf(m, top), keep = to == -INFINITY ? 1.f : exp2_fast(top - to);
                         top = to;
                         sum *= keep;
-                        if (i > 0) {  // (the last product into O is done: the scores behind it are)
-#pragma unroll
-                            for (int c = 0; c < D / 32; ++c) {
-                                uint32_t v[32];
-                                dg_tmem_ld_32x32b_x32(tmem_o + lanes + 32 * c, v);
+                        if (i > 0) {
+                            if (!(ok = mbar_wait_bounded_warp(added_of(n - 1), added_phase(n - 1), limit))) break;
+                            dg_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D / 16; ++c) {
+                                uint32_t u[16];
+                                dg_tmem_ld_32x32b_x16(tmem_o + lanes + 16 * c, u);
                                 dg_tmem_ld_wait();
-                                uint32_t u[2][16];
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) u[e >> 4][e & 15] = __float_as_uint(__uint_as_float(v[e]) * keep);
-                                at_tmem_st_x16(tmem_o + lanes + 32 * c, u[0]);
-                                at_tmem_st_x16(tmem_o + lanes + 32 * c + 16, u[1]);
+                                for (int e = 0; e < 16; ++e) u[e] = __float_as_uint(__uint_as_float(u[e]) * keep);
+                                at_tmem_st_x16(tmem_o + lanes + 16 * c, u);
                             }
                         }
                     }
                     const float ref = top == -INFINITY ? 0.f : top;
+                    uint64_t sums[2] = {0, 0};
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t v[32], p[16];
-                        dg_tmem_ld_32x32b_x32(tmem + lanes + 32 * c, v);
-                        dg_tmem_ld_wait();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(fmaf(__uint_as_float(v[e]), scale, -ref));
-                        if (partly) {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) v[e] = vis[c] >> e & 1 ? v[e] : 0xff800000u;
-                        }
-                        float s0 = 0.f, s1 = 0.f;
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t p[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            const float p0 = exp2_fast(__uint_as_float(v[2 * e])), p1 = exp2_fast(__uint_as_float(v[2 * e + 1]));
-                            s0 += p0;
-                            s1 += p1;
-                            p[e] = pack16x2<F16>(p0, p1);
+                            float x0, x1;
+                            at_fma2(x0, x1, __uint_as_float(v[c][2 * e]), __uint_as_float(v[c][2 * e + 1]), scale, -ref);
+                            x0 = exp2_fast(x0), x1 = exp2_fast(x1);
+                            at_add2(sums[e & 1], x0, x1);
+                            p[e] = pack16x2<F16>(x0, x1);
                         }
-                        sum += s0 + s1;
-                        at_tmem_st_x16(tmem + lanes + 16 * c, p);  // (over scores that have been read)
+                        at_tmem_st_x16(s_cols + 16 * c, p);  // (over scores that have been read)
                     }
+                    sum += at_sum2(sums[0]) + at_sum2(sums[1]);
                     dg_tmem_st_wait();
                 }
                 dg_fence_before();
-                mbar_arrive(weighed);
+                mbar_arrive(bar_of(weighed, n));
             }
             if (!ok) break;
             if (!(ok = mbar_wait_bounded_warp(summed, seg & 1, limit))) break;

@@ -1,0 +1,151 @@
+"""The barriers of tree_attention's tcgen05 kernel, modelled on the host: its warp roles as coroutines under random schedules, with
+waits that, like an mbarrier's, tell a phase from its neighbour only.  No schedule may deadlock, and nothing may be written while it is
+still to be read: the stages of K and V, the scores, the sums, the words that say which keys there are."""
+import random
+
+import pytest
+
+LOADERS = 3
+
+
+class Bar:
+    """An mbarrier: `count` arrivals complete a phase; a wait on parity p passes unless the current phase has that parity."""
+
+    def __init__(self, count):
+        self.count, self.pending, self.phase = count, count, 0
+
+    def arrive(self):
+        self.pending -= 1
+        if self.pending == 0:
+            self.pending, self.phase = self.count, self.phase + 1
+
+    def passes(self, parity):
+        return self.phase % 2 != parity
+
+
+def run(segments, seed, rescale=0.5):
+    rng = random.Random(seed)
+    total = sum(segments)
+    k_full, v_full, scored, weighed = ([Bar(1), Bar(1)] for _ in range(4))
+    added, q_full, summed = [Bar(1) for _ in range(4)], Bar(1), Bar(1)
+    K, V, S, valid = [None] * 2, [None] * 2, [None] * 2, [None] * 4  # what each place holds
+    queue, state = [], dict(q=None, o=None, weights={}, done=0)
+
+    def phase(t):
+        return t >> 1 & 1
+
+    def loader(w):
+        turn, n = w, 0
+        for tiles in segments:
+            for _ in range(tiles):
+                for is_v in (0, 1):
+                    turn -= 1
+                    if turn >= 0:
+                        continue
+                    turn = LOADERS - 1
+                    if n > 1:
+                        yield (added[(n - 2) % 4], (n - 2) >> 2 & 1) if is_v else (scored[n % 2], phase(n - 2))
+                    place = V if is_v else K
+                    assert place[n % 2] is None or place[n % 2][1] == "read", (n, is_v, place)
+                    place[n % 2] = (n, "loading")
+                    if not is_v:
+                        assert valid[n % 4] is None or valid[n % 4][1] == "read"
+                        valid[n % 4] = (n, "there")
+                    yield None
+                    place[n % 2] = (n, "there")
+                    (v_full if is_v else k_full)[n % 2].arrive()
+                n += 1
+
+    def score(n):
+        yield k_full[n % 2], phase(n)
+        assert K[n % 2] == (n, "there")
+        queue.append(("score", n))
+
+    def products():
+        n = 0
+        for seg, tiles in enumerate(segments):
+            yield q_full, seg % 2
+            yield from score(n)
+            for i in range(tiles):
+                if i + 1 < tiles:
+                    yield from score(n + 1)
+                yield v_full[n % 2], phase(n)
+                yield weighed[n % 2], phase(n)
+                assert V[n % 2] == (n, "there")
+                queue.append(("add", n, i == 0, i + 1 == tiles))
+                n += 1
+
+    def tensor_cores():
+        """Takes the products in the order they were issued; a commit's arrival comes a while after its product."""
+        while state["done"] < 2 * total:
+            if not queue:
+                yield None
+                continue
+            op = queue.pop(0)
+            n = op[1]
+            yield None
+            if op[0] == "score":
+                assert K[n % 2] == (n, "there") and state["q"] is not None
+                assert S[n % 2] is None or S[n % 2][1] == "added", "scores over weights that are still wanted"
+                yield None
+                S[n % 2], K[n % 2] = (n, "scores"), (n, "read")
+                scored[n % 2].arrive()
+            else:
+                assert V[n % 2] == (n, "there") and S[n % 2] == (n, "weights")
+                assert state["o"] != "busy"
+                yield None
+                S[n % 2], V[n % 2] = (n, "added"), (n, "read")
+                state["o"] = n
+                added[n % 4].arrive()
+                if op[3]:
+                    summed.arrive()
+            state["done"] += 1
+
+    def softmax():
+        n = 0
+        for seg, tiles in enumerate(segments):
+            state["q"] = seg
+            yield None
+            q_full.arrive()
+            for i in range(tiles):
+                yield scored[n % 2], phase(n)
+                assert S[n % 2] == (n, "scores") and valid[n % 4] == (n, "there")
+                yield None
+                valid[n % 4] = (n, "read")
+                if i > 0 and rng.random() < rescale:
+                    yield added[(n - 1) % 4], (n - 1) >> 2 & 1
+                    assert state["o"] == n - 1, "sums rescaled before the last product is in them"
+                    state["o"] = "busy"
+                    yield None
+                    state["o"] = n - 1
+                assert S[n % 2] == (n, "scores")
+                S[n % 2] = (n, "weights")
+                weighed[n % 2].arrive()
+                n += 1
+            yield summed, seg % 2
+            assert state["o"] == n - 1
+            yield None
+
+    roles = {name: [r, None] for name, r in [("mma", products()), ("tc", tensor_cores()), ("softmax", softmax())] +
+             [(f"load{w}", loader(w)) for w in range(LOADERS)]}
+    speed = {name: rng.choice([1, 1, 3, 30]) for name in roles}  # some roles far behind the others
+    idle = 0
+    while roles:
+        name = rng.choices(list(roles), [1.0 / speed[k] for k in roles])[0]
+        role, wait = roles[name]
+        if wait is not None and not wait[0].passes(wait[1]):
+            idle += 1
+            assert idle < 20000, f"no progress: {sorted(roles)} at {state}"
+            continue
+        idle = 0
+        try:
+            roles[name][1] = next(role)
+        except StopIteration:
+            del roles[name]
+    assert state["done"] == 2 * total and not queue
+
+
+@pytest.mark.parametrize("segments", [[1], [2], [3], [1, 1, 1, 1, 1], [2, 1, 3, 1, 1, 4], [17], [5, 9, 1, 6], [40]])
+def test_no_schedule_deadlocks_or_overwrites(segments):
+    for seed in range(120):
+        run(segments, seed, rescale=(0.0, 0.5, 1.0)[seed % 3])
