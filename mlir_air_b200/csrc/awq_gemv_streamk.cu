@@ -238,6 +238,18 @@ int encode_tensor_map_2d(CUtensorMap *map, int dtype, const void *base, uint64_t
     return encode_tensor_map_3d(map, dtype, base, dim0, dim1, 0, stride1_bytes, 0, box0, box1, 1, swizzle);
 }
 
+int encode_tensor_map_4d(CUtensorMap *map, int dtype, const void *base, const uint64_t (&dims)[4], const uint64_t (&strides_bytes)[3],
+                         const uint32_t (&box)[4], int swizzle) {
+    PFN_cuTensorMapEncodeTiled_v12000 fn = get_encode_fn();
+    if (!fn) return set_error(AWQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]}, s[3] = {strides_bytes[0], strides_bytes[1], strides_bytes[2]};
+    const cuuint32_t b[4] = {box[0], box[1], box[2], box[3]}, estr[4] = {1, 1, 1, 1};
+    CUresult r = fn(map, (CUtensorMapDataType)dtype, 4, const_cast<void *>(base), d, s, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    (CUtensorMapSwizzle)swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(AWQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d, four dimensions)", (int)r);
+    return AWQ_OK;
+}
+
 // A rank signals once per EPI_F32_PUSH launch, when its last sub-strip is stored.
 int gemv_push_arrivals_per_rank(int N) {
     (void)N;

@@ -12,6 +12,9 @@
 
 namespace awq {
 
+int encode_tensor_map_4d(CUtensorMap *map, int dtype, const void *base, const uint64_t (&dims)[4], const uint64_t (&strides_bytes)[3],
+                         const uint32_t (&box)[4], int swizzle);
+
 struct AttendArgs {
     const uint16_t *q;
     long long q_row, q_head;
@@ -551,9 +554,11 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
 // =====================================================================================
 // Many rows per cache head (trees, prompts): tcgen05, 128 rows at a time.
 //
-// A unit of work is 64 keys of a segment = (request, cache head, 128 rows), split over the CTAs and joined as above.  Two CTAs an SM;
+// A unit of work is 64 keys of a segment = (request, cache head, 128 rows), split over the CTAs as above.  Two CTAs an SM;
 // in each
-//   3 warps  copy K and V (16-byte asynchronous copies, whole lines) into the 128-byte swizzle, two tiles of each held;
+//   2 warps  bring K and V by TMA, box by box of slots that lie in one page, two tiles of each held (pages that do not consist of
+//            eights of slots: by 16-byte asynchronous copies into the same 128-byte swizzle);
+//   1 warp   brings Q of the next segment while the last tiles of this one are weighed;
 //   1 warp   issues the products: S = Q K^T into 64 columns of tensor memory, O += P V into D others;
 //   4 warps  hold a row per thread: maximum, weights, and P as 16-bit pairs over S's own columns, from where the tensor cores take
 //            it as the left operand of the next product.
@@ -563,15 +568,20 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
 // Weights are rounded to the rows' 16-bit type for the product, as they have to be for one tensor-core operand (their sum is
 // not): half a step per weight, independent from key to key.
 // =====================================================================================
-constexpr int AT_ROWS = 128, AT_TILE = 64, AT_LOADERS = 3, AT_THREADS = 8 * 32, AT_PER_SM = 2, AT_MAX_CTAS = 192 * AT_PER_SM, AT_COLS = 256;
-static_assert(AT_MAX_CTAS <= AR_MAX_CTAS, "the counters of both kernels share their place");
+constexpr int AT_ROWS = 128, AT_TILE = 64, AT_THREADS = 8 * 32, AT_PER_SM = 2, AT_MAX_CTAS = 192 * AT_PER_SM, AT_COLS = 256;
+// A segment that begins in a CTA and goes on behind it: where it ends, and its rows.  The next launch joins its parts.
+struct AttendJoin {
+    int last, q0, n, hk, m;
+};
+constexpr int AT_JOINS = 4 * AR_MAX_CTAS;  // their place in the scratch, behind the other kernel's counters
 struct AttendTilesShared {
-    // mbarriers, of even and odd tiles: K, V there; QK^T, PV (of every fourth) done; P there.  Of a segment: Q there, O done.
-    uint64_t k_full[2], v_full[2], scored[2], added[4], weighed[2], q_full, summed;
+    // mbarriers, of even and odd tiles: K, V there; QK^T, PV (of every fourth) done; P there.  Of a segment: Q there, Q done with, O done.  V that is
+    // not ready for the product yet.
+    uint64_t k_full[2], v_full[2], scored[2], added[4], weighed[2], q_full, q_free, summed, v_landed;
     uint32_t tmem;
-    int last, odd[2], pad;
+    int odd[2], pad;
     uint32_t valid[4][2];                  // of a tile: which of its keys there are
-    long long places[AT_LOADERS][AT_TILE];  // of a copying warp: the keys of its tile
+    long long places[2][AT_TILE];  // of a copying warp: the keys of its tile
 };
 template <int D>
 constexpr int AT_OPERAND = AT_TILE * D * 2;
@@ -669,8 +679,40 @@ __device__ __forceinline__ void at_copy_keys(uint32_t dst0, uint32_t dst1, const
     }
 }
 
+// A weight of 0 must not meet infinity or NaN: in V's tile the slots without a token become 0, and of the keys from `from` on, which
+// some rows do not see, what is not finite; that is added where it is seen, at the segment's end.  A warp: eight lanes a line.
 template <bool F16, int D>
-__global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_kernel(AttendArgs a, int min_units, long long limit) {
+__device__ __forceinline__ void at_clean(uint8_t *tile, const uint32_t (&valid)[2], int from, int lane, int *odd) {
+    const unsigned long long there = (unsigned long long)valid[1] << 32 | valid[0];
+    uint8_t *mine = tile + (lane >> 3) * 128 + (lane & 7) * 16;
+    const int q0 = (int)(there == ~0ull ? max(from, 0) : 0) / 4;
+#pragma unroll 1
+    for (int h = 0; h < D / 64; ++h)
+#pragma unroll 1
+        for (int q = q0 & ~3; q < AT_TILE / 4; q += 4) {
+            uint4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4 *>(mine + h * AT_TILE * 128 + (q + i) * 512);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int k = 4 * (q + i) + (lane >> 3);
+                const bool is = there >> k & 1;
+                const bool bad = not_finite16x2<F16>(v[i].x) || not_finite16x2<F16>(v[i].y) || not_finite16x2<F16>(v[i].z) || not_finite16x2<F16>(v[i].w);
+                if (is && !(bad && k >= from)) continue;
+                uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+                if (is) *odd = 1;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    w[e] = !is ? 0 : w[e] & (not_finite16x2<F16>(w[e] & 0xffffu) ? 0xffff0000u : 0xffffffffu) & (not_finite16x2<F16>(w[e] >> 16) ? 0xffffu : 0xffffffffu);
+                *reinterpret_cast<uint4 *>(mine + h * AT_TILE * 128 + (q + i) * 512) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+}
+
+template <bool F16, int D>
+__global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_kernel(AttendArgs a, const __grid_constant__ CUtensorMap k_map,
+                                                                                            const __grid_constant__ CUtensorMap v_map, int box,
+                                                                                            int min_units, long long limit) {
     constexpr uint32_t IDESC = (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(AT_ROWS >> 4) << 24);
     constexpr uint32_t IDESC_QK = IDESC | ((uint32_t)(AT_TILE >> 3) << 17), IDESC_PV = IDESC | (1u << 16) | ((uint32_t)(D >> 3) << 17);
     constexpr int HALF = AT_TILE * 128, Q_HALF = AT_ROWS * 128;  // bytes of 64 columns of an operand
@@ -683,18 +725,20 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int group = a.n_heads / a.cache.n_kv, page_size = a.cache.page_size;
     const uint32_t k_full = smem_u32(sh.k_full), v_full = smem_u32(sh.v_full), scored = smem_u32(sh.scored), added = smem_u32(sh.added),
-                   weighed = smem_u32(sh.weighed), q_full = smem_u32(&sh.q_full), summed = smem_u32(&sh.summed);
+                   weighed = smem_u32(sh.weighed), q_full = smem_u32(&sh.q_full), q_free = smem_u32(&sh.q_free), summed = smem_u32(&sh.summed);
     if (tid == 0) {
         for (int b = 0; b < 16; b += 8) {
-            mbar_init(k_full + b, 32);
-            mbar_init(v_full + b, 32);
+            mbar_init(k_full + b, 1);
+            mbar_init(v_full + b, 1);
             mbar_init(scored + b, 1);
             mbar_init(added + b, 1);
             mbar_init(added + 16 + b, 1);
             mbar_init(weighed + b, 128);
         }
-        mbar_init(q_full, 128);
+        mbar_init(q_full, 1);
+        mbar_init(q_free, 1);
         mbar_init(summed, 1);
+        mbar_init(smem_u32(&sh.v_landed), 1);
         mbar_fence_init();
         sh.odd[0] = sh.odd[1] = 0;
     }
@@ -721,73 +765,137 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
     bool ok = true;
     int n = 0;  // tiles so far: tile n has place n % 2 of everything that is held twice, in phase n / 2 % 2
     auto bar_of = [](uint32_t bar, int t) { return bar + 8 * (t & 1); };
+    // keys that all rows of a segment see, from the front on
+    auto seen_by_all = [&](const AttendSegment &s) { return s.rq.len + (a.mask ? 0 : s.m * AT_ROWS / group + 1); };
     auto phase_of = [](int t) { return (uint32_t)(t >> 1 & 1); };
     auto added_of = [&](int t) { return added + 8 * (t & 3); };
     auto added_phase = [](int t) { return (uint32_t)(t >> 2 & 1); };
 
-    if (warp >= 4 && warp < 4 + AT_LOADERS) {
-        // ---- copies: K and V of tile after tile, in turn ----
-        const int ck = lane >> 3, cp = lane & 7;
-        long long *places = sh.places[warp - 4];
-        int turn = warp - 4;  // loads until the next one of this warp
+    if (box && (warp == 4 || warp == 5)) {
+        // ---- TMA: warp 4 K, warp 5 V; lane l brings box l of a tile ----
+        const bool is_v = warp == 5;
+        const CUtensorMap *map = is_v ? &v_map : &k_map;
+        const int boxes = AT_TILE / box;
+        const uint32_t landed = smem_u32(&sh.v_landed);
+        int cleaned = 0;  // tiles that went through `landed`
+        if (lane == 0) tma_prefetch_desc(map);
         for (int seg = 0; ok && walk.next(g); ++seg) {
             const int total = g.rq.len + g.rq.n;
             const int32_t *table = a.table + g.r * a.table_stride;
-            for (int i = 0; ok && i < g.tiles; ++i, ++n) {
-#pragma unroll 1
-                for (int is_v = 0; is_v < 2; ++is_v) {
-                    if (turn-- > 0) continue;
-                    turn = AT_LOADERS - 1;
-                    const int key0 = (g.tile0 + i) * AT_TILE;
-                    const uint16_t *base = (is_v ? a.cache.v + g.hk * a.cache.v_head : a.cache.k + g.hk * a.cache.k_head) + 8 * cp;
-                    const long long s_page = is_v ? a.cache.v_page : a.cache.k_page, s_slot = is_v ? a.cache.v_slot : a.cache.k_slot;
-                    uint32_t valid[2];
-                    __syncwarp();
+            auto page_of = [&](int i) {
+                const int key = (g.tile0 + i) * AT_TILE + lane * box;
+                return i < g.tiles && lane < boxes && key < total ? __ldg(table + page_index(a, key)) : -1;
+            };
+            int page = page_of(0);
+            for (int i = 0; i < g.tiles; ++i, ++n) {
+                const int key0 = (g.tile0 + i) * AT_TILE, first = key0 + lane * box, off = first - page_index(a, first) * page_size;
+                const bool there = (unsigned)page < (unsigned)a.cache.n_pages;
+                if (lane < boxes && first < total && !there) req_error(&a.header->error, REQ_ERR_PAGE);
+                const uint32_t got = __ballot_sync(0xffffffffu, there);
+                uint32_t valid[2];
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int key = key0 + 32 * k + lane, block = page_index(a, key);
-                        const int page = key < total ? __ldg(table + block) : -1;
-                        const bool there = (unsigned)page < (unsigned)a.cache.n_pages;
-                        if (key < total && !there) req_error(&a.header->error, REQ_ERR_PAGE);
-                        places[32 * k + lane] = there ? page * s_page + (key - block * page_size) * s_slot : -8;
-                        valid[k] = __ballot_sync(0xffffffffu, there);
-                    }
-                    __syncwarp();
-                    // A wait tells a phase from the one before it only, so that one has to be known to be over.  For K: this warp's last
-                    // load was V of tile n - 2, behind the sum of tile n - 4.  For V, whose four barriers come round every four
-                    // tiles: it was K of tile n - 1, behind the scores of n - 3, which were asked for behind the sum of n - 5.
-                    if (n > 1 && !(ok = is_v ? mbar_wait_bounded_warp(added_of(n - 2), added_phase(n - 2), limit)
-                                             : mbar_wait_bounded_warp(bar_of(scored, n), phase_of(n - 2), limit)))
-                        break;
-                    // (scores of tile n - 2 were asked for behind the weights of tile n - 4, whose place this is)
-                    if (!is_v && lane == 0) sh.valid[n & 3][0] = valid[0], sh.valid[n & 3][1] = valid[1];
-                    const uint32_t to = smem_u32((is_v ? vs : ks) + (n & 1) * AT_OPERAND<D>) + ck * 128;
-                    at_copy_keys<D, 0, AT_TILE / 4>(to + (cp ^ ck) * 16, to + (cp ^ ck ^ 4) * 16, base, places + ck);
-                    asm volatile("cp.async.wait_all;" ::: "memory");
-                    if (is_v && key0 + AT_TILE > g.rq.len) {
-                        // new tokens that some rows do not see: what is not finite is taken out here and added where it is seen, at the end
-                        uint8_t *mine = vs + (n & 1) * AT_OPERAND<D>;
-#pragma unroll 1
-                        for (int q = 0; q < AT_TILE / 4; ++q) {
-                            if (key0 + 4 * q + ck < g.rq.len) continue;
-#pragma unroll 1
-                            for (int w = 0; w < 4 * (D / 64); ++w) {
-                                uint32_t &v = reinterpret_cast<uint32_t *>(mine + (w >> 2) * HALF + (4 * q + ck) * 128 + (cp ^ ((4 * q + ck) & 7)) * 16)[w & 3];
-                                if (!not_finite16x2<F16>(v)) continue;
-                                sh.odd[seg & 1] = 1;
-                                v &= (not_finite16x2<F16>(v & 0xffffu) ? 0xffff0000u : 0xffffffffu) & (not_finite16x2<F16>(v >> 16) ? 0xffffu : 0xffffffffu);
-                            }
-                        }
-                    }
+                for (int k = 0; k < 2; ++k)
+                    valid[k] = __ballot_sync(0xffffffffu, (got >> ((32 * k + lane) / box) & 1) && key0 + 32 * k + lane < total);
+                // (A wait tells a phase from the one before it only; that one, of tile n - 4 or n - 6, this warp has seen.)
+                if (n > 1 && !(ok = is_v ? mbar_wait_bounded_warp(added_of(n - 2), added_phase(n - 2), limit)
+                                         : mbar_wait_bounded_warp(bar_of(scored, n), phase_of(n - 2), limit)))
+                    break;
+                // (scores of tile n - 2 were asked for behind the weights of tile n - 4, whose place this is)
+                if (!is_v && lane == 0) sh.valid[n & 3][0] = valid[0], sh.valid[n & 3][1] = valid[1];
+                // V of new tokens and of slots without a token: see below
+                const bool clean = is_v && (key0 + AT_TILE > seen_by_all(g) || (valid[0] & valid[1]) != 0xffffffffu);
+                const uint32_t bar = clean ? landed : bar_of(is_v ? v_full : k_full, n);
+                if (lane == 0) mbar_expect_tx(bar, __popc(got) * box * 128 * (D / 64));
+                __syncwarp();
+                if (there) {
+                    const uint32_t dst = smem_u32((is_v ? vs : ks) + (n & 1) * AT_OPERAND<D>) + lane * box * 128;
+#pragma unroll
+                    for (int h = 0; h < D / 64; ++h) tma_load_4d(dst + h * HALF, map, 64 * h, g.hk, off, page, bar);
+                }
+                page = page_of(i + 1);
+                if (clean) {
+                    // A weight of 0 must not meet infinity or NaN: slots without a token become 0, and of new tokens, which some rows do
+                    // not see, what is not finite; it is added where it is seen, at the end.
+                    if (!(ok = mbar_wait_bounded_warp(landed, cleaned++ & 1, limit))) break;
+                    at_clean<F16, D>(vs + (n & 1) * AT_OPERAND<D>, valid, seen_by_all(g) - key0, lane, &sh.odd[seg & 1]);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    mbar_arrive(bar_of(is_v ? v_full : k_full, n));
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_of(v_full, n));
                 }
             }
+        }
+    } else if (warp == 4 || warp == 5) {
+        // ---- the same by copies: lanes 8 i to 8 i + 7 bring lines of keys 4 q + i ----
+        const bool is_v = warp == 5;
+        const int ck = lane >> 3, cp = lane & 7;
+        long long *places = sh.places[is_v];
+        for (int seg = 0; ok && walk.next(g); ++seg) {
+            const int total = g.rq.len + g.rq.n;
+            const int32_t *table = a.table + g.r * a.table_stride;
+            const uint16_t *base = (is_v ? a.cache.v + g.hk * a.cache.v_head : a.cache.k + g.hk * a.cache.k_head) + 8 * cp;
+            const long long s_page = is_v ? a.cache.v_page : a.cache.k_page, s_slot = is_v ? a.cache.v_slot : a.cache.k_slot;
+            for (int i = 0; i < g.tiles; ++i, ++n) {
+                const int key0 = (g.tile0 + i) * AT_TILE;
+                uint32_t valid[2];
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int key = key0 + 32 * k + lane, block = page_index(a, key);
+                    const int page = key < total ? __ldg(table + block) : -1;
+                    const bool there = (unsigned)page < (unsigned)a.cache.n_pages;
+                    if (key < total && !there) req_error(&a.header->error, REQ_ERR_PAGE);
+                    places[32 * k + lane] = there ? page * s_page + (key - block * page_size) * s_slot : -8;
+                    valid[k] = __ballot_sync(0xffffffffu, there);
+                }
+                __syncwarp();
+                if (n > 1 && !(ok = is_v ? mbar_wait_bounded_warp(added_of(n - 2), added_phase(n - 2), limit)
+                                         : mbar_wait_bounded_warp(bar_of(scored, n), phase_of(n - 2), limit)))
+                    break;
+                if (!is_v && lane == 0) sh.valid[n & 3][0] = valid[0], sh.valid[n & 3][1] = valid[1];
+                const uint32_t to = smem_u32((is_v ? vs : ks) + (n & 1) * AT_OPERAND<D>) + ck * 128;
+                at_copy_keys<D, 0, AT_TILE / 4>(to + (cp ^ ck) * 16, to + (cp ^ ck ^ 4) * 16, base, places + ck);
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                __syncwarp();
+                if (is_v && (key0 + AT_TILE > seen_by_all(g) || (valid[0] & valid[1]) != 0xffffffffu))
+                    at_clean<F16, D>(vs + (n & 1) * AT_OPERAND<D>, valid, seen_by_all(g) - key0, lane, &sh.odd[seg & 1]);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_of(is_v ? v_full : k_full, n));
+            }
+        }
+    } else if (warp == 6) {
+        // ---- Q of segment after segment, as soon as the last scores of the one before are there ----
+        const int ck = lane >> 3, cp = lane & 7;
+        for (int seg = 0; ok && walk.next(g); ++seg) {
+            if (seg && !(ok = mbar_wait_bounded_warp(q_free, (seg - 1) & 1, limit))) break;
+            const int rows = (int)min((long long)AT_ROWS, (long long)g.rq.n * group - (long long)g.m * AT_ROWS);
+            const uint32_t to = smem_u32(qs) + ck * 128;
+            const uint16_t *base = a.q + (long long)g.rq.q0 * a.q_row + (long long)g.hk * group * a.q_head + 8 * cp;
+            int j = (g.m * AT_ROWS + ck) / group, h = (g.m * AT_ROWS + ck) % group;  // of row 4 q + ck
+            for (int q = 0; q < AT_ROWS / 4; ++q) {
+                copies16<D / 64, Q_HALF, 128>(to + q * 512 + (cp ^ ((4 * q + ck) & 7)) * 16, base + (4 * q + ck < rows ? j * a.q_row + h * a.q_head : 0),
+                                              4 * q + ck < rows ? 16 : 0);
+                for (h += 4; h >= group; h -= group) ++j;
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (a.scale_log2 < 0.f) {  // a negative scale turns Q's signs
+                __syncwarp();
+                for (int q = 0; q < AT_ROWS / 4; ++q)
+#pragma unroll
+                    for (int x = 0; x < D / 64; ++x) {
+                        uint4 &v = *reinterpret_cast<uint4 *>(qs + x * Q_HALF + (4 * q + ck) * 128 + cp * 16);
+                        v = make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u);
+                        // (every piece of a row is some lane's, whatever its place)
+                    }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
         }
     } else if (warp == 7) {
         // ---- products: the scores of a tile are asked for before the weighted sum of the one in front of it ----
         const uint64_t q_desc = dg_desc_sw128(smem_u32(qs)), k_desc = dg_desc_sw128(smem_u32(ks)), v_desc = at_desc_mn(smem_u32(vs), HALF);
-        auto score = [&](int t) {
+        auto score = [&](int t, bool last) {
             ok = mbar_wait_bounded_warp(bar_of(k_full, t), phase_of(t), limit);
             if (!ok) return;
             dg_fence_after();
@@ -797,14 +905,15 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
                 for (int k = 0; k < D / 16; ++k)
                     dg_umma_bf16(tmem + (t & 1) * AT_TILE, q_desc + (k >> 2) * (Q_HALF >> 4) + 2 * (k & 3), kd + (k >> 2) * (HALF >> 4) + 2 * (k & 3), IDESC_QK, k > 0);
                 dg_umma_commit(bar_of(scored, t));
+                if (last) dg_umma_commit(q_free);
             }
             __syncwarp();
         };
         for (int seg = 0; ok && walk.next(g); ++seg) {
             if (!(ok = mbar_wait_bounded_warp(q_full, seg & 1, limit))) break;
-            score(n);
+            score(n, g.tiles == 1);
             for (int i = 0; ok && i < g.tiles; ++i, ++n) {
-                if (i + 1 < g.tiles) score(n + 1);
+                if (i + 1 < g.tiles) score(n + 1, i + 2 == g.tiles);
                 if (!ok) break;
                 if (!(ok = mbar_wait_bounded_warp(bar_of(v_full, n), phase_of(n), limit) && mbar_wait_bounded_warp(bar_of(weighed, n), phase_of(n), limit))) break;
                 dg_fence_after();
@@ -819,33 +928,19 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
                 __syncwarp();
             }
         }
-    } else {
+    } else if (warp < 4) {
         // ---- a row a thread ----
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
         const float scale = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);  // (a negative one has turned Q's signs; 0 times -inf is not a number)
-        float *parts = reinterpret_cast<float *>(a.scratch + 4 * AR_MAX_CTAS);
-        int *counters = reinterpret_cast<int *>(a.scratch);
+        float *parts = reinterpret_cast<float *>(a.scratch + AT_JOINS + sizeof(AttendJoin) * AT_MAX_CTAS);
+        AttendJoin *joins = reinterpret_cast<AttendJoin *>(a.scratch + AT_JOINS);
+        bool joined = false;
         for (int seg = 0; ok && walk.next(g); ++seg) {
             const int rows = (int)min((long long)AT_ROWS, (long long)g.rq.n * group - (long long)g.m * AT_ROWS);
             const bool mine = tid < rows, busy = warp * 32 < rows;
             const int row = g.m * AT_ROWS + tid, j = row / group, head = g.hk * group + row % group;
             const unsigned long long bits = a.mask && mine ? (unsigned long long)a.mask[g.rq.q0 + j] : 0;
-            const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
-            // Q, eight lanes a line
-            for (int q = tid >> 3; q < AT_ROWS; q += 16) {
-                const int rw = g.m * AT_ROWS + q;
-                const uint16_t *src = a.q + (long long)(g.rq.q0 + rw / group) * a.q_row + (long long)(g.hk * group + rw % group) * a.q_head + 8 * (tid & 7);
-#pragma unroll
-                for (int h = 0; h < D / 64; ++h) {
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (q < rows) v = *reinterpret_cast<const uint4 *>(src + 64 * h);
-                    v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-                    *reinterpret_cast<uint4 *>(qs + h * Q_HALF + q * 128 + ((tid & 7) ^ (q & 7)) * 16) = v;
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            dg_fence_before();
-            mbar_arrive(q_full);
+            const int all_see = seen_by_all(g);
             float top = -INFINITY, sum = 0.f;
             for (int i = 0; i < g.tiles; ++i, ++n) {
                 if (!(ok = mbar_wait_bounded_warp(bar_of(scored, n), phase_of(n), limit))) break;
@@ -858,7 +953,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
                     dg_tmem_ld_32x32b_x32(s_cols + 32, v[1]);
                     uint32_t vis[2] = {sh.valid[n & 3][0], sh.valid[n & 3][1]};
                     dg_tmem_ld_wait();
-                    if (key0 + AT_TILE > g.rq.len || (vis[0] & vis[1]) != 0xffffffffu) at_mask(a, g.rq, key0, j, bits, vis, v);
+                    if (key0 + AT_TILE > all_see || (vis[0] & vis[1]) != 0xffffffffu) at_mask(a, g.rq, key0, j, bits, vis, v);
                     float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
                     for (int e = 0; e < 32; ++e) m0 = fmaxf(m0, __uint_as_float(v[0][e])), m1 = fmaxf(m1, __uint_as_float(v[1][e]));
@@ -951,40 +1046,14 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
                 if (!whole) part[D * AT_ROWS + tid] = top, part[(D + 1) * AT_ROWS + tid] = sum;
             }
             dg_fence_before();
-            if (!whole) __threadfence();
             named_bar_sync(1, 128);
-            if (tid == 0) sh.odd[seg & 1] = 0;
-            if (!whole) {
-                if (tid == 0) sh.last = atomicAdd(counters + c0, 1) == c1 - c0;
-                named_bar_sync(1, 128);
-                if (sh.last) {
-                    __threadfence();
-                    if (mine) {
-                        float m = -INFINITY, total = 0.f;
-                        for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(parts + (long long)(2 * c + (c == c0)) * PART + D * AT_ROWS + tid));
-                        const float ref = m == -INFINITY ? 0.f : m;
-                        for (int c = c0; c <= c1; ++c) {
-                            const float *src = parts + (long long)(2 * c + (c == c0)) * PART + D * AT_ROWS + tid;
-                            total += exp2_fast(__ldcg(src) - ref) * __ldcg(src + AT_ROWS);
-                        }
-#pragma unroll 1
-                        for (int q = 0; q < D / 32; ++q) {
-                            float o[32] = {};
-                            for (int c = c0; c <= c1; ++c) {
-                                const float *src = parts + (long long)(2 * c + (c == c0)) * PART + tid;
-                                const float f = exp2_fast(__ldcg(src + D * AT_ROWS) - ref);
-                                if (f == 0.f) continue;
-#pragma unroll
-                                for (int e = 0; e < 32; ++e) o[e] = fmaf(f, __ldcg(src + (32 * q + e) * AT_ROWS), o[e]);
-                            }
-                            store32(q, o, total);
-                        }
-                    }
-                    if (tid == 0) counters[c0] = 0;
-                }
-                named_bar_sync(1, 128);  // (`last` is one segment's at a time)
+            if (tid == 0) {
+                sh.odd[seg & 1] = 0;
+                // what begins here and goes on is this CTA's last segment
+                if (!whole && (int)blockIdx.x == c0) joins[blockIdx.x] = AttendJoin{c1, g.rq.q0, g.rq.n, g.hk, g.m}, joined = true;
             }
         }
+        if (tid == 0 && !joined) joins[blockIdx.x].last = -1;
     }
     if (!ok && lane == 0) req_error(&a.header->error, REQ_ERR_TIMEOUT);
     dg_fence_before();
@@ -993,8 +1062,44 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
     if (warp == 6) dg_tmem_dealloc(tmem, AT_COLS);
 }
 
+// The parts of the segments that several CTAs have shared: a CTA per segment and 16 columns, a thread per row.  (Done by the last
+// CTA to finish a segment it took that one 10 to 15 us, with its next segment waiting.)
+constexpr int AJ_COLS = 16;
+template <bool F16, int D>
+__global__ void __launch_bounds__(AT_ROWS) tree_attention_join_kernel(AttendArgs a) {
+    pdl_wait();
+    pdl_launch_dependents();
+    constexpr int PART = AT_ROWS * (D + 2);
+    const int c0 = blockIdx.x, tid = threadIdx.x, d0 = blockIdx.y * AJ_COLS, group = a.n_heads / a.cache.n_kv;
+    const AttendJoin s = reinterpret_cast<const AttendJoin *>(a.scratch + AT_JOINS)[c0];
+    const int row = s.m * AT_ROWS + tid;
+    if (s.last < 0 || row >= s.n * group) return;
+    const float *parts = reinterpret_cast<const float *>(a.scratch + AT_JOINS + sizeof(AttendJoin) * AT_MAX_CTAS);
+    float top = -INFINITY, total = 0.f, o[AJ_COLS] = {};
+#pragma unroll 2
+    for (int c = c0; c <= s.last; ++c) {
+        const float *src = parts + (long long)(2 * c + (c == c0)) * PART + tid;
+        const float m = src[D * AT_ROWS], l = src[(D + 1) * AT_ROWS];
+        float v[AJ_COLS];
+#pragma unroll
+        for (int e = 0; e < AJ_COLS; ++e) v[e] = src[(d0 + e) * AT_ROWS];
+        const float to = fmaxf(top, m), ref = to == -INFINITY ? 0.f : to, keep = exp2_fast(top - ref), f = exp2_fast(m - ref);
+        top = to;
+        total = total * keep + l * f;
+#pragma unroll
+        for (int e = 0; e < AJ_COLS; ++e) o[e] = (keep == 0.f ? 0.f : o[e] * keep) + (f == 0.f ? 0.f : v[e] * f);
+    }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    uint16_t *out = a.out + (long long)(s.q0 + row / group) * a.o_row + (long long)(s.hk * group + row % group) * a.o_head + d0;
+#pragma unroll
+    for (int e = 0; e < AJ_COLS; e += 8)
+        *reinterpret_cast<uint4 *>(out + e) = make_uint4(pack16x2<F16>(o[e] * inv, o[e + 1] * inv), pack16x2<F16>(o[e + 2] * inv, o[e + 3] * inv),
+                                                         pack16x2<F16>(o[e + 4] * inv, o[e + 5] * inv), pack16x2<F16>(o[e + 6] * inv, o[e + 7] * inv));
+}
+
 size_t tree_attention_scratch_bytes() {
-    const size_t rows = (size_t)2 * AR_MAX_CTAS * AR_ROWS * (128 + 2) * 4, tiles = (size_t)2 * AT_MAX_CTAS * AT_ROWS * (128 + 2) * 4;
+    const size_t rows = (size_t)2 * AR_MAX_CTAS * AR_ROWS * (128 + 2) * 4,
+                 tiles = sizeof(AttendJoin) * AT_MAX_CTAS + (size_t)2 * AT_MAX_CTAS * AT_ROWS * (128 + 2) * 4;
     return 4 * AR_MAX_CTAS + (rows > tiles ? rows : tiles);
 }
 
@@ -1034,7 +1139,28 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
             const int smem = (view.head_dim == 64 ? AT_SMEM<64> : AT_SMEM<128>) + (R + 1) * 8;
             if ((rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "tree_attention shared memory"))) return rc;
             const int grid = min(device_sm_count() * AT_PER_SM, AT_MAX_CTAS);
-            return check_cuda(launch_pdl(kernel, dim3(grid), dim3(AT_THREADS), smem, as_stream(stream), a, 1, wait_limit_cycles()), "tree_attention launch");
+            // boxes of slots that never straddle a page or a tile
+            int box = AT_TILE;
+            while (box >= 8 && view.page_size % box) box >>= 1;
+            CUtensorMap maps[2] = {};
+            const long long longest = 1LL << 38;  // elements of 2 bytes: TMA strides are below 2^40 bytes
+            if (box < 8 || view.k_page > longest || view.v_page > longest || view.k_slot > longest || view.v_slot > longest || view.k_head > longest || view.v_head > longest)
+                box = 0;
+            for (int i = 0; box && i < 2; ++i) {
+                const long long st[3] = {i ? view.v_head : view.k_head, i ? view.v_slot : view.k_slot, i ? view.v_page : view.k_page};
+                // (a dimension of one may come with a stride of 0)
+                const uint64_t strides[3] = {(uint64_t)max(2 * st[0], 16LL), (uint64_t)max(2 * st[1], 16LL), (uint64_t)max(2 * st[2], 16LL)};
+                if ((rc = encode_tensor_map_4d(&maps[i], f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, i ? view.v : view.k,
+                                               {(uint64_t)view.head_dim, (uint64_t)view.n_kv, (uint64_t)view.page_size, (uint64_t)view.n_pages}, strides,
+                                               {64u, 1u, (uint32_t)box, 1u}, CU_TENSOR_MAP_SWIZZLE_128B)))
+                    return rc;
+            }
+            if ((rc = check_cuda(launch_pdl(kernel, dim3(grid), dim3(AT_THREADS), smem, as_stream(stream), a, maps[0], maps[1], box, 1, wait_limit_cycles()),
+                                 "tree_attention launch")))
+                return rc;
+            auto join = view.head_dim == 64 ? (f16 ? tree_attention_join_kernel<true, 64> : tree_attention_join_kernel<false, 64>)
+                                            : (f16 ? tree_attention_join_kernel<true, 128> : tree_attention_join_kernel<false, 128>);
+            return check_cuda(launch_pdl(join, dim3(grid, view.head_dim / AJ_COLS), dim3(AT_ROWS), 0, as_stream(stream), a), "tree_attention join launch");
         }
         auto kernel = view.head_dim == 64 ? (f16 ? tree_attention_rows_kernel<true, 64> : tree_attention_rows_kernel<false, 64>)
                                           : (f16 ? tree_attention_rows_kernel<true, 128> : tree_attention_rows_kernel<false, 128>);

@@ -5,8 +5,6 @@ import random
 
 import pytest
 
-LOADERS = 3
-
 
 class Bar:
     """An mbarrier: `count` arrivals complete a phase; a wait on parity p passes unless the current phase has that parity."""
@@ -23,52 +21,89 @@ class Bar:
         return self.phase % 2 != parity
 
 
-def run(segments, seed, rescale=0.5):
+def run(segments, seed, rescale=0.5, tma=False):
     rng = random.Random(seed)
     total = sum(segments)
     k_full, v_full, scored, weighed = ([Bar(1), Bar(1)] for _ in range(4))
-    added, q_full, summed = [Bar(1) for _ in range(4)], Bar(1), Bar(1)
+    added, q_full, q_free, summed = [Bar(1) for _ in range(4)], Bar(1), Bar(1), Bar(1)
+    segment_of = [i for i, t in enumerate(segments) for _ in range(t)]
     K, V, S, valid = [None] * 2, [None] * 2, [None] * 2, [None] * 4  # what each place holds
     queue, state = [], dict(q=None, o=None, weights={}, done=0)
 
     def phase(t):
         return t >> 1 & 1
 
-    def loader(w):
-        turn, n = w, 0
+    def loader(is_v):
+        """One warp for K, one for V; it waits for its own copies."""
+        n = 0
         for tiles in segments:
             for _ in range(tiles):
-                for is_v in (0, 1):
-                    turn -= 1
-                    if turn >= 0:
-                        continue
-                    turn = LOADERS - 1
-                    if n > 1:
-                        yield (added[(n - 2) % 4], (n - 2) >> 2 & 1) if is_v else (scored[n % 2], phase(n - 2))
-                    place = V if is_v else K
-                    assert place[n % 2] is None or place[n % 2][1] == "read", (n, is_v, place)
-                    place[n % 2] = (n, "loading")
-                    if not is_v:
-                        assert valid[n % 4] is None or valid[n % 4][1] == "read"
-                        valid[n % 4] = (n, "there")
-                    yield None
-                    place[n % 2] = (n, "there")
-                    (v_full if is_v else k_full)[n % 2].arrive()
+                if n > 1:
+                    yield (added[(n - 2) % 4], (n - 2) >> 2 & 1) if is_v else (scored[n % 2], phase(n - 2))
+                place = V if is_v else K
+                assert place[n % 2] is None or place[n % 2][1] == "read", (n, is_v, place)
+                place[n % 2] = (n, "loading")
+                if not is_v:
+                    assert valid[n % 4] is None or valid[n % 4][1] == "read"
+                    valid[n % 4] = (n, "there")
+                yield None
+                place[n % 2] = (n, "there")
+                (v_full if is_v else k_full)[n % 2].arrive()
                 n += 1
 
-    def score(n):
+    def q_loader():
+        for seg in range(len(segments)):
+            if seg:
+                yield q_free, (seg - 1) % 2
+            assert state["q"] is None or state["q"][1] == "read"
+            state["q"] = (seg, "loading")
+            yield None
+            state["q"] = (seg, "there")
+            q_full.arrive()
+
+    def tma_loader(is_v, landing):
+        """One warp for K, one for V; the bytes arrive by themselves, later, while it goes on.  Some tiles of V are put right first."""
+        n = 0
+        for tiles in segments:
+            for _ in range(tiles):
+                if n > 1:
+                    yield (added[(n - 2) % 4], (n - 2) >> 2 & 1) if is_v else (scored[n % 2], phase(n - 2))
+                place = V if is_v else K
+                assert place[n % 2] is None or place[n % 2][1] == "read", (n, is_v, place)
+                place[n % 2] = (n, "loading")
+                if not is_v:
+                    assert valid[n % 4] is None or valid[n % 4][1] == "read"
+                    valid[n % 4] = (n, "there")
+                if is_v and rng.random() < 0.3:
+                    yield None
+                    place[n % 2] = (n, "there")
+                    v_full[n % 2].arrive()
+                else:
+                    landing.append((place, n, v_full if is_v else k_full))
+                n += 1
+
+    def memory(landing):
+        left = 200 * total
+        while state["done"] < 2 * total and left:
+            if landing:
+                place, n, bar = landing.pop(rng.randrange(len(landing)))
+                place[n % 2] = (n, "there")
+                bar[n % 2].arrive()
+            yield None
+
+    def score(n, last):
         yield k_full[n % 2], phase(n)
         assert K[n % 2] == (n, "there")
-        queue.append(("score", n))
+        queue.append(("score", n, last))
 
     def products():
         n = 0
         for seg, tiles in enumerate(segments):
             yield q_full, seg % 2
-            yield from score(n)
+            yield from score(n, tiles == 1)
             for i in range(tiles):
                 if i + 1 < tiles:
-                    yield from score(n + 1)
+                    yield from score(n + 1, i + 2 == tiles)
                 yield v_full[n % 2], phase(n)
                 yield weighed[n % 2], phase(n)
                 assert V[n % 2] == (n, "there")
@@ -85,14 +120,17 @@ def run(segments, seed, rescale=0.5):
             n = op[1]
             yield None
             if op[0] == "score":
-                assert K[n % 2] == (n, "there") and state["q"] is not None
+                assert K[n % 2] == (n, "there") and state["q"] == (segment_of[n], "there")
                 assert S[n % 2] is None or S[n % 2][1] == "added", "scores over weights that are still wanted"
                 yield None
                 S[n % 2], K[n % 2] = (n, "scores"), (n, "read")
                 scored[n % 2].arrive()
+                if op[2]:
+                    state["q"] = (segment_of[n], "read")
+                    q_free.arrive()
             else:
                 assert V[n % 2] == (n, "there") and S[n % 2] == (n, "weights")
-                assert state["o"] != "busy"
+                assert state["o"] != "busy" and (not op[2] or state["o"] is None), "sums overwritten before they were taken"
                 yield None
                 S[n % 2], V[n % 2] = (n, "added"), (n, "read")
                 state["o"] = n
@@ -104,9 +142,6 @@ def run(segments, seed, rescale=0.5):
     def softmax():
         n = 0
         for seg, tiles in enumerate(segments):
-            state["q"] = seg
-            yield None
-            q_full.arrive()
             for i in range(tiles):
                 yield scored[n % 2], phase(n)
                 assert S[n % 2] == (n, "scores") and valid[n % 4] == (n, "there")
@@ -125,9 +160,12 @@ def run(segments, seed, rescale=0.5):
             yield summed, seg % 2
             assert state["o"] == n - 1
             yield None
+            state["o"] = None
 
-    roles = {name: [r, None] for name, r in [("mma", products()), ("tc", tensor_cores()), ("softmax", softmax())] +
-             [(f"load{w}", loader(w)) for w in range(LOADERS)]}
+    landing = []
+    loaders = [("k", tma_loader(0, landing)), ("v", tma_loader(1, landing)), ("memory", memory(landing))] if tma else \
+        [("k", loader(0)), ("v", loader(1))]
+    roles = {name: [r, None] for name, r in [("mma", products()), ("tc", tensor_cores()), ("softmax", softmax()), ("q", q_loader())] + loaders}
     speed = {name: rng.choice([1, 1, 3, 30]) for name in roles}  # some roles far behind the others
     idle = 0
     while roles:
@@ -145,7 +183,8 @@ def run(segments, seed, rescale=0.5):
     assert state["done"] == 2 * total and not queue
 
 
+@pytest.mark.parametrize("tma", [False, True])
 @pytest.mark.parametrize("segments", [[1], [2], [3], [1, 1, 1, 1, 1], [2, 1, 3, 1, 1, 4], [17], [5, 9, 1, 6], [40]])
-def test_no_schedule_deadlocks_or_overwrites(segments):
-    for seed in range(120):
-        run(segments, seed, rescale=(0.0, 0.5, 1.0)[seed % 3])
+def test_no_schedule_deadlocks_or_overwrites(segments, tma):
+    for seed in range(60):
+        run(segments, seed, rescale=(0.0, 0.5, 1.0)[seed % 3], tma=tma)
