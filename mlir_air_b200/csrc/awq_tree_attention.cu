@@ -645,27 +645,39 @@ struct AttendSegment {
     int r, hk, m, tile0, tiles, n_tiles;
     long long start;  // its first unit
 };
+__device__ __forceinline__ long long at_div(long long x, long long y) { return (x | y) >> 32 ? x / y : (long long)((uint32_t)x / (uint32_t)y); }
 template <int D>
 struct AttendWalk {
     const AttendArgs &a;
     const long long *cum;
     long long x, end;
     int group;
+    long long pad;  // units of a segment come in multiples of this
     __device__ __forceinline__ bool next(AttendSegment &s) {
-        if (x >= end) return false;
-        s.r = request_of_unit(cum, a.R, x);
-        s.rq = attend_request(a, s.r);
-        const long long rem = x - cum[s.r], per_head = (cum[s.r + 1] - cum[s.r]) / a.cache.n_kv;
-        s.hk = (int)(rem / per_head);
-        long long left = rem % per_head;
-        s.m = 0;
-        while (left >= (s.n_tiles = at_tiles(a, s.rq, group, s.m))) left -= s.n_tiles, ++s.m;
-        s.tile0 = (int)left;
-        s.start = x - left;
-        s.tiles = (int)min(end - x, (long long)s.n_tiles - left);
-        x += s.tiles;
-        return true;
+        while (x < end) {
+            s.r = request_of_unit(cum, a.R, x);
+            s.rq = attend_request(a, s.r);
+            const long long rem = x - cum[s.r], per_head = at_div(cum[s.r + 1] - cum[s.r], a.cache.n_kv);
+            s.hk = (int)at_div(rem, per_head);
+            long long left = rem - s.hk * per_head, units;
+            s.m = 0;
+            if (a.mask) {  // all segments of a request are as long
+                s.n_tiles = at_tiles(a, s.rq, group, 0);
+                units = at_padded(s.n_tiles, pad);
+                s.m = (int)at_div(left, units);
+                left -= s.m * units;
+            } else {
+                while (left >= (units = at_padded(s.n_tiles = at_tiles(a, s.rq, group, s.m), pad))) left -= units, ++s.m;
+            }
+            s.tile0 = (int)left;
+            s.start = x - left;
+            s.tiles = (int)min(end - x, (long long)s.n_tiles - left);
+            x += min(end - x, units - left);
+            if (s.tiles > 0) return true;
+        }
+        return false;
     }
+    __device__ __forceinline__ static long long at_padded(int tiles, long long pad) { return pad > 1 ? at_div(tiles + pad - 1, pad) * pad : tiles; }
 };
 
 // Keys 4 q + (the lane's of four) of a tile for q = Q .. END - 1, in lines of 128 bytes swizzled by key % 8: the lane's piece has one
@@ -679,40 +691,54 @@ __device__ __forceinline__ void at_copy_keys(uint32_t dst0, uint32_t dst1, const
     }
 }
 
+// acc + 0 v for two 16-bit values: not a number once v was infinite or none.
+template <bool F16>
+__device__ __forceinline__ uint32_t at_zero_fma(uint32_t v, uint32_t acc) {
+    if (F16) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0u));
+    else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0u));
+    return acc;
+}
+template <bool F16, int D>
+__device__ __noinline__ void at_clean_values(uint8_t *mine, int from, int row, int *odd) {
+#pragma unroll 1
+    for (int k = row; k < AT_TILE; k += 4)
+#pragma unroll 1
+        for (int w = 0; k >= from && w < 4 * (D / 64); ++w) {
+            uint32_t &v = reinterpret_cast<uint32_t *>(mine + (w >> 2) * AT_TILE * 128 + (k - row) * 128)[w & 3];
+            if (!not_finite16x2<F16>(v)) continue;
+            *odd = 1;
+            v &= (not_finite16x2<F16>(v & 0xffffu) ? 0xffff0000u : 0xffffffffu) & (not_finite16x2<F16>(v >> 16) ? 0xffffu : 0xffffffffu);
+        }
+}
 // A weight of 0 must not meet infinity or NaN: in V's tile the slots without a token become 0, and of the keys from `from` on, which
 // some rows do not see, what is not finite; that is added where it is seen, at the segment's end.  A warp: eight lanes a line.
+// (The warp is alone with this, and the product waits for it: a look at every value costs one fused multiply-add for two.)
 template <bool F16, int D>
 __device__ __forceinline__ void at_clean(uint8_t *tile, const uint32_t (&valid)[2], int from, int lane, int *odd) {
-    const unsigned long long there = (unsigned long long)valid[1] << 32 | valid[0];
-    uint8_t *mine = tile + (lane >> 3) * 128 + (lane & 7) * 16;
-    const int q0 = (int)(there == ~0ull ? max(from, 0) : 0) / 4;
-#pragma unroll 1
-    for (int h = 0; h < D / 64; ++h)
-#pragma unroll 1
-        for (int q = q0 & ~3; q < AT_TILE / 4; q += 4) {
-            uint4 v[4];
+    const int row = lane >> 3;
+    uint8_t *mine = tile + row * 128 + (lane & 7) * 16;
+    const uint32_t there[2] = {valid[0] >> row, valid[1] >> row};
+    uint32_t acc[4] = {};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const uint4 *>(mine + h * AT_TILE * 128 + (q + i) * 512);
+    for (int q = 0; q < AT_TILE / 4; ++q) {
+        const bool is = there[q >> 3] >> (4 * (q & 7)) & 1;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int k = 4 * (q + i) + (lane >> 3);
-                const bool is = there >> k & 1;
-                const bool bad = not_finite16x2<F16>(v[i].x) || not_finite16x2<F16>(v[i].y) || not_finite16x2<F16>(v[i].z) || not_finite16x2<F16>(v[i].w);
-                if (is && !(bad && k >= from)) continue;
-                uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-                if (is) *odd = 1;
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    w[e] = !is ? 0 : w[e] & (not_finite16x2<F16>(w[e] & 0xffffu) ? 0xffff0000u : 0xffffffffu) & (not_finite16x2<F16>(w[e] >> 16) ? 0xffffu : 0xffffffffu);
-                *reinterpret_cast<uint4 *>(mine + h * AT_TILE * 128 + (q + i) * 512) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+        for (int h = 0; h < D / 64; ++h) {
+            uint4 &p = *reinterpret_cast<uint4 *>(mine + h * AT_TILE * 128 + q * 512);
+            if (!is) p = make_uint4(0, 0, 0, 0);
+            const uint4 v = p;
+            acc[0] = at_zero_fma<F16>(v.x, acc[0]), acc[1] = at_zero_fma<F16>(v.y, acc[1]);
+            acc[2] = at_zero_fma<F16>(v.z, acc[2]), acc[3] = at_zero_fma<F16>(v.w, acc[3]);
         }
+    }
+    if (__any_sync(0xffffffffu, not_finite16x2<F16>(acc[0]) || not_finite16x2<F16>(acc[1]) || not_finite16x2<F16>(acc[2]) || not_finite16x2<F16>(acc[3])))
+        at_clean_values<F16, D>(mine, from, row, odd);
 }
 
 template <bool F16, int D>
 __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_kernel(AttendArgs a, const __grid_constant__ CUtensorMap k_map,
                                                                                             const __grid_constant__ CUtensorMap v_map, int box,
-                                                                                            int min_units, long long limit) {
+                                                                                            int min_units, int align, long long limit) {
     constexpr uint32_t IDESC = (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(AT_ROWS >> 4) << 24);
     constexpr uint32_t IDESC_QK = IDESC | ((uint32_t)(AT_TILE >> 3) << 17), IDESC_PV = IDESC | (1u << 16) | ((uint32_t)(D >> 3) << 17);
     constexpr int HALF = AT_TILE * 128, Q_HALF = AT_ROWS * 128;  // bytes of 64 columns of an operand
@@ -748,19 +774,35 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
         dg_tmem_alloc(smem_u32(&sh.tmem), AT_COLS);
         dg_tmem_relinquish();
     }
-    const long long units = scan_units<AT_THREADS>(a, cum, [&](const AttendRequest &q) {
-        const int m_tiles = (int)(((long long)q.n * group + AT_ROWS - 1) / AT_ROWS);
-        long long tiles = 0;
-        if (a.mask) tiles = (long long)m_tiles * at_tiles(a, q, group, 0);
-        else for (int m = 0; m < m_tiles; ++m) tiles += at_tiles(a, q, group, m);
-        return tiles * a.cache.n_kv;
-    });
+    auto all_units = [&](long long pad) {
+        return scan_units<AT_THREADS>(a, cum, [&](const AttendRequest &q) {
+            const int m_tiles = (int)(((long long)q.n * group + AT_ROWS - 1) / AT_ROWS);
+            long long tiles = 0;
+            if (a.mask) tiles = m_tiles * AttendWalk<D>::at_padded(at_tiles(a, q, group, 0), pad);
+            else for (int m = 0; m < m_tiles; ++m) tiles += AttendWalk<D>::at_padded(at_tiles(a, q, group, m), pad);
+            return tiles * a.cache.n_kv;
+        });
+    };
+    long long units = all_units(1), per = max((units + gridDim.x - 1) / gridDim.x, (long long)min_units), pad = 1;
+    // Segments of the same keys (a request's rows beyond 128) should run in step, so that the keys come from memory once.  They do if
+    // every segment begins at a CTA of its own; that takes longer parts, so it is done where the keys do not stay in the L2 anyway.
+    if (align && units * (AT_TILE * D * 4LL) > (long long)align << 20) {
+        for (long long p = per; p <= per + per / 4; p += max(per / 32, 1LL)) {
+            __syncthreads();
+            if (all_units(p) <= p * gridDim.x) {
+                pad = per = p;
+                break;
+            }
+        }
+        __syncthreads();
+        if (pad == 1) units = all_units(1);
+        else units = cum[a.R];
+    }
     dg_fence_before();
     __syncthreads();
     dg_fence_after();
     const uint32_t tmem = sh.tmem, tmem_o = tmem + 2 * AT_TILE;
-    const long long per = max((units + gridDim.x - 1) / gridDim.x, (long long)min_units);
-    AttendWalk<D> walk{a, cum, blockIdx.x * per, min((blockIdx.x + 1) * per, units), group};
+    AttendWalk<D> walk{a, cum, blockIdx.x * per, min((blockIdx.x + 1) * per, units), group, pad};
     AttendSegment g;
     bool ok = true;
     int n = 0;  // tiles so far: tile n has place n % 2 of everything that is held twice, in phase n / 2 % 2
@@ -865,17 +907,20 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
         }
     } else if (warp == 6) {
         // ---- Q of segment after segment, as soon as the last scores of the one before are there ----
-        const int ck = lane >> 3, cp = lane & 7;
+        const int ck = lane >> 3, cp = lane & 7, step_j = 4 / group, step_h = 4 % group;
         for (int seg = 0; ok && walk.next(g); ++seg) {
             if (seg && !(ok = mbar_wait_bounded_warp(q_free, (seg - 1) & 1, limit))) break;
             const int rows = (int)min((long long)AT_ROWS, (long long)g.rq.n * group - (long long)g.m * AT_ROWS);
             const uint32_t to = smem_u32(qs) + ck * 128;
             const uint16_t *base = a.q + (long long)g.rq.q0 * a.q_row + (long long)g.hk * group * a.q_head + 8 * cp;
-            int j = (g.m * AT_ROWS + ck) / group, h = (g.m * AT_ROWS + ck) % group;  // of row 4 q + ck
-            for (int q = 0; q < AT_ROWS / 4; ++q) {
-                copies16<D / 64, Q_HALF, 128>(to + q * 512 + (cp ^ ((4 * q + ck) & 7)) * 16, base + (4 * q + ck < rows ? j * a.q_row + h * a.q_head : 0),
-                                              4 * q + ck < rows ? 16 : 0);
-                for (h += 4; h >= group; h -= group) ++j;
+            int j = (g.m * AT_ROWS + ck) / group, h = (g.m * AT_ROWS + ck) % group;  // token and head of row 4 q + ck
+            // (rows that there are not are worked on like the others, and not stored)
+#pragma unroll 4
+            for (int q = 0; q < (rows + 3) / 4; ++q) {
+                if (4 * q + ck < rows) copies16<D / 64, Q_HALF, 128>(to + q * 512 + (cp ^ ((4 * q + ck) & 7)) * 16, base + (j * a.q_row + h * a.q_head), 16);
+                h += step_h;
+                j += step_j;
+                if (h >= group) h -= group, ++j;
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
             if (a.scale_log2 < 0.f) {  // a negative scale turns Q's signs
@@ -1139,6 +1184,7 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
             const int smem = (view.head_dim == 64 ? AT_SMEM<64> : AT_SMEM<128>) + (R + 1) * 8;
             if ((rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "tree_attention shared memory"))) return rc;
             const int grid = min(device_sm_count() * AT_PER_SM, AT_MAX_CTAS);
+            const int align = (long long)T * (n_heads / view.n_kv) > (long long)AT_ROWS * R ? 100 : 0;  // MB of keys
             // boxes of slots that never straddle a page or a tile
             int box = AT_TILE;
             while (box >= 8 && view.page_size % box) box >>= 1;
@@ -1155,7 +1201,7 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
                                                {64u, 1u, (uint32_t)box, 1u}, CU_TENSOR_MAP_SWIZZLE_128B)))
                     return rc;
             }
-            if ((rc = check_cuda(launch_pdl(kernel, dim3(grid), dim3(AT_THREADS), smem, as_stream(stream), a, maps[0], maps[1], box, 1, wait_limit_cycles()),
+            if ((rc = check_cuda(launch_pdl(kernel, dim3(grid), dim3(AT_THREADS), smem, as_stream(stream), a, maps[0], maps[1], box, 1, align, wait_limit_cycles()),
                                  "tree_attention launch")))
                 return rc;
             auto join = view.head_dim == 64 ? (f16 ? tree_attention_join_kernel<true, 64> : tree_attention_join_kernel<false, 64>)
