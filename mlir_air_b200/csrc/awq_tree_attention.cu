@@ -574,12 +574,19 @@ struct AttendJoin {
     int last, q0, n, hk, m;
 };
 constexpr int AT_JOINS = 4 * AR_MAX_CTAS;  // their place in the scratch, behind the other kernel's counters
+// A piece of a segment that one CTA works on: keys from tile0 on, `tiles` of its n_tiles.
+struct AttendSegment {
+    int r, q0, n, len, hk, m, tile0, tiles, n_tiles, c0, c1;  // c0, c1: the CTAs that have its first and last tile
+};
 struct AttendTilesShared {
     // mbarriers, of even and odd tiles: K, V there; QK^T, PV (of every fourth) done; P there.  Of a segment: Q there, Q done with, O done.  V that is
     // not ready for the product yet.
     uint64_t k_full[2], v_full[2], scored[2], added[4], weighed[2], q_full, q_free, summed, v_landed;
     uint32_t tmem;
     int odd[2], pad;
+    uint64_t found[4];                     // mbarriers: a segment's description is there
+    AttendSegment segments[4];             // (no tiles: the last one is over)
+    unsigned long long bits[2][AT_ROWS];   // of a segment's rows: their tokens' masks
     uint32_t valid[4][2];                  // of a tile: which of its keys there are
     long long places[2][AT_TILE];  // of a copying warp: the keys of its tile
 };
@@ -630,21 +637,16 @@ __device__ __noinline__ void at_see(const AttendArgs &a, int len, int key0, int 
         vis[c] &= d0 < 0 ? (uint32_t)(b << -d0) | ((1u << -d0) - 1) : (uint32_t)b;
     }
 }
-__device__ __forceinline__ void at_mask(const AttendArgs &a, const AttendRequest &rq, int key0, int j, unsigned long long bits, uint32_t (&vis)[2],
+__device__ __forceinline__ void at_mask(const AttendArgs &a, int len, int key0, int j, unsigned long long bits, uint32_t (&vis)[2],
                                         uint32_t (&v)[2][32]) {
-    at_see(a, rq.len, key0, j, bits, vis);
+    at_see(a, len, key0, j, bits, vis);
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[c][e] = vis[c] >> e & 1 ? v[c][e] : 0xff800000u;
 }
 
-// A CTA's walk over its part of the units, segment by segment; every warp role walks for itself.
-struct AttendSegment {
-    AttendRequest rq;
-    int r, hk, m, tile0, tiles, n_tiles;
-    long long start;  // its first unit
-};
+// A CTA's walk over its part of the units, segment by segment.
 __device__ __forceinline__ long long at_div(long long x, long long y) { return (x | y) >> 32 ? x / y : (long long)((uint32_t)x / (uint32_t)y); }
 template <int D>
 struct AttendWalk {
@@ -653,25 +655,27 @@ struct AttendWalk {
     long long x, end;
     int group;
     long long pad;  // units of a segment come in multiples of this
-    __device__ __forceinline__ bool next(AttendSegment &s) {
+    __device__ __forceinline__ bool next(AttendSegment &s, long long per) {
         while (x < end) {
             s.r = request_of_unit(cum, a.R, x);
-            s.rq = attend_request(a, s.r);
+            const AttendRequest rq = attend_request(a, s.r);
+            s.q0 = rq.q0, s.n = rq.n, s.len = rq.len;
             const long long rem = x - cum[s.r], per_head = at_div(cum[s.r + 1] - cum[s.r], a.cache.n_kv);
             s.hk = (int)at_div(rem, per_head);
             long long left = rem - s.hk * per_head, units;
             s.m = 0;
             if (a.mask) {  // all segments of a request are as long
-                s.n_tiles = at_tiles(a, s.rq, group, 0);
+                s.n_tiles = at_tiles(a, rq, group, 0);
                 units = at_padded(s.n_tiles, pad);
                 s.m = (int)at_div(left, units);
                 left -= s.m * units;
             } else {
-                while (left >= (units = at_padded(s.n_tiles = at_tiles(a, s.rq, group, s.m), pad))) left -= units, ++s.m;
+                while (left >= (units = at_padded(s.n_tiles = at_tiles(a, rq, group, s.m), pad))) left -= units, ++s.m;
             }
             s.tile0 = (int)left;
-            s.start = x - left;
             s.tiles = (int)min(end - x, (long long)s.n_tiles - left);
+            s.c0 = (int)at_div(x - left, per);
+            s.c1 = (int)at_div(x - left + s.n_tiles - 1, per);
             x += min(end - x, units - left);
             if (s.tiles > 0) return true;
         }
@@ -765,6 +769,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
         mbar_init(q_free, 1);
         mbar_init(summed, 1);
         mbar_init(smem_u32(&sh.v_landed), 1);
+        for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&sh.found[i]), 1);
         mbar_fence_init();
         sh.odd[0] = sh.odd[1] = 0;
     }
@@ -787,28 +792,28 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
     // Segments of the same keys (a request's rows beyond 128) should run in step, so that the keys come from memory once.  They do if
     // every segment begins at a CTA of its own; that takes longer parts, so it is done where the keys do not stay in the L2 anyway.
     if (align && units * (AT_TILE * D * 4LL) > (long long)align << 20) {
-        for (long long p = per; p <= per + per / 4; p += max(per / 32, 1LL)) {
-            __syncthreads();
-            if (all_units(p) <= p * gridDim.x) {
-                pad = per = p;
-                break;
-            }
-        }
-        __syncthreads();
-        if (pad == 1) units = all_units(1);
-        else units = cum[a.R];
+        if (all_units(per) <= (per + per / 4) * gridDim.x)
+            for (long long p = per; pad == 1 && p <= per + per / 4; p += max(per / 32, 1LL))
+                if (all_units(p) <= p * gridDim.x) pad = p;
+        if (pad > 1) per = pad;
+        units = pad > 1 ? cum[a.R] : all_units(1);
     }
     dg_fence_before();
     __syncthreads();
     dg_fence_after();
     const uint32_t tmem = sh.tmem, tmem_o = tmem + 2 * AT_TILE;
-    AttendWalk<D> walk{a, cum, blockIdx.x * per, min((blockIdx.x + 1) * per, units), group, pad};
     AttendSegment g;
     bool ok = true;
     int n = 0;  // tiles so far: tile n has place n % 2 of everything that is held twice, in phase n / 2 % 2
     auto bar_of = [](uint32_t bar, int t) { return bar + 8 * (t & 1); };
     // keys that all rows of a segment see, from the front on
-    auto seen_by_all = [&](const AttendSegment &s) { return s.rq.len + (a.mask ? 0 : s.m * AT_ROWS / group + 1); };
+    auto seen_by_all = [&](const AttendSegment &s) { return s.len + (a.mask ? 0 : s.m * AT_ROWS / group + 1); };
+    // the next segment, as warp 6 has found it
+    auto next = [&](int seg) {
+        ok = mbar_wait_bounded_warp(smem_u32(&sh.found[seg & 3]), seg >> 2 & 1, limit);
+        if (ok) g = sh.segments[seg & 3];
+        return ok && g.tiles > 0;
+    };
     auto phase_of = [](int t) { return (uint32_t)(t >> 1 & 1); };
     auto added_of = [&](int t) { return added + 8 * (t & 3); };
     auto added_phase = [](int t) { return (uint32_t)(t >> 2 & 1); };
@@ -821,8 +826,8 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
         const uint32_t landed = smem_u32(&sh.v_landed);
         int cleaned = 0;  // tiles that went through `landed`
         if (lane == 0) tma_prefetch_desc(map);
-        for (int seg = 0; ok && walk.next(g); ++seg) {
-            const int total = g.rq.len + g.rq.n;
+        for (int seg = 0; ok && next(seg); ++seg) {
+            const int total = g.len + g.n;
             const int32_t *table = a.table + g.r * a.table_stride;
             auto page_of = [&](int i) {
                 const int key = (g.tile0 + i) * AT_TILE + lane * box;
@@ -871,8 +876,8 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
         const bool is_v = warp == 5;
         const int ck = lane >> 3, cp = lane & 7;
         long long *places = sh.places[is_v];
-        for (int seg = 0; ok && walk.next(g); ++seg) {
-            const int total = g.rq.len + g.rq.n;
+        for (int seg = 0; ok && next(seg); ++seg) {
+            const int total = g.len + g.n;
             const int32_t *table = a.table + g.r * a.table_stride;
             const uint16_t *base = (is_v ? a.cache.v + g.hk * a.cache.v_head : a.cache.k + g.hk * a.cache.k_head) + 8 * cp;
             const long long s_page = is_v ? a.cache.v_page : a.cache.k_page, s_slot = is_v ? a.cache.v_slot : a.cache.k_slot;
@@ -906,13 +911,26 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
             }
         }
     } else if (warp == 6) {
-        // ---- Q of segment after segment, as soon as the last scores of the one before are there ----
+        // ---- what comes next: the segment for everyone, then its Q, as soon as the last scores of the one before are there ----
         const int ck = lane >> 3, cp = lane & 7, step_j = 4 / group, step_h = 4 % group;
-        for (int seg = 0; ok && walk.next(g); ++seg) {
+        AttendWalk<D> walk{a, cum, blockIdx.x * per, min((blockIdx.x + 1) * per, units), group, pad};
+        for (int seg = 0; ok; ++seg) {
+            const bool more = walk.next(g, per);
+            if (!more) g.tiles = 0;
+            // (its place was that of segment seg - 4; the scores of seg - 2 are there, so that everybody is behind seg - 3)
+            if (lane == 0) {
+                sh.segments[seg & 3] = g;
+                mbar_arrive(smem_u32(&sh.found[seg & 3]));
+            }
+            if (!more) break;
+            const int rows = (int)min((long long)AT_ROWS, (long long)g.n * group - (long long)g.m * AT_ROWS);
+            unsigned long long bits[AT_ROWS / 32];
+#pragma unroll
+            for (int k = 0; k < AT_ROWS / 32; ++k)
+                bits[k] = a.mask && 32 * k + lane < rows ? (unsigned long long)a.mask[g.q0 + (g.m * AT_ROWS + 32 * k + lane) / group] : 0;
             if (seg && !(ok = mbar_wait_bounded_warp(q_free, (seg - 1) & 1, limit))) break;
-            const int rows = (int)min((long long)AT_ROWS, (long long)g.rq.n * group - (long long)g.m * AT_ROWS);
             const uint32_t to = smem_u32(qs) + ck * 128;
-            const uint16_t *base = a.q + (long long)g.rq.q0 * a.q_row + (long long)g.hk * group * a.q_head + 8 * cp;
+            const uint16_t *base = a.q + (long long)g.q0 * a.q_row + (long long)g.hk * group * a.q_head + 8 * cp;
             int j = (g.m * AT_ROWS + ck) / group, h = (g.m * AT_ROWS + ck) % group;  // token and head of row 4 q + ck
             // (rows that there are not are worked on like the others, and not stored)
 #pragma unroll 4
@@ -922,6 +940,8 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
                 j += step_j;
                 if (h >= group) h -= group, ++j;
             }
+#pragma unroll
+            for (int k = 0; k < AT_ROWS / 32; ++k) sh.bits[seg & 1][32 * k + lane] = bits[k];
             asm volatile("cp.async.wait_all;" ::: "memory");
             if (a.scale_log2 < 0.f) {  // a negative scale turns Q's signs
                 __syncwarp();
@@ -954,7 +974,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
             }
             __syncwarp();
         };
-        for (int seg = 0; ok && walk.next(g); ++seg) {
+        for (int seg = 0; ok && next(seg); ++seg) {
             if (!(ok = mbar_wait_bounded_warp(q_full, seg & 1, limit))) break;
             score(n, g.tiles == 1);
             for (int i = 0; ok && i < g.tiles; ++i, ++n) {
@@ -980,16 +1000,17 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
         float *parts = reinterpret_cast<float *>(a.scratch + AT_JOINS + sizeof(AttendJoin) * AT_MAX_CTAS);
         AttendJoin *joins = reinterpret_cast<AttendJoin *>(a.scratch + AT_JOINS);
         bool joined = false;
-        for (int seg = 0; ok && walk.next(g); ++seg) {
-            const int rows = (int)min((long long)AT_ROWS, (long long)g.rq.n * group - (long long)g.m * AT_ROWS);
+        for (int seg = 0; ok && next(seg); ++seg) {
+            const int rows = (int)min((long long)AT_ROWS, (long long)g.n * group - (long long)g.m * AT_ROWS);
             const bool mine = tid < rows, busy = warp * 32 < rows;
             const int row = g.m * AT_ROWS + tid, j = row / group, head = g.hk * group + row % group;
-            const unsigned long long bits = a.mask && mine ? (unsigned long long)a.mask[g.rq.q0 + j] : 0;
+            unsigned long long bits = 0;
             const int all_see = seen_by_all(g);
             float top = -INFINITY, sum = 0.f;
             for (int i = 0; i < g.tiles; ++i, ++n) {
                 if (!(ok = mbar_wait_bounded_warp(bar_of(scored, n), phase_of(n), limit))) break;
                 dg_fence_after();
+                if (i == 0) bits = sh.bits[seg & 1][tid];  // (there with Q.  Q of the next but one segment may be there too by now: no wait for q_full)
                 if (busy) {
                     const uint32_t s_cols = tmem + lanes + (n & 1) * AT_TILE;
                     const int key0 = (g.tile0 + i) * AT_TILE;
@@ -998,7 +1019,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
                     dg_tmem_ld_32x32b_x32(s_cols + 32, v[1]);
                     uint32_t vis[2] = {sh.valid[n & 3][0], sh.valid[n & 3][1]};
                     dg_tmem_ld_wait();
-                    if (key0 + AT_TILE > all_see || (vis[0] & vis[1]) != 0xffffffffu) at_mask(a, g.rq, key0, j, bits, vis, v);
+                    if (key0 + AT_TILE > all_see || (vis[0] & vis[1]) != 0xffffffffu) at_mask(a, g.len, key0, j, bits, vis, v);
                     float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
                     for (int e = 0; e < 32; ++e) m0 = fmaxf(m0, __uint_as_float(v[0][e])), m1 = fmaxf(m1, __uint_as_float(v[1][e]));
@@ -1047,11 +1068,11 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
             if (!(ok = mbar_wait_bounded_warp(summed, seg & 1, limit))) break;
             dg_fence_after();
             // ---- the segment's sums: out, or to the CTA that joins them ----
-            const int c0 = (int)(g.start / per), c1 = (int)((g.start + g.n_tiles - 1) / per);
+            const int c0 = g.c0, c1 = g.c1;
             const bool whole = c0 == c1;
             const bool odd = *reinterpret_cast<volatile int *>(&sh.odd[seg & 1]) != 0;
             float *part = parts + (long long)(2 * blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0)) * PART;  // [D + 2][128]
-            uint16_t *out = a.out + (long long)(g.rq.q0 + j) * a.o_row + (long long)head * a.o_head;
+            uint16_t *out = a.out + (long long)(g.q0 + j) * a.o_row + (long long)head * a.o_head;
             auto store32 = [&](int c, const float (&o)[32], float total) {
                 const float inv = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
@@ -1070,10 +1091,10 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(v[e]);
                     if (odd && mine) {
-                        const int first = max(g.tile0 * AT_TILE - g.rq.len, 0), last = min((g.tile0 + g.tiles) * AT_TILE - g.rq.len, g.rq.n);
+                        const int first = max(g.tile0 * AT_TILE - g.len, 0), last = min((g.tile0 + g.tiles) * AT_TILE - g.len, g.n);
                         for (int d = first; d < last; ++d) {
                             if (!(a.mask ? d < 64 && (bits >> d & 1) : d <= j)) continue;
-                            const int key = g.rq.len + d, page = a.table[g.r * a.table_stride + page_index(a, key)];
+                            const int key = g.len + d, page = a.table[g.r * a.table_stride + page_index(a, key)];
                             if ((unsigned)page >= (unsigned)a.cache.n_pages) continue;
                             const uint16_t *src = a.cache.v + page * a.cache.v_page + (key - page_index(a, key) * page_size) * a.cache.v_slot + g.hk * a.cache.v_head + 32 * c;
 #pragma unroll
@@ -1095,7 +1116,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
             if (tid == 0) {
                 sh.odd[seg & 1] = 0;
                 // what begins here and goes on is this CTA's last segment
-                if (!whole && (int)blockIdx.x == c0) joins[blockIdx.x] = AttendJoin{c1, g.rq.q0, g.rq.n, g.hk, g.m}, joined = true;
+                if (!whole && (int)blockIdx.x == c0) joins[blockIdx.x] = AttendJoin{c1, g.q0, g.n, g.hk, g.m}, joined = true;
             }
         }
         if (tid == 0 && !joined) joins[blockIdx.x].last = -1;

@@ -36,7 +36,8 @@ def run(segments, seed, rescale=0.5, tma=False):
     def loader(is_v):
         """One warp for K, one for V; it waits for its own copies."""
         n = 0
-        for tiles in segments:
+        for seg, tiles in enumerate(segments):
+            yield from describe(seg)
             for _ in range(tiles):
                 if n > 1:
                     yield (added[(n - 2) % 4], (n - 2) >> 2 & 1) if is_v else (scored[n % 2], phase(n - 2))
@@ -51,8 +52,20 @@ def run(segments, seed, rescale=0.5, tma=False):
                 (v_full if is_v else k_full)[n % 2].arrive()
                 n += 1
 
+    found, ring = [Bar(1) for _ in range(4)], [None] * 4  # the segments' descriptions, and the roles that have read each
+
+    def describe(seg):
+        """A role's wait for a segment's description."""
+        yield found[seg % 4], seg >> 2 & 1
+        assert ring[seg % 4][0] == seg, "a description overwritten before a role had it"
+        ring[seg % 4][1] += 1
+
     def q_loader():
         for seg in range(len(segments)):
+            assert ring[seg % 4] is None or ring[seg % 4][1] == 4
+            ring[seg % 4] = [seg, 0]
+            found[seg % 4].arrive()
+            yield None
             if seg:
                 yield q_free, (seg - 1) % 2
             assert state["q"] is None or state["q"][1] == "read"
@@ -64,7 +77,8 @@ def run(segments, seed, rescale=0.5, tma=False):
     def tma_loader(is_v, landing):
         """One warp for K, one for V; the bytes arrive by themselves, later, while it goes on.  Some tiles of V are put right first."""
         n = 0
-        for tiles in segments:
+        for seg, tiles in enumerate(segments):
+            yield from describe(seg)
             for _ in range(tiles):
                 if n > 1:
                     yield (added[(n - 2) % 4], (n - 2) >> 2 & 1) if is_v else (scored[n % 2], phase(n - 2))
@@ -83,13 +97,14 @@ def run(segments, seed, rescale=0.5, tma=False):
                 n += 1
 
     def memory(landing):
-        left = 200 * total
-        while state["done"] < 2 * total and left:
+        while state["done"] < 2 * total:
             if landing:
                 place, n, bar = landing.pop(rng.randrange(len(landing)))
                 place[n % 2] = (n, "there")
                 bar[n % 2].arrive()
-            yield None
+                yield None
+            else:
+                yield False
 
     def score(n, last):
         yield k_full[n % 2], phase(n)
@@ -99,6 +114,7 @@ def run(segments, seed, rescale=0.5, tma=False):
     def products():
         n = 0
         for seg, tiles in enumerate(segments):
+            yield from describe(seg)
             yield q_full, seg % 2
             yield from score(n, tiles == 1)
             for i in range(tiles):
@@ -114,7 +130,7 @@ def run(segments, seed, rescale=0.5, tma=False):
         """Takes the products in the order they were issued; a commit's arrival comes a while after its product."""
         while state["done"] < 2 * total:
             if not queue:
-                yield None
+                yield False
                 continue
             op = queue.pop(0)
             n = op[1]
@@ -142,6 +158,7 @@ def run(segments, seed, rescale=0.5, tma=False):
     def softmax():
         n = 0
         for seg, tiles in enumerate(segments):
+            yield from describe(seg)
             for i in range(tiles):
                 yield scored[n % 2], phase(n)
                 assert S[n % 2] == (n, "scores") and valid[n % 4] == (n, "there")
@@ -175,9 +192,11 @@ def run(segments, seed, rescale=0.5, tma=False):
             idle += 1
             assert idle < 20000, f"no progress: {sorted(roles)} at {state}"
             continue
-        idle = 0
         try:
-            roles[name][1] = next(role)
+            step = next(role)
+            idle = idle + 1 if step is False else 0
+            assert idle < 20000, f"no progress: {sorted(roles)} at {state}"
+            roles[name][1] = step or None
         except StopIteration:
             del roles[name]
     assert state["done"] == 2 * total and not queue
