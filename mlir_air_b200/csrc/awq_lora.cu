@@ -71,10 +71,11 @@ __device__ __forceinline__ void lora_down(float (&acc)[MT][NB][4], const uint16_
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                mma_bf16_16816(acc[m][b], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, av[b].x, av[b].y);
-                mma_bf16_16816(acc[m][b], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, av[b].z, av[b].w);
-            }
+            for (int b = 0; b < NB; ++b) mma_bf16_16816(acc[m][b], xv[m][0].x, xv[m][1].x, xv[m][0].y, xv[m][1].y, av[b].x, av[b].y);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int b = 0; b < NB; ++b) mma_bf16_16816(acc[m][b], xv[m][0].z, xv[m][1].z, xv[m][0].w, xv[m][1].w, av[b].z, av[b].w);
     }
 }
 
@@ -247,10 +248,9 @@ __global__ void __cluster_dims__(LF_CLUSTER, 1, 1) __launch_bounds__(LF_WARPS * 
                 for (int p = 0; p < 2; ++p) {
                     const uint4 u = frag[c][p][0][lane], v = frag[c][p][1][lane];
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        mma_bf16_16816(acc[b], u.x, v.x, u.y, v.y, bv[b][c].x, bv[b][c].y);
-                        mma_bf16_16816(acc[b], u.z, v.z, u.w, v.w, bv[b][c].z, bv[b][c].w);
-                    }
+                    for (int b = 0; b < 4; ++b) mma_bf16_16816(acc[b], u.x, v.x, u.y, v.y, bv[b][c].x, bv[b][c].y);
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) mma_bf16_16816(acc[b], u.z, v.z, u.w, v.w, bv[b][c].z, bv[b][c].w);
                 }
         }
         const int col = 32 * cb + 8 * t4;
@@ -384,10 +384,9 @@ __global__ void __launch_bounds__(LD_WARPS * 32, 2) lora_down_kernel(LoraArgs a)
                 if (r0 + 8 * NB * half >= rank) break;  // (no ranks for this warp)
                 const uint4 x0 = lds128(at + 16 * m * 256), x1 = lds128(at + (16 * m + 8) * 256);
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    mma_bf16_16816(acc[m][b], x0.x, x1.x, x0.y, x1.y, av[b].x, av[b].y);
-                    mma_bf16_16816(acc[m][b], x0.z, x1.z, x0.w, x1.w, av[b].z, av[b].w);
-                }
+                for (int b = 0; b < NB; ++b) mma_bf16_16816(acc[m][b], x0.x, x1.x, x0.y, x1.y, av[b].x, av[b].y);
+#pragma unroll
+                for (int b = 0; b < NB; ++b) mma_bf16_16816(acc[m][b], x0.z, x1.z, x0.w, x1.w, av[b].z, av[b].w);
             }
         }
         __syncthreads();  // (the copies still pending are empty groups)
@@ -502,10 +501,9 @@ __global__ void __launch_bounds__(LU_WARPS * 32, RC == 4 ? 2 : F32 ? 3 : 4) lora
                 for (int p = 0; p < 2; ++p) {
                     const uint4 u = lu_frag[((m * RC + c) * 2 + p) * 64 + lane], v = lu_frag[((m * RC + c) * 2 + p) * 64 + 32 + lane];
 #pragma unroll
-                    for (int b = 0; b < 4; ++b) {
-                        mma_bf16_16816(acc[b], u.x, v.x, u.y, v.y, bv[b][c].x, bv[b][c].y);
-                        mma_bf16_16816(acc[b], u.z, v.z, u.w, v.w, bv[b][c].z, bv[b][c].w);
-                    }
+                    for (int b = 0; b < 4; ++b) mma_bf16_16816(acc[b], u.x, v.x, u.y, v.y, bv[b][c].x, bv[b][c].y);
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) mma_bf16_16816(acc[b], u.z, v.z, u.w, v.w, bv[b][c].z, bv[b][c].w);
                 }
             }
 #pragma unroll
@@ -553,9 +551,10 @@ static int launch_lora_down(const LoraArgs &a, int tiles, cudaStream_t stream) {
 }
 template <int RC>
 static int launch_lora_up(const LoraArgs &a, int tiles, cudaStream_t stream) {
-    // as many columns a CTA as leave four CTAs to each of the four places on an SM
+    // as many columns a CTA as leave about two CTAs to each of the four places on an SM (nine prompts, K 4096, N 14336: 79 us;
+    // four 84, one 82)
     const int blocks = (a.N + 32 * LU_WARPS - 1) / (32 * LU_WARPS), busy = (a.T + LM_ROWS - 1) / LM_ROWS;
-    const int loops = max(1, min(16, (int)((long long)blocks * busy / (16 * device_sm_count()))));
+    const int loops = max(1, min(16, (int)((long long)blocks * busy / (7 * device_sm_count()))));
     const dim3 grid((blocks + loops - 1) / loops, tiles), block(LU_WARPS * 32);
     const int smem = LM_MT * RC * 128 * 16;
     auto kernel = a.base_f32 ? lora_up_kernel<RC, true> : lora_up_kernel<RC, false>;

@@ -215,6 +215,8 @@ __device__ __forceinline__ long long scan_units(const AttendArgs &a, long long *
     __syncthreads();
     return total;
 }
+// (64-bit divisions cost some hundred cycles; units rarely need them)
+__device__ __forceinline__ long long at_div(long long x, long long y) { return (x | y) >> 32 ? x / y : (long long)((uint32_t)x / (uint32_t)y); }
 __device__ __forceinline__ int request_of_unit(const long long *cum, int n, long long x) {
     int lo = 0, hi = n;
     while (hi - lo > 1) {
@@ -258,7 +260,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
     const long long units = scan_units<THREADS>(a, cum, [&](const AttendRequest &q) {
         return (((long long)q.n * group + AR_ROWS - 1) / AR_ROWS) * a.cache.n_kv * ((q.len + q.n + AR_TILE - 1) / AR_TILE);
     });
-    const long long per = max((units + gridDim.x - 1) / gridDim.x, (long long)min_units);
+    const long long per = max(at_div(units + gridDim.x - 1, gridDim.x), (long long)min_units);
     long long x = blockIdx.x * per;
     const long long end = min(x + per, units);
     const int page_size = a.cache.page_size;
@@ -271,7 +273,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
         const AttendRequest rq = attend_request(a, r);
         const int total = rq.len + rq.n, n_tiles = (total + AR_TILE - 1) / AR_TILE, m_tiles = (rq.n * group + AR_ROWS - 1) / AR_ROWS;
         const long long rem = x - cum[r];
-        const int seg = (int)(rem / n_tiles), tile0 = (int)(rem % n_tiles), hk = seg / m_tiles, row0 = (seg % m_tiles) * AR_ROWS;
+        const int seg = (int)at_div(rem, n_tiles), tile0 = (int)(rem - (long long)seg * n_tiles), hk = seg / m_tiles, row0 = (seg % m_tiles) * AR_ROWS;
         const long long seg_start = x - tile0, seg_end = seg_start + n_tiles;
         const int tiles = (int)(min(end, seg_end) - x);
         const int32_t *table = a.table + r * a.table_stride;
@@ -492,7 +494,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
                 }
         }
         __syncthreads();
-        const int c0 = (int)(seg_start / per), c1 = (int)((seg_end - 1) / per), rows = min(AR_ROWS, rq.n * group - row0);
+        const int c0 = (int)at_div(seg_start, per), c1 = (int)at_div(seg_end - 1, per), rows = min(AR_ROWS, rq.n * group - row0);
         const bool whole = c0 == c1;
         float *part = parts + (long long)(2 * blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0)) * PART;
         auto store = [&](int row, int d, const float (&o)[4], float total_w) {
@@ -647,7 +649,6 @@ __device__ __forceinline__ void at_mask(const AttendArgs &a, int len, int key0, 
 }
 
 // A CTA's walk over its part of the units, segment by segment.
-__device__ __forceinline__ long long at_div(long long x, long long y) { return (x | y) >> 32 ? x / y : (long long)((uint32_t)x / (uint32_t)y); }
 template <int D>
 struct AttendWalk {
     const AttendArgs &a;
