@@ -31,7 +31,6 @@ struct LoraArgs {
     uint16_t *out;
     long long x_row;
     int base_f32, T, K, N, n, rank_max;
-    int splits;  // clusters that share a tile's columns (few rows)
     RequestHeader *header;
     int32_t *order;   // [T] rows by adapter
     int4 *tiles;      // adapter, first of `order`, rows, rank
@@ -139,132 +138,140 @@ __device__ __forceinline__ void lora_store(const LoraArgs &a, long long at, cons
 // Up to LORA_FEW rows: one launch.  A cluster of eight CTAs takes a tile of 16 rows: each an eighth of K, its warps a share of
 // that; the partial sums meet in distributed shared memory, and each CTA goes on with its share of the columns of B, whose
 // first pieces are on their way before the sums meet.  Every CTA puts the rows in order for itself (a few hundred comparisons a
-// thread), which is cheaper than a launch in front.  Where the tiles are few, several clusters share a tile's columns and each
-// forms x A^T for itself.
+// thread), which is cheaper than a launch in front.  How many tiles there are only the device knows: as many clusters as run at
+// once go through them, and where the tiles are few, several share a tile's columns and each forms x A^T for itself.
 // =====================================================================================
 constexpr int LORA_FEW = 128, LF_WARPS = 8, LF_CLUSTER = 8;
 
 template <int RC>  // rank_max up to 32 RC
-__global__ void __cluster_dims__(LF_CLUSTER, 1, 1) __launch_bounds__(LF_WARPS * 32) lora_few_kernel(LoraArgs a) {
+__global__ void __cluster_dims__(LF_CLUSTER, 1, 1) __launch_bounds__(LF_WARPS * 32, RC == 4 ? 1 : 2) lora_few_kernel(LoraArgs a) {
     constexpr int NB = 4 * RC, RP = 32 * RC, THREADS = LF_WARPS * 32;
     extern __shared__ __align__(16) float lf_smem[];
     float(*red)[16][RP + 4] = reinterpret_cast<float(*)[16][RP + 4]>(lf_smem);  // [WARPS / 2]
     __shared__ __align__(16) float part[16][RP + 4];
     __shared__ uint4 frag[RC][2][2][32];  // chunk, hi / lo, rows g / g + 8, lane
-    __shared__ int key[LORA_FEW], start[LORA_FEW], rows[16], s_tile[2];
+    __shared__ int key[LORA_FEW], start[LORA_FEW], rows[16], s_adapter;
     const cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-    const int rank_in = blockIdx.x % LF_CLUSTER, tile = blockIdx.x / LF_CLUSTER / a.splits, split = blockIdx.x / LF_CLUSTER % a.splits;
+    const int rank_in = blockIdx.x % LF_CLUSTER, n_clusters = gridDim.x / LF_CLUSTER;
     pdl_wait();
     pdl_launch_dependents();
-    // ---- the tile: the rows of one adapter, 16 at a time, adapters in order ----
+    // ---- the tiles: the rows of one adapter, 16 at a time, adapters in order ----
     if (tid < a.T) key[tid] = lora_adapter(a, tid, blockIdx.x == 0);
-    if (tid < 16) rows[tid] = -1;
-    if (tid == 0) s_tile[0] = -1;
     __syncthreads();
-    int mine = -1, pos = 0;
+    int mine = -1, pos = 0, of = -1;  // of row tid: its adapter, its place among that one's rows, its tile
     if (tid < a.T) {
         mine = key[tid];
         for (int u = 0; u < tid; ++u) pos += key[u] == mine;
         start[tid] = pos % 16 == 0 ? mine : -1;
     }
-    __syncthreads();
+    const int tiles = __syncthreads_count(tid < a.T && pos % 16 == 0);
     if (tid < a.T) {
-        int before = pos / 16;  // tiles of smaller adapters, and this one's earlier ones
-        for (int u = 0; u < a.T; ++u) before += start[u] >= 0 && start[u] < mine;
-        if (before == tile) {
-            rows[pos % 16] = tid;
-            if (pos % 16 == 0) s_tile[0] = mine;
-        }
+        of = pos / 16;  // behind the tiles of smaller adapters
+        for (int u = 0; u < a.T; ++u) of += start[u] >= 0 && start[u] < mine;
     }
-    __syncthreads();
-    const int ad = s_tile[0];
-    if (ad < 0) return;  // (the whole cluster)
-    const int rank = lora_rank(a, ad), r_lo = rows[g], r_hi = rows[g + 8];
-    // ---- x A^T ----
-    if (rank > 0) {
-        const int chunks = (a.K + 31) / 32, c0 = chunks * rank_in / LF_CLUSTER, c1 = chunks * (rank_in + 1) / LF_CLUSTER;
-        const uint16_t *x[1][2] = {{r_lo >= 0 ? a.x + r_lo * a.x_row : nullptr, r_hi >= 0 ? a.x + r_hi * a.x_row : nullptr}};
-        float acc[1][NB][4] = {};
-        lora_down<1, NB>(acc, x, a.A + (long long)ad * a.rank_max * a.K, a.K, rank, 0, c0 + warp, c1, LF_WARPS, lane);
+    const int blocks = (a.N + 31) / 32;
+    // Columns a warp would have with one cluster per tile, counted in blocks of 32: shared while clusters would idle.
+    const int splits = max(1, min(n_clusters / tiles, blocks / (LF_CLUSTER * LF_WARPS)));
+    bool reading = false;  // whether other CTAs may still read this one's sums
+    for (int item = blockIdx.x / LF_CLUSTER; item < tiles * splits; item += n_clusters) {
+        const int tile = item / splits, split = item % splits;
+        __syncthreads();  // the last tile's readers are done
+        if (tid < 16) rows[tid] = -1;
+        __syncthreads();
+        if (of == tile) {
+            rows[pos % 16] = tid;
+            if (pos % 16 == 0) s_adapter = mine;
+        }
+        __syncthreads();
+        const int ad = s_adapter, rank = lora_rank(a, ad), r_lo = rows[g], r_hi = rows[g + 8];
+        // ---- x A^T ----
+        if (rank > 0) {
+            const int chunks = (a.K + 31) / 32, c0 = chunks * rank_in / LF_CLUSTER, c1 = chunks * (rank_in + 1) / LF_CLUSTER;
+            const uint16_t *x[1][2] = {{r_lo >= 0 ? a.x + r_lo * a.x_row : nullptr, r_hi >= 0 ? a.x + r_hi * a.x_row : nullptr}};
+            float acc[1][NB][4] = {};
+            lora_down<1, NB>(acc, x, a.A + (long long)ad * a.rank_max * a.K, a.K, rank, 0, c0 + warp, c1, LF_WARPS, lane);
 #pragma unroll
-        for (int half = 1; half >= 0; --half) {
-            if (warp / (LF_WARPS / 2) == half)
+            for (int half = 1; half >= 0; --half) {
+                if (warp / (LF_WARPS / 2) == half)
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
+                    for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float &d = red[warp % (LF_WARPS / 2)][g + 8 * (e >> 1)][8 * b + 2 * t4 + (e & 1)];
-                        d = half ? acc[0][b][e] : d + acc[0][b][e];
-                    }
+                        for (int e = 0; e < 4; ++e) {
+                            float &d = red[warp % (LF_WARPS / 2)][g + 8 * (e >> 1)][8 * b + 2 * t4 + (e & 1)];
+                            d = half ? acc[0][b][e] : d + acc[0][b][e];
+                        }
+                __syncthreads();
+            }
+            if (reading) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+            reading = true;
+            for (int i = tid; i < 16 * RP; i += THREADS) {
+                float s = 0.f;
+#pragma unroll
+                for (int w = 0; w < LF_WARPS / 2; ++w) s += red[w][i / RP][i % RP];
+                part[i / RP][i % RP] = s;
+            }
+        }
+        // ---- this warp's first columns, before the sums meet ----
+        const int stride = LF_CLUSTER * splits * LF_WARPS;
+        int cb = (split * LF_CLUSTER + rank_in) * LF_WARPS + warp;
+        uint4 bv[4][RC];
+        Base8 base[2];
+        auto fetch = [&]() {
+            const int n0 = 32 * cb, col = n0 + 8 * t4;
+            lora_load_b<RC>(bv, a, ad, cb < blocks ? rank : 0, n0, lane);
+            base[0] = lora_base(a, (long long)r_lo * a.N + col, r_lo >= 0 && cb < blocks && col < a.N);
+            base[1] = lora_base(a, (long long)r_hi * a.N + col, r_hi >= 0 && cb < blocks && col < a.N);
+        };
+        fetch();
+        if (rank > 0) {
+            cluster.sync();
+            const float scale = a.scales[ad];
+            for (int i = tid; i < 16 * RP / 2; i += THREADS) {
+                const int row = i / (RP / 2), r = 2 * (i % (RP / 2));
+                float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int c = 0; c < LF_CLUSTER; ++c) {
+                    const float2 v = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(&part[row][r], c));
+                    s.x += v.x, s.y += v.y;
+                }
+                s.x *= scale, s.y *= scale;
+                const uint32_t hi = pack16x2<false>(s.x, s.y), lo = pack16x2<false>(s.x - bf16x2_lo(hi), s.y - bf16x2_hi(hi));
+                // element r of the row: chunk, the lane's eight, the word in it
+                const int c = r / 32, l = (row % 8) * 4 + r % 32 / 8, w = r % 8 / 2;
+                reinterpret_cast<uint32_t *>(&frag[c][0][row / 8][l])[w] = hi;
+                reinterpret_cast<uint32_t *>(&frag[c][1][row / 8][l])[w] = lo;
+            }
+            asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // done with the other CTAs' sums
             __syncthreads();
         }
-        for (int i = tid; i < 16 * RP; i += THREADS) {
-            float s = 0.f;
+        while (cb < blocks) {
+            float acc[4][4] = {};
+            if (rank > 0) {
 #pragma unroll
-            for (int w = 0; w < LF_WARPS / 2; ++w) s += red[w][i / RP][i % RP];
-            part[i / RP][i % RP] = s;
-        }
-    }
-    // ---- this warp's first columns, before the sums meet ----
-    const int blocks = (a.N + 31) / 32, stride = LF_CLUSTER * a.splits * LF_WARPS;
-    int cb = (split * LF_CLUSTER + rank_in) * LF_WARPS + warp;
-    uint4 bv[4][RC];
-    Base8 base[2];
-    auto fetch = [&]() {
-        const int n0 = 32 * cb, col = n0 + 8 * t4;
-        lora_load_b<RC>(bv, a, ad, cb < blocks ? rank : 0, n0, lane);
-        base[0] = lora_base(a, (long long)r_lo * a.N + col, r_lo >= 0 && cb < blocks && col < a.N);
-        base[1] = lora_base(a, (long long)r_hi * a.N + col, r_hi >= 0 && cb < blocks && col < a.N);
-    };
-    fetch();
-    if (rank > 0) {
-        cluster.sync();
-        const float scale = a.scales[ad];
-        for (int i = tid; i < 16 * RP / 2; i += THREADS) {
-            const int row = i / (RP / 2), r = 2 * (i % (RP / 2));
-            float2 s = make_float2(0.f, 0.f);
+                for (int c = 0; c < RC; ++c)
 #pragma unroll
-            for (int c = 0; c < LF_CLUSTER; ++c) {
-                const float2 v = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(&part[row][r], c));
-                s.x += v.x, s.y += v.y;
+                    for (int p = 0; p < 2; ++p) {
+                        const uint4 u = frag[c][p][0][lane], v = frag[c][p][1][lane];
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) mma_bf16_16816(acc[b], u.x, v.x, u.y, v.y, bv[b][c].x, bv[b][c].y);
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) mma_bf16_16816(acc[b], u.z, v.z, u.w, v.w, bv[b][c].z, bv[b][c].w);
+                    }
             }
-            s.x *= scale, s.y *= scale;
-            const uint32_t hi = pack16x2<false>(s.x, s.y), lo = pack16x2<false>(s.x - bf16x2_lo(hi), s.y - bf16x2_hi(hi));
-            // element r of the row: chunk, the lane's eight, the word in it
-            const int c = r / 32, l = (row % 8) * 4 + r % 32 / 8, w = r % 8 / 2;
-            reinterpret_cast<uint32_t *>(&frag[c][0][row / 8][l])[w] = hi;
-            reinterpret_cast<uint32_t *>(&frag[c][1][row / 8][l])[w] = lo;
-        }
-        asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");  // done with the other CTAs' sums
-        __syncthreads();
-    }
-    while (cb < blocks) {
-        float acc[4][4] = {};
-        if (rank > 0) {
-#pragma unroll
-            for (int c = 0; c < RC; ++c)
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const uint4 u = frag[c][p][0][lane], v = frag[c][p][1][lane];
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) mma_bf16_16816(acc[b], u.x, v.x, u.y, v.y, bv[b][c].x, bv[b][c].y);
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) mma_bf16_16816(acc[b], u.z, v.z, u.w, v.w, bv[b][c].z, bv[b][c].w);
-                }
-        }
-        const int col = 32 * cb + 8 * t4;
-        const Base8 b0 = base[0], b1 = base[1];
-        cb += stride;
-        fetch();
-        if (col < a.N) {
-            const float u[8] = {acc[0][0], acc[0][1], acc[1][0], acc[1][1], acc[2][0], acc[2][1], acc[3][0], acc[3][1]};
-            const float v[8] = {acc[0][2], acc[0][3], acc[1][2], acc[1][3], acc[2][2], acc[2][3], acc[3][2], acc[3][3]};
-            if (r_lo >= 0) lora_store(a, (long long)r_lo * a.N + col, b0, u);
-            if (r_hi >= 0) lora_store(a, (long long)r_hi * a.N + col, b1, v);
+            const int col = 32 * cb + 8 * t4;
+            const Base8 b0 = base[0], b1 = base[1];
+            cb += stride;
+            fetch();
+            if (col < a.N) {
+                const float u[8] = {acc[0][0], acc[0][1], acc[1][0], acc[1][1], acc[2][0], acc[2][1], acc[3][0], acc[3][1]};
+                const float v[8] = {acc[0][2], acc[0][3], acc[1][2], acc[1][3], acc[2][2], acc[2][3], acc[3][2], acc[3][3]};
+                if (r_lo >= 0) lora_store(a, (long long)r_lo * a.N + col, b0, u);
+                if (r_hi >= 0) lora_store(a, (long long)r_hi * a.N + col, b1, v);
+            }
         }
     }
-    if (rank > 0) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (reading) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // =====================================================================================
@@ -564,10 +571,9 @@ static int launch_lora_up(const LoraArgs &a, int tiles, cudaStream_t stream) {
 static int launch_lora(LoraArgs a, cudaStream_t stream) {
     const int rc32 = (a.rank_max + 31) / 32;
     if (a.T <= LORA_FEW) {
-        // Columns a warp would have with one cluster per tile, counted in blocks of 32: share them while SMs would idle.
-        const int tiles = (a.T + 15) / 16, blocks = (a.N + 31) / 32;
-        a.splits = max(1, min(2 * device_sm_count() / (LF_CLUSTER * tiles), blocks / (LF_CLUSTER * LF_WARPS)));
-        const dim3 grid(LF_CLUSTER * a.splits * min(a.T, tiles + a.n + 1)), block(LF_WARPS * 32);
+        // as many clusters as find room at once (two CTAs an SM), or as there may be tiles and shares of their columns
+        const int shares = max(1, (a.N + 31) / 32 / (LF_CLUSTER * LF_WARPS)), tiles = min(a.T, (a.T + 15) / 16 + a.n + 1);
+        const dim3 grid(LF_CLUSTER * min(2 * device_sm_count() / LF_CLUSTER, shares * tiles)), block(LF_WARPS * 32);
         auto kernel = rc32 == 1 ? lora_few_kernel<1> : rc32 == 2 ? lora_few_kernel<2> : lora_few_kernel<4>;
         const int smem = LF_WARPS / 2 * 16 * ((rc32 == 3 ? 4 : rc32) * 32 + 4) * 4;
         int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "lora shared memory");
@@ -608,7 +614,7 @@ extern "C" int awq_b200_lora_bf16(const uint16_t *x, long long x_row_stride, con
     const RequestWorkspaceView w = request_workspace(workspace);
     LoraArgs a{};
     a.x = x, a.A = A, a.B = B, a.scales = scales, a.ranks = ranks, a.idx = idx, a.base = base, a.residual = residual, a.out = out;
-    a.x_row = x_row_stride, a.base_f32 = base_is_f32, a.T = T, a.K = K, a.N = N, a.n = n_adapters, a.rank_max = rank_max, a.splits = 1;
+    a.x_row = x_row_stride, a.base_f32 = base_is_f32, a.T = T, a.K = K, a.N = N, a.n = n_adapters, a.rank_max = rank_max;
     a.header = w.header;
     uint8_t *p = w.lora;
     a.n_tiles = reinterpret_cast<int32_t *>(p), p += 256;

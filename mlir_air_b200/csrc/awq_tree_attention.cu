@@ -42,7 +42,7 @@ __device__ __forceinline__ AttendRequest attend_request(const AttendArgs &a, int
     const int s = a.q_start[r], e = a.q_start[r + 1], len = a.lens[r];
     q.q0 = min(max(s, 0), a.T);
     q.n = min(max(e, q.q0), a.T) - q.q0;
-    const long long capacity = min((long long)a.table_width * a.cache.page_size, 0x7fffffffLL);
+    const long long capacity = min((long long)a.table_width * a.cache.page_size, 0x7fff0000LL);  // (keys of a last tile still fit 32 bits)
     q.len = (int)min((long long)max(len, 0), max(capacity - q.n, 0LL));
     q.bad = q.q0 != s || q.q0 + q.n != e || q.len != len || (a.mask && q.n > REQ_MAX_TREE) || q.n > capacity;
     if (q.n > capacity) q.n = 0;
@@ -188,7 +188,7 @@ __device__ __forceinline__ long long scan_units(const AttendArgs &a, long long *
     for (int r = r0; r < r1; ++r) {
         const AttendRequest q = attend_request(a, r);
         if (q.bad && blockIdx.x == 0) req_error(&a.header->error, REQ_ERR_REQUEST);
-        const long long units = q.n ? units_of(q) : 0;
+        const long long units = q.n ? units_of(q, r) : 0;
         cum[r] = units;
         mine += units;
     }
@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
     pdl_wait();
     pdl_launch_dependents();
     const int group = a.n_heads / a.cache.n_kv;
-    const long long units = scan_units<THREADS>(a, cum, [&](const AttendRequest &q) {
+    const long long units = scan_units<THREADS>(a, cum, [&](const AttendRequest &q, int) {
         return (((long long)q.n * group + AR_ROWS - 1) / AR_ROWS) * a.cache.n_kv * ((q.len + q.n + AR_TILE - 1) / AR_TILE);
     });
     const long long per = max(at_div(units + gridDim.x - 1, gridDim.x), (long long)min_units);
@@ -599,7 +599,7 @@ constexpr int AT_SMEM = AT_ROWS * D * 2 + 4 * AT_OPERAND<D> + 1024 + (int)sizeof
 
 // Keys that some of rows [128 m, 128 m + 128) see, from the front on.
 __device__ __forceinline__ int at_tiles(const AttendArgs &a, const AttendRequest &q, int group, int m) {
-    const int seen = a.mask ? q.n : (int)min((long long)q.n, ((long long)(m + 1) * AT_ROWS - 1) / group + 1);
+    const int seen = a.mask ? q.n : (int)min((long long)q.n, at_div((long long)(m + 1) * AT_ROWS - 1, group) + 1);
     return (q.len + seen + AT_TILE - 1) / AT_TILE;
 }
 // 128-byte swizzle, columns of the operand side by side (MN-major): blocks of 64 columns `block` bytes apart, groups of eight k 1024.
@@ -664,14 +664,33 @@ struct AttendWalk {
             const long long rem = x - cum[s.r], per_head = at_div(cum[s.r + 1] - cum[s.r], a.cache.n_kv);
             s.hk = (int)at_div(rem, per_head);
             long long left = rem - s.hk * per_head, units;
-            s.m = 0;
             if (a.mask) {  // all segments of a request are as long
                 s.n_tiles = at_tiles(a, rq, group, 0);
                 units = at_padded(s.n_tiles, pad);
                 s.m = (int)at_div(left, units);
                 left -= s.m * units;
-            } else {
-                while (left >= (units = at_padded(s.n_tiles = at_tiles(a, rq, group, s.m), pad))) left -= units, ++s.m;
+            } else {  // a prompt's grow: 32 at a time (a warp calls this)
+                const int lane = threadIdx.x & 31;
+                for (s.m = 0;; s.m += 32) {
+                    const int mine = at_tiles(a, rq, group, s.m + lane);
+                    const long long u = at_padded(mine, pad);
+                    long long incl = u;
+#pragma unroll
+                    for (int d = 1; d < 32; d <<= 1) {
+                        const long long v = __shfl_up_sync(0xffffffffu, incl, d);
+                        if (lane >= d) incl += v;
+                    }
+                    const uint32_t behind = __ballot_sync(0xffffffffu, incl > left);
+                    if (behind) {
+                        const int at = __ffs(behind) - 1;
+                        s.m += at;
+                        s.n_tiles = __shfl_sync(0xffffffffu, mine, at);
+                        units = __shfl_sync(0xffffffffu, u, at);
+                        left -= __shfl_sync(0xffffffffu, incl, at) - units;
+                        break;
+                    }
+                    left -= __shfl_sync(0xffffffffu, incl, 31);
+                }
             }
             s.tile0 = (int)left;
             s.tiles = (int)min(end - x, (long long)s.n_tiles - left);
@@ -780,9 +799,22 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
         dg_tmem_alloc(smem_u32(&sh.tmem), AT_COLS);
         dg_tmem_relinquish();
     }
+    // (few requests without masks may be long prompts, whose segments differ: a warp per request adds theirs up)
+    const bool by_warp = !a.mask && a.R <= 64;
     auto all_units = [&](long long pad) {
-        return scan_units<AT_THREADS>(a, cum, [&](const AttendRequest &q) {
-            const int m_tiles = (int)(((long long)q.n * group + AT_ROWS - 1) / AT_ROWS);
+        for (int r = warp; by_warp && r < a.R; r += AT_THREADS / 32) {
+            const AttendRequest q = attend_request(a, r);
+            const int m_tiles = (int)at_div((long long)q.n * group + AT_ROWS - 1, AT_ROWS);
+            long long tiles = 0;
+            for (int m = lane; m < m_tiles; m += 32) tiles += AttendWalk<D>::at_padded(at_tiles(a, q, group, m), pad);
+#pragma unroll
+            for (int d = 16; d; d >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, d);
+            if (lane == 0) cum[r] = tiles * a.cache.n_kv;
+        }
+        __syncthreads();
+        return scan_units<AT_THREADS>(a, cum, [&](const AttendRequest &q, int r) {
+            if (by_warp) return cum[r];
+            const int m_tiles = (int)at_div((long long)q.n * group + AT_ROWS - 1, AT_ROWS);
             long long tiles = 0;
             if (a.mask) tiles = m_tiles * AttendWalk<D>::at_padded(at_tiles(a, q, group, 0), pad);
             else for (int m = 0; m < m_tiles; ++m) tiles += AttendWalk<D>::at_padded(at_tiles(a, q, group, m), pad);

@@ -507,17 +507,19 @@ def rope_halfsplit(x, lut, n_heads: int, head_dim: int, out=None):
 # ---- many requests: paged cache, drafted tokens, adapters -----------------------------------------------------------------
 def _on(t: torch.Tensor, name: str, dtype, device: int, dim: int = 1):
     """`t` as an argument on `device`: its type, its dimensions, its values side by side."""
+    if t.dtype is dtype and t.get_device() == device and t.dim() == dim and t.is_contiguous():
+        return t.data_ptr()
     if t.dtype != dtype or t.dim() != dim or t.get_device() != device:
         raise _lib.AwqBackendError(f"{name} must be a {dim}-dimensional {dtype} tensor on cuda:{device}, got {t.dim()} dimensions of {t.dtype} "
                                    f"on {t.device}")
-    if not t.is_contiguous():
-        raise _lib.AwqBackendError(f"{name} must be contiguous")
-    return t.data_ptr()
+    raise _lib.AwqBackendError(f"{name} must be contiguous")
 
 
-def _numel(t: torch.Tensor, name: str, n: int, at_least=False):
-    if t.numel() < n or (t.numel() > n and not at_least):
-        raise _lib.AwqBackendError(f"{name} must have {'at least ' if at_least else ''}{n} elements, got {t.numel()}")
+def _sizes(**want):
+    """Raises for the first (tensor, elements) that does not fit."""
+    for name, (t, n) in want.items():
+        if t.numel() != n:
+            raise _lib.AwqBackendError(f"{name} must have {n} elements, got {t.numel()}")
 
 
 def _call_on(device: int, name: str, *args):
@@ -574,13 +576,15 @@ class KVCache:
 
     def rows(self, t: torch.Tensor, name: str, n_heads=None, rows=None):
         """Checks [T, heads, head_dim] rows that go with the cache (column slices of a wider projection are fine)."""
-        if t.dim() != 3 or t.dtype != self.dtype or t.get_device() != self.device or t.shape[2] != self.head_dim or t.stride(2) != 1:
-            raise _lib.AwqBackendError(f"{name} must be [T, heads, {self.head_dim}] of {self.dtype} on cuda:{self.device} with unit stride over head_dim, "
-                                       f"got {tuple(t.shape)} of {t.dtype} on {t.device}")
-        if (n_heads is not None and t.shape[1] != n_heads) or (rows is not None and t.shape[0] != rows):
-            raise _lib.AwqBackendError(f"{name} must be [{rows}, {n_heads}, {self.head_dim}], got {tuple(t.shape)}")
+        if t.dim() != 3 or t.dtype is not self.dtype or t.get_device() != self.device:
+            raise _lib.AwqBackendError(f"{name} must be [T, heads, {self.head_dim}] of {self.dtype} on cuda:{self.device}, got {tuple(t.shape)} of {t.dtype} on {t.device}")
+        T, heads, dim = t.shape
+        row, head, unit = t.stride()
+        if dim != self.head_dim or unit != 1 or (n_heads is not None and heads != n_heads) or (rows is not None and T != rows):
+            raise _lib.AwqBackendError(f"{name} must be [{'T' if rows is None else rows}, {'heads' if n_heads is None else n_heads}, {self.head_dim}] with unit "
+                                       f"stride over head_dim, got {tuple(t.shape)}")
         # the stride of a dimension of one is arbitrary and never used
-        return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0
+        return t.data_ptr(), row if T > 1 else 0, head if heads > 1 else 0
 
 
 @dataclass
@@ -593,10 +597,11 @@ class StepPlan:
 
 
 def _table(table: torch.Tensor, R: int, device: int):
-    if table.dtype != torch.int32 or table.dim() != 2 or table.get_device() != device or table.shape[0] != R or \
-            (table.shape[1] > 1 and table.stride(1) != 1):
-        raise _lib.AwqBackendError(f"table must be int32 [{R}, width] on cuda:{device} with unit column stride, got {tuple(table.shape)} of {table.dtype}")
-    return table.data_ptr(), table.stride(0) if R > 1 else table.shape[1], table.shape[1]
+    if table.dtype is torch.int32 and table.dim() == 2 and table.get_device() == device:
+        (rows, width), (stride, unit) = table.shape, table.stride()
+        if rows == R and (unit == 1 or width <= 1):
+            return table.data_ptr(), stride if R > 1 else width, width
+    raise _lib.AwqBackendError(f"table must be int32 [{R}, width] on cuda:{device} with unit column stride, got {tuple(table.shape)} of {table.dtype}")
 
 
 def page_plan(lens, new, table, free_pages, free_count, page_size: int, T: int, ws: RequestWorkspace, parents=None, free_count_out=None,
@@ -607,34 +612,29 @@ def page_plan(lens, new, table, free_pages, free_count, page_size: int, T: int, 
     -1: the last cached one; at most 64 per request), the mask of its ancestors.  free_count is updated in place unless
     free_count_out is given; lens stays: `page_keep` moves it on.  A step that does not fit changes nothing, has no rows, and
     ws.check() says so; rows behind the last request get slot -1."""
-    dev, R = ws.device, lens.numel()
-    lens_p, new_p = _on(lens, "lens", torch.int32, dev), _on(new, "new", torch.int32, dev)
-    _numel(new, "new", R)
-    table_p, stride, width = _table(table, R, dev)
-    free_p, count_p = _on(free_pages, "free_pages", torch.int32, dev), _on(free_count, "free_count", torch.int32, dev)
-    _numel(free_count, "free_count", 1)
+    dev, R, i32 = ws.device, lens.numel(), torch.int32
     count_out = free_count if free_count_out is None else free_count_out
-    count_out_p = _on(count_out, "free_count_out", torch.int32, dev)
-    _numel(count_out, "free_count_out", 1)
-    if out is None:
-        i32 = dict(dtype=torch.int32, device=lens.device)
-        out = StepPlan(torch.empty(R + 1, **i32), torch.empty(T, **i32), torch.empty(T, **i32),
-                       None if parents is None else torch.empty(T, dtype=torch.int64, device=lens.device))
+    lens_p, new_p, free_p, count_p, count_out_p = (_on(lens, "lens", i32, dev), _on(new, "new", i32, dev), _on(free_pages, "free_pages", i32, dev),
+                                                   _on(free_count, "free_count", i32, dev), _on(count_out, "free_count_out", i32, dev))
+    table_p, stride, width = _table(table, R, dev)
+    if new.numel() != R or free_count.numel() != 1 or count_out.numel() != 1:
+        _sizes(new=(new, R), free_count=(free_count, 1), free_count_out=(count_out, 1))
+    if out is None:  # one allocation, three views of it
+        rows = torch.empty(R + 1 + 2 * T, dtype=i32, device=lens.device)
+        out = StepPlan(*rows.split((R + 1, T, T)), None if parents is None else torch.empty(T, dtype=torch.int64, device=lens.device))
     parents_p = mask_p = None
     if parents is not None:
-        parents_p = _on(parents, "parents", torch.int32, dev)
-        _numel(parents, "parents", T)
+        parents_p = _on(parents, "parents", i32, dev)
         if out.mask is None:
             raise _lib.AwqBackendError("page_plan: parents need a mask in `out`")
         mask_p = _on(out.mask, "out.mask", torch.int64, dev)
-        _numel(out.mask, "out.mask", T)
+        if parents.numel() != T or out.mask.numel() != T:
+            _sizes(parents=(parents, T), mask=(out.mask, T))
     elif out.mask is not None:
         raise _lib.AwqBackendError("page_plan: a mask in `out` needs parents")
-    start_p, slots_p, pos_p = (_on(t, n, torch.int32, dev) for t, n in (
-        (out.q_start, "out.q_start"), (out.slots, "out.slots"), (out.positions, "out.positions")))
-    _numel(out.q_start, "out.q_start", R + 1)
-    _numel(out.slots, "out.slots", T)
-    _numel(out.positions, "out.positions", T)
+    start_p, slots_p, pos_p = _on(out.q_start, "out.q_start", i32, dev), _on(out.slots, "out.slots", i32, dev), _on(out.positions, "out.positions", i32, dev)
+    if out.q_start.numel() != R + 1 or out.slots.numel() != T or out.positions.numel() != T:
+        _sizes(q_start=(out.q_start, R + 1), slots=(out.slots, T), positions=(out.positions, T))
     _call_on(dev, "awq_b200_page_plan", lens_p, new_p, table_p, stride, width, free_p, free_pages.numel(), count_p, count_out_p, parents_p,
              int(page_size), start_p, slots_p, pos_p, mask_p, R, T, ws.ptr, ws.nbytes)
     return out
@@ -657,8 +657,8 @@ def rope_append(q, k, v, lut, positions, slots, cache: KVCache, ws: RequestWorks
     if lut.shape[1] != cache.head_dim or lut.shape[0] == 0:
         raise _lib.AwqBackendError(f"lut must be [positions, {cache.head_dim}], got {tuple(lut.shape)}")
     pos_p, slots_p = _on(positions, "positions", torch.int32, dev), _on(slots, "slots", torch.int32, dev)
-    _numel(positions, "positions", T)
-    _numel(slots, "slots", T)
+    if positions.numel() != T or slots.numel() != T:
+        _sizes(positions=(positions, T), slots=(slots, T))
     _call_on(dev, "awq_b200_rope_append", qp, qr, qh, kp, kr, kh, vp, vr, vh, lut_p, lut.shape[0], pos_p, slots_p, op, orow, oh, cache.ptr, T, H,
              ws.ptr, ws.nbytes)
     return q if q_out is None else q_out
@@ -679,12 +679,14 @@ def tree_attention(q, cache: KVCache, table, lens, q_start, ws: RequestWorkspace
     op, orow, oh = cache.rows(out, "out", H, T)
     R = lens.numel()
     lens_p, start_p = _on(lens, "lens", torch.int32, dev), _on(q_start, "q_start", torch.int32, dev)
-    _numel(q_start, "q_start", R + 1)
+    if q_start.numel() != R + 1:
+        _sizes(q_start=(q_start, R + 1))
     table_p, stride, width = _table(table, R, dev)
     mask_p = None
     if mask is not None:
         mask_p = _on(mask, "mask", torch.int64, dev)
-        _numel(mask, "mask", T)
+        if mask.numel() != T:
+            _sizes(mask=(mask, T))
     _call_on(dev, "awq_b200_tree_attention", qp, qr, qh, cache.ptr, table_p, stride, width, lens_p, start_p, mask_p,
              cache.head_dim ** -0.5 if scale is None else float(scale), op, orow, oh, R, T, H, ws.ptr, ws.nbytes)
     return out
@@ -699,22 +701,24 @@ def page_keep(kv, table, lens, q_start, kept, free_pages, free_count, ws: Reques
     if kv.dim() != 6 or kv.shape[1] != 2 or kv.element_size() != 2 or kv.get_device() != dev or kv.numel() == 0:
         raise _lib.AwqBackendError(f"kv must be [layers, 2, n_pages, page_size, n_kv_heads, head_dim] of 16-bit values on cuda:{dev}, got "
                                    f"{tuple(kv.shape)} of {kv.dtype} on {kv.device}")
-    strides = [kv.stride(i) if kv.shape[i] > 1 else 0 for i in range(5)]
-    if kv.stride(5) != 1 or any(s % 8 or (s <= 0 and kv.shape[i] > 1) for i, s in enumerate(strides)):
+    shape, step = kv.shape, kv.stride()
+    strides = [step[i] if shape[i] > 1 else 0 for i in range(5)]
+    if step[5] != 1 or any(s % 8 or (s <= 0 and n > 1) for s, n in zip(strides, shape)):
         raise _lib.AwqBackendError("kv needs a unit stride over head_dim and positive multiples of 8 elsewhere")
     table_p, stride, width = _table(table, R, dev)
     lens_out = lens if lens_out is None else lens_out
     count_out = free_count if free_count_out is None else free_count_out
-    lens_p, lens_out_p, start_p, kept_p, free_p, count_p, count_out_p = (_on(t, n, torch.int32, dev) for t, n in (
-        (lens, "lens"), (lens_out, "lens_out"), (q_start, "q_start"), (kept, "kept"), (free_pages, "free_pages"), (free_count, "free_count"),
-        (count_out, "free_count_out")))
-    for t, n, k in ((lens_out, "lens_out", R), (q_start, "q_start", R + 1), (kept, "kept", R), (free_count, "free_count", 1),
-                    (count_out, "free_count_out", 1)):
-        _numel(t, n, k)
+    i32 = torch.int32
+    lens_p, lens_out_p, start_p, kept_p = (_on(lens, "lens", i32, dev), _on(lens_out, "lens_out", i32, dev), _on(q_start, "q_start", i32, dev),
+                                           _on(kept, "kept", i32, dev))
+    free_p, count_p, count_out_p = (_on(free_pages, "free_pages", i32, dev), _on(free_count, "free_count", i32, dev),
+                                    _on(count_out, "free_count_out", i32, dev))
+    if lens_out.numel() != R or q_start.numel() != R + 1 or kept.numel() != R or free_count.numel() != 1 or count_out.numel() != 1:
+        _sizes(lens_out=(lens_out, R), q_start=(q_start, R + 1), kept=(kept, R), free_count=(free_count, 1), free_count_out=(count_out, 1))
     path_p, T = None, _lib.MAX_ROWS
     if path is not None:
         path_p, T = _on(path, "path", torch.int32, dev), path.numel()
-    _call_on(dev, "awq_b200_page_keep", kv.data_ptr(), *strides, kv.shape[0], kv.shape[2], kv.shape[3], kv.shape[4], kv.shape[5], table_p, stride,
+    _call_on(dev, "awq_b200_page_keep", kv.data_ptr(), *strides, shape[0], *shape[2:], table_p, stride,
              width, lens_p, lens_out_p, start_p, kept_p, path_p, free_p, free_pages.numel(), count_p, count_out_p, R, T, ws.ptr, ws.nbytes)
     return lens_out
 
@@ -738,9 +742,7 @@ class LoraAdapters:
         self.A, self.B, self.scales, self.ranks = A, B, scales, ranks
         self._ptrs = (_on(A, "A", torch.bfloat16, self.device, 3), _on(B, "B", torch.bfloat16, self.device, 3),
                       _on(scales, "scales", torch.float32, self.device), None if ranks is None else _on(ranks, "ranks", torch.int32, self.device))
-        _numel(scales, "scales", self.n)
-        if ranks is not None:
-            _numel(ranks, "ranks", self.n)
+        _sizes(scales=(scales, self.n), **({} if ranks is None else dict(ranks=(ranks, self.n))))
         if not _aligned16(A, B):
             raise _lib.AwqBackendError("LoraAdapters: A and B must be 16-byte aligned")
 
@@ -756,7 +758,8 @@ def lora(x, adapters: LoraAdapters, idx, base, ws: RequestWorkspace, out=None, r
     T = x.shape[0]
     shape = (T, adapters.N)
     idx_p = _on(idx, "idx", torch.int32, dev)
-    _numel(idx, "idx", T)
+    if idx.numel() != T:
+        _sizes(idx=(idx, T))
     f32 = base.dtype == torch.float32
     base_p = _on(base, "base", torch.float32 if f32 else torch.bfloat16, dev, 2)
     if out is None:
