@@ -1175,18 +1175,24 @@ __global__ void __launch_bounds__(AT_ROWS) tree_attention_join_kernel(AttendArgs
     if (s.last < 0 || row >= s.n * group) return;
     const float *parts = reinterpret_cast<const float *>(a.scratch + AT_JOINS + sizeof(AttendJoin) * AT_MAX_CTAS);
     float top = -INFINITY, total = 0.f, o[AJ_COLS] = {};
-#pragma unroll 2
-    for (int c = c0; c <= s.last; ++c) {
-        const float *src = parts + (long long)(2 * c + (c == c0)) * PART + tid;
-        const float m = src[D * AT_ROWS], l = src[(D + 1) * AT_ROWS];
-        float v[AJ_COLS];
+    for (int c = c0; c <= s.last; c += 4) {  // four parts' values on their way at a time
+        float m[4], l[4], v[4][AJ_COLS];
 #pragma unroll
-        for (int e = 0; e < AJ_COLS; ++e) v[e] = src[(d0 + e) * AT_ROWS];
-        const float to = fmaxf(top, m), ref = to == -INFINITY ? 0.f : to, keep = exp2_fast(top - ref), f = exp2_fast(m - ref);
-        top = to;
-        total = total * keep + l * f;
+        for (int k = 0; k < 4; ++k) {
+            const float *src = parts + (long long)(2 * min(c + k, s.last) + (c + k == c0)) * PART + tid;
+            m[k] = c + k <= s.last ? src[D * AT_ROWS] : -INFINITY;
+            l[k] = src[(D + 1) * AT_ROWS];
 #pragma unroll
-        for (int e = 0; e < AJ_COLS; ++e) o[e] = (keep == 0.f ? 0.f : o[e] * keep) + (f == 0.f ? 0.f : v[e] * f);
+            for (int e = 0; e < AJ_COLS; ++e) v[k][e] = src[(d0 + e) * AT_ROWS];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float to = fmaxf(top, m[k]), ref = to == -INFINITY ? 0.f : to, keep = exp2_fast(top - ref), f = exp2_fast(m[k] - ref);
+            top = to;
+            total = total * keep + (f == 0.f ? 0.f : l[k] * f);
+#pragma unroll
+            for (int e = 0; e < AJ_COLS; ++e) o[e] = (keep == 0.f ? 0.f : o[e] * keep) + (f == 0.f ? 0.f : v[k][e] * f);
+        }
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;
     uint16_t *out = a.out + (long long)(s.q0 + row / group) * a.o_row + (long long)(s.hk * group + row % group) * a.o_head + d0;
