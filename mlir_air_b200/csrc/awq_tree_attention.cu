@@ -532,17 +532,26 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
                 for (int i = tid; i < rows * (D / 4); i += THREADS) {
                     const int row = i / (D / 4), d = 4 * (i % (D / 4));
                     float m = -INFINITY, l = 0.f, o[4] = {};
-#pragma unroll 8
-                    for (int c = c0; c <= c1; ++c) {
-                        const float *src = parts + (long long)(2 * c + (c == c0 ? 1 : 0)) * PART;
-                        const float mc = __ldcg(src + AR_ROWS * D + row), lc = __ldcg(src + AR_ROWS * D + AR_ROWS + row);
-                        const float4 u = __ldcg(reinterpret_cast<const float4 *>(src + row * D + d));
-                        const float m2 = fmaxf(m, mc), ref = m2 == -INFINITY ? 0.f : m2, f = exp2_fast(m - ref), fc = exp2_fast(mc - ref);
-                        m = m2;
-                        l = l * f + lc * fc;
-                        const float add[4] = {u.x, u.y, u.z, u.w};
+                    for (int at = c0; at <= c1; at += 8) {  // eight parts' loads at once
+                        float mc[8], lc[8];
+                        float4 u[8];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[e] = (f == 0.f ? 0.f : o[e] * f) + (fc == 0.f ? 0.f : add[e] * fc);
+                        for (int k = 0; k < 8; ++k) {
+                            const int c = min(at + k, c1);
+                            const float *src = parts + (long long)(2 * c + (c == c0 ? 1 : 0)) * PART;
+                            mc[k] = __ldcg(src + AR_ROWS * D + row), lc[k] = __ldcg(src + AR_ROWS * D + AR_ROWS + row);
+                            u[k] = __ldcg(reinterpret_cast<const float4 *>(src + row * D + d));
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            if (at + k <= c1) {
+                                const float m2 = fmaxf(m, mc[k]), ref = m2 == -INFINITY ? 0.f : m2, f = exp2_fast(m - ref), fc = exp2_fast(mc[k] - ref);
+                                m = m2;
+                                l = l * f + lc[k] * fc;
+                                const float add[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[e] = (f == 0.f ? 0.f : o[e] * f) + (fc == 0.f ? 0.f : add[e] * fc);
+                            }
                     }
                     store(row, d, o, l);
                 }
