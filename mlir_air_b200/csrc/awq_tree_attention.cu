@@ -177,21 +177,11 @@ __device__ __forceinline__ bool not_finite16x2(uint32_t v) {
     return (v & e) == e || ((v >> 16) & e) == e;
 }
 
-// Units of all requests before each one, in shared memory; returns their number.  Requests that do not fit are reported by
-// CTA 0 and have what attend_request leaves of them.
-template <int THREADS, typename F>
-__device__ __forceinline__ long long scan_units(const AttendArgs &a, long long *cum, F units_of) {
+// Of the block's threads before this one, and of all.
+template <int THREADS>
+__device__ __forceinline__ long long exclusive_sum(long long mine, long long &total) {
     __shared__ long long sums[THREADS / 32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per = (a.R + THREADS - 1) / THREADS, r0 = min(tid * per, a.R), r1 = min(r0 + per, a.R);
-    long long mine = 0;
-    for (int r = r0; r < r1; ++r) {
-        const AttendRequest q = attend_request(a, r);
-        if (q.bad && blockIdx.x == 0) req_error(&a.header->error, REQ_ERR_REQUEST);
-        const long long units = q.n ? units_of(q, r) : 0;
-        cum[r] = units;
-        mine += units;
-    }
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     long long incl = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -200,12 +190,29 @@ __device__ __forceinline__ long long scan_units(const AttendArgs &a, long long *
     }
     if (lane == 31) sums[warp] = incl;
     __syncthreads();
-    long long base = incl - mine, total = 0;
+    long long base = incl - mine;
+    total = 0;
 #pragma unroll
     for (int w = 0; w < THREADS / 32; ++w) {
         if (w < warp) base += sums[w];
         total += sums[w];
     }
+    return base;
+}
+// Units of all requests before each one, in shared memory; returns their number.  Requests that do not fit are reported by
+// CTA 0 and have what attend_request leaves of them.
+template <int THREADS, typename F>
+__device__ __forceinline__ long long scan_units(const AttendArgs &a, long long *cum, F units_of) {
+    const int tid = threadIdx.x, per = (a.R + THREADS - 1) / THREADS, r0 = min(tid * per, a.R), r1 = min(r0 + per, a.R);
+    long long mine = 0;
+    for (int r = r0; r < r1; ++r) {
+        const AttendRequest q = attend_request(a, r);
+        if (q.bad && blockIdx.x == 0) req_error(&a.header->error, REQ_ERR_REQUEST);
+        const long long units = q.n ? units_of(q, r) : 0;
+        cum[r] = units;
+        mine += units;
+    }
+    long long total, base = exclusive_sum<THREADS>(mine, total);
     for (int r = r0; r < r1; ++r) {
         const long long u = cum[r];
         cum[r] = base;
@@ -226,14 +233,17 @@ __device__ __forceinline__ int request_of_unit(const long long *cum, int n, long
     return lo;
 }
 
-// Shared memory: Q in operand order | places of the keys | K and V, later the warps' results | tiles before each request
+// Shared memory: Q in operand order | places of the keys | K and V, later the warps' results | units.  The same for any number of
+// requests (three CTAs fit an SM): a thread adds up the units of several, and who has some of them looks through these requests again.
 constexpr int AR_PLACES = 4 * 16 * 16 + 64;  // of a warp: four blocks of 16 keys, and which of them there are (stages start on 128 bytes)
 template <int D>
 constexpr int AR_STAGE = 16 * D * 4;  // K and V of a warp's block
 template <int D>
 constexpr int AR_STAGES = AR_WARPS * (2 * AR_STAGE<D> > AR_ROWS * (D + 2) * 4 ? 2 * AR_STAGE<D> : AR_ROWS * (D + 2) * 4);
+constexpr int AR_CUM = (AR_WARPS * 32 + 1) * 8;  // units before each thread's requests
 template <int D>
-constexpr int AR_SMEM = D * 32 + AR_WARPS * AR_PLACES + AR_STAGES<D>;
+constexpr int AR_SMEM = D * 32 + AR_WARPS * AR_PLACES + AR_STAGES<D> + AR_CUM;
+static_assert(AR_SMEM<128> + 64 <= 224 * 1024 / AR_PER_SM - 1024, "three CTAs an SM (76096 bytes a CTA measured two)");
 
 template <bool F16, int D>
 __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_kernel(AttendArgs a, int min_units) {
@@ -252,14 +262,24 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
     const uint32_t piece_v[2] = {(uint32_t)(cp ^ (ck & 2)) * 16, (uint32_t)(cp ^ (ck & 2) ^ 4) * 16};
     float *ow = reinterpret_cast<float *>(stages);                           // [WARPS][16][D]
     float *mw = ow + AR_WARPS * AR_ROWS * D, *lw = mw + AR_WARPS * AR_ROWS;   // [WARPS][16]
-    long long *cum = reinterpret_cast<long long *>(smem + AR_SMEM<D>);
+    long long *cum = reinterpret_cast<long long *>(smem + AR_SMEM<D> - AR_CUM);
     __shared__ int s_last;
     pdl_wait();
     pdl_launch_dependents();
     const int group = a.n_heads / a.cache.n_kv;
-    const long long units = scan_units<THREADS>(a, cum, [&](const AttendRequest &q, int) {
+    auto units_of = [&](const AttendRequest &q) {
         return (((long long)q.n * group + AR_ROWS - 1) / AR_ROWS) * a.cache.n_kv * ((q.len + q.n + AR_TILE - 1) / AR_TILE);
-    });
+    };
+    const int of_thread = (a.R + THREADS - 1) / THREADS;  // requests
+    long long mine_units = 0, units;
+    for (int r = tid * of_thread; r < min((tid + 1) * of_thread, a.R); ++r) {
+        const AttendRequest q = attend_request(a, r);
+        if (q.bad && blockIdx.x == 0) req_error(&a.header->error, REQ_ERR_REQUEST);
+        mine_units += units_of(q);
+    }
+    cum[tid] = exclusive_sum<THREADS>(mine_units, units);
+    if (tid == 0) cum[THREADS] = units;
+    __syncthreads();
     const long long per = max(at_div(units + gridDim.x - 1, gridDim.x), (long long)min_units);
     long long x = blockIdx.x * per;
     const long long end = min(x + per, units);
@@ -269,10 +289,30 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
     constexpr int PART = AR_ROWS * (D + 2);
 
     while (x < end) {
-        const int r = request_of_unit(cum, a.R, x);
-        const AttendRequest rq = attend_request(a, r);
+        int r = request_of_unit(cum, THREADS, x);  // the thread whose requests these are
+        long long rem = x - cum[r];
+        AttendRequest rq;
+        if (of_thread == 1) {
+            rq = attend_request(a, r);
+        } else {
+            for (int r0 = r * of_thread;; r0 += 32) {  // (units of one of them lie behind x)
+                const AttendRequest q = r0 + lane < a.R ? attend_request(a, r0 + lane) : AttendRequest{};
+                const long long u = units_of(q);
+                long long incl = u;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const long long v = __shfl_up_sync(0xffffffffu, incl, d);
+                    if (lane >= d) incl += v;
+                }
+                const uint32_t behind = __ballot_sync(0xffffffffu, incl > rem);
+                const int l = behind ? __ffs(behind) - 1 : 31;
+                r = r0 + l;
+                rem -= __shfl_sync(0xffffffffu, behind ? incl - u : incl, l);
+                rq = {__shfl_sync(0xffffffffu, q.q0, l), __shfl_sync(0xffffffffu, q.n, l), __shfl_sync(0xffffffffu, q.len, l), false};
+                if (behind || r0 + 32 >= a.R) break;
+            }
+        }
         const int total = rq.len + rq.n, n_tiles = (total + AR_TILE - 1) / AR_TILE, m_tiles = (rq.n * group + AR_ROWS - 1) / AR_ROWS;
-        const long long rem = x - cum[r];
         const int seg = (int)at_div(rem, n_tiles), tile0 = (int)(rem - (long long)seg * n_tiles), hk = seg / m_tiles, row0 = (seg % m_tiles) * AR_ROWS;
         const long long seg_start = x - tile0, seg_end = seg_start + n_tiles;
         const int tiles = (int)(min(end, seg_end) - x);
@@ -1279,7 +1319,7 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
         }
         auto kernel = view.head_dim == 64 ? (f16 ? tree_attention_rows_kernel<true, 64> : tree_attention_rows_kernel<false, 64>)
                                           : (f16 ? tree_attention_rows_kernel<true, 128> : tree_attention_rows_kernel<false, 128>);
-        const int smem = (view.head_dim == 64 ? AR_SMEM<64> : AR_SMEM<128>) + (R + 1) * 8;
+        const int smem = (view.head_dim == 64 ? AR_SMEM<64> : AR_SMEM<128>);
         if ((rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "tree_attention shared memory"))) return rc;
         const int grid = min(device_sm_count() * AR_PER_SM, AR_MAX_CTAS);
         return check_cuda(launch_pdl(kernel, dim3(grid), dim3(AR_WARPS * 32), smem, as_stream(stream), a, 1), "tree_attention launch");

@@ -83,6 +83,12 @@ def test_many_requests_of_all_lengths():
     run(lens, [(i * 7) % 5 for i in range(150)], 8, 2, 128, 16, tree=True)
 
 
+@pytest.mark.parametrize("H,kv", [(2, 1), (24, 1)])
+@pytest.mark.parametrize("n", [128, 129, 300, 1000, 4096])
+def test_as_many_requests_as_there_may_be(n, H, kv):
+    run([(i * 37) % 90 for i in range(n)], [0 if i % 50 < 40 and i > n // 2 else 1 + (i % 9 == 0) for i in range(n)], H, kv, 64, 16)
+
+
 @pytest.mark.parametrize("q_scale", [0.0, 12.0, 60.0])
 def test_flat_and_peaked_scores(q_scale):
     run([700, 40], [5, 1], 8, 2, 128, 16, tree=True, q_scale=q_scale)
