@@ -246,7 +246,7 @@ constexpr int AR_SMEM = D * 32 + AR_WARPS * AR_PLACES + AR_STAGES<D> + AR_CUM;
 static_assert(AR_SMEM<128> + 64 <= 224 * 1024 / AR_PER_SM - 1024, "three CTAs an SM (76096 bytes a CTA measured two)");
 
 template <bool F16, int D>
-__global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_kernel(AttendArgs a, int min_units) {
+__global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_kernel(AttendArgs a) {
     constexpr int THREADS = AR_WARPS * 32, QC = D / 32, VC = D / 64;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
@@ -267,20 +267,44 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
     pdl_wait();
     pdl_launch_dependents();
     const int group = a.n_heads / a.cache.n_kv;
-    auto units_of = [&](const AttendRequest &q) {
-        return (((long long)q.n * group + AR_ROWS - 1) / AR_ROWS) * a.cache.n_kv * ((q.len + q.n + AR_TILE - 1) / AR_TILE);
+    long long pad = 1;  // a segment takes a multiple of this
+    auto segments_of = [&](const AttendRequest &q) { return (((long long)q.n * group + AR_ROWS - 1) / AR_ROWS) * a.cache.n_kv; };
+    auto units_of = [&](const AttendRequest &q, long long pad) {
+        const int tiles = (q.len + q.n + AR_TILE - 1) / AR_TILE;
+        return segments_of(q) * (pad > 1 ? at_div(tiles + pad - 1, pad) * pad : tiles);
     };
     const int of_thread = (a.R + THREADS - 1) / THREADS;  // requests
-    long long mine_units = 0, units;
-    for (int r = tid * of_thread; r < min((tid + 1) * of_thread, a.R); ++r) {
-        const AttendRequest q = attend_request(a, r);
-        if (q.bad && blockIdx.x == 0) req_error(&a.header->error, REQ_ERR_REQUEST);
-        mine_units += units_of(q);
+    AttendRequest own{};
+    auto sum_over_requests = [&](auto f) {
+        long long sum = 0, total;
+        for (int r = tid * of_thread; r < min((tid + 1) * of_thread, a.R); ++r) {
+            if (of_thread > 1) own = attend_request(a, r);
+            sum += f(own);
+        }
+        __syncthreads();  // (the last sums have been read)
+        cum[tid] = exclusive_sum<THREADS>(sum, total);
+        if (tid == 0) cum[THREADS] = total;
+        __syncthreads();
+        return total;
+    };
+    if (of_thread == 1 && tid < a.R) own = attend_request(a, tid);
+    if (blockIdx.x == 0)
+        for (int r = tid; r < a.R; r += THREADS)
+            if (attend_request(a, r).bad) req_error(&a.header->error, REQ_ERR_REQUEST);
+    long long units = sum_over_requests([&](const AttendRequest &q) { return units_of(q, 1); });
+    long long per = max(at_div(units + gridDim.x - 1, gridDim.x), 1LL);
+    // A CTA that goes on with another segment pays for a chain of loads again (starts, pages, keys), about as long as four tiles take.
+    // Where CTAs have few tiles anyway, every segment begins at one of its own, if that makes none of them much longer: one token of 16
+    // requests of 100 to 2000, 32/8 heads of 128, 23.4 -> 18.7 us.
+    if (per > 1 && per <= 16) {
+        const long long segments = sum_over_requests(segments_of);
+        for (long long p = per; segments <= gridDim.x && pad == 1 && p <= per + at_div(4 * segments, gridDim.x); ++p)
+            if (sum_over_requests([&](const AttendRequest &q) { return units_of(q, p); }) <= p * gridDim.x) pad = p;
+        if (pad > 1)
+            per = pad, units = cum[THREADS];
+        else
+            units = sum_over_requests([&](const AttendRequest &q) { return units_of(q, 1); });
     }
-    cum[tid] = exclusive_sum<THREADS>(mine_units, units);
-    if (tid == 0) cum[THREADS] = units;
-    __syncthreads();
-    const long long per = max(at_div(units + gridDim.x - 1, gridDim.x), (long long)min_units);
     long long x = blockIdx.x * per;
     const long long end = min(x + per, units);
     const int page_size = a.cache.page_size;
@@ -297,7 +321,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
         } else {
             for (int r0 = r * of_thread;; r0 += 32) {  // (units of one of them lie behind x)
                 const AttendRequest q = r0 + lane < a.R ? attend_request(a, r0 + lane) : AttendRequest{};
-                const long long u = units_of(q);
+                const long long u = units_of(q, pad);
                 long long incl = u;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
@@ -313,9 +337,12 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
             }
         }
         const int total = rq.len + rq.n, n_tiles = (total + AR_TILE - 1) / AR_TILE, m_tiles = (rq.n * group + AR_ROWS - 1) / AR_ROWS;
-        const int seg = (int)at_div(rem, n_tiles), tile0 = (int)(rem - (long long)seg * n_tiles), hk = seg / m_tiles, row0 = (seg % m_tiles) * AR_ROWS;
+        const long long n_units = pad > 1 ? at_div(n_tiles + pad - 1, pad) * pad : n_tiles;
+        const int seg = (int)at_div(rem, n_units), tile0 = (int)(rem - seg * n_units), hk = seg / m_tiles, row0 = (seg % m_tiles) * AR_ROWS;
         const long long seg_start = x - tile0, seg_end = seg_start + n_tiles;
         const int tiles = (int)(min(end, seg_end) - x);
+        x = min(end, seg_start + n_units);
+        if (tiles <= 0) continue;
         const int32_t *table = a.table + r * a.table_stride;
         const uint16_t *kbase = a.cache.k + hk * a.cache.k_head + 8 * cp, *vbase = a.cache.v + hk * a.cache.v_head + 8 * cp;
 
@@ -598,7 +625,6 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
                 if (tid == 0) counters[c0] = 0;
             }
         }
-        x += tiles;
     }
 }
 
@@ -1322,7 +1348,7 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
         const int smem = (view.head_dim == 64 ? AR_SMEM<64> : AR_SMEM<128>);
         if ((rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "tree_attention shared memory"))) return rc;
         const int grid = min(device_sm_count() * AR_PER_SM, AR_MAX_CTAS);
-        return check_cuda(launch_pdl(kernel, dim3(grid), dim3(AR_WARPS * 32), smem, as_stream(stream), a, 1), "tree_attention launch");
+        return check_cuda(launch_pdl(kernel, dim3(grid), dim3(AR_WARPS * 32), smem, as_stream(stream), a), "tree_attention launch");
     }
     const long long items = (long long)T * n_heads;
     AWQ_REQUIRE((items + 3) / 4 <= 0x7fffffffLL, "tree_attention: too many rows and heads");
