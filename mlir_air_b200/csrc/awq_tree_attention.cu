@@ -56,76 +56,113 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2 units in the last pl
 }
 __device__ __forceinline__ int page_index(const AttendArgs &a, int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / a.cache.page_size; }
 
-// Any head size: a warp per row and head, one key after another.  Head sizes that have no tensor-core kernel.
+// Head sizes above 128: a CTA per row and head, a warp per 32 keys, four of them at a time; f32 throughout.  Rows of a group do not share
+// their loads.  Bound by instructions (64 requests of 500 to 4000 tokens, 8/4 heads of 256: 767 us, 0.6 TB/s).
+constexpr int AA_WARPS = 4;
 template <bool F16>
-__global__ void __launch_bounds__(128) tree_attention_any_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(AA_WARPS * 32) tree_attention_any_kernel(AttendArgs a) {
+    constexpr int AHEAD = 4;
+    __shared__ float2 accs[AA_WARPS][128];
+    __shared__ float tops[AA_WARPS], totals[AA_WARPS];
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int t = (int)(item / a.n_heads), h = (int)(item % a.n_heads);
-    if (t >= a.T) return;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, t = blockIdx.x / a.n_heads, h = blockIdx.x % a.n_heads;
     int lo = 0, hi = a.R;  // the request of row t
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (a.q_start[mid] <= t) lo = mid; else hi = mid;
     }
     const AttendRequest q = attend_request(a, lo);
-    if (q.bad && lane == 0) req_error(&a.header->error, REQ_ERR_REQUEST);
+    if (blockIdx.x == 0)
+        for (int r = tid; r < a.R; r += AA_WARPS * 32)
+            if (attend_request(a, r).bad) req_error(&a.header->error, REQ_ERR_REQUEST);
     const int j = t - q.q0;
     if (j < 0 || j >= q.n) return;  // behind the last request
     const int D = a.cache.head_dim, pairs = D >> 1, hk = h / (a.n_heads / a.cache.n_kv);
     const unsigned long long bits = a.mask ? (unsigned long long)a.mask[t] : 0;
-    const uint16_t *qp = a.q + t * a.q_row + h * a.q_head;
+    const uint32_t *qp = reinterpret_cast<const uint32_t *>(a.q + t * a.q_row + h * a.q_head);
+    const uint32_t *kb = reinterpret_cast<const uint32_t *>(a.cache.k + hk * a.cache.k_head) + lane;
+    const uint32_t *vb = reinterpret_cast<const uint32_t *>(a.cache.v + hk * a.cache.v_head) + lane;
     float2 qv[4], acc[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int c = lane + 32 * i;
-        qv[i] = c < pairs ? unpack16x2<F16>(reinterpret_cast<const uint32_t *>(qp)[c]) : make_float2(0.f, 0.f);
+        qv[i] = c < pairs ? unpack16x2<F16>(qp[c]) : make_float2(0.f, 0.f);
         acc[i] = make_float2(0.f, 0.f);
     }
     float top = -INFINITY, total = 0.f;
-    for (int p = 0; p < q.len + q.n; ++p) {
-        const int d = p - q.len;
-        if (d >= 0 && !(a.mask ? d < 64 && (bits >> d & 1) : d <= j)) continue;
-        const int page = a.table[lo * a.table_stride + p / a.cache.page_size], off = p % a.cache.page_size;
-        if ((unsigned)page >= (unsigned)a.cache.n_pages) {
-            if (lane == 0) req_error(&a.header->error, REQ_ERR_PAGE);
-            continue;
+    for (int p0 = warp * 32; p0 < q.len + q.n; p0 += AA_WARPS * 32) {
+        const int p = p0 + lane, d = p - q.len;
+        long long k_at = -1, v_at = -1;  // of this lane's key, in pairs
+        if (p < q.len + q.n && (d < 0 || (a.mask ? d < 64 && (bits >> d & 1) : d <= j))) {
+            const int block = page_index(a, p), page = a.table[lo * a.table_stride + block], off = p - block * a.cache.page_size;
+            if ((unsigned)page < (unsigned)a.cache.n_pages)
+                k_at = (page * a.cache.k_page + off * a.cache.k_slot) >> 1, v_at = (page * a.cache.v_page + off * a.cache.v_slot) >> 1;
+            else
+                req_error(&a.header->error, REQ_ERR_PAGE);
         }
-        const uint32_t *kp = reinterpret_cast<const uint32_t *>(a.cache.k + page * a.cache.k_page + off * a.cache.k_slot + hk * a.cache.k_head);
-        const uint32_t *vp = reinterpret_cast<const uint32_t *>(a.cache.v + page * a.cache.v_page + off * a.cache.v_slot + hk * a.cache.v_head);
-        float s = 0.f;
+        const uint32_t seen = __ballot_sync(0xffffffffu, k_at >= 0);
+        for (int i0 = 0; i0 < 32; i0 += AHEAD) {
+            if (!(seen >> i0 & ((1u << AHEAD) - 1))) continue;
+            uint32_t kw[AHEAD][4], vw[AHEAD][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = lane + 32 * i;
-            if (c < pairs) {
-                const float2 k = unpack16x2<F16>(kp[c]);
-                s = fmaf(qv[i].x, k.x, fmaf(qv[i].y, k.y, s));
+            for (int n = 0; n < AHEAD; ++n) {
+                const long long ko = __shfl_sync(0xffffffffu, k_at, i0 + n), vo = __shfl_sync(0xffffffffu, v_at, i0 + n);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool there = ko >= 0 && lane + 32 * i < pairs;
+                    kw[n][i] = there ? __ldg(kb + ko + 32 * i) : 0;
+                    vw[n][i] = there ? __ldg(vb + vo + 32 * i) : 0;
+                }
             }
-        }
+            float s[AHEAD], m = top;
 #pragma unroll
-        for (int d2 = 16; d2; d2 >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d2);
-        s *= a.scale_log2;
-        const float m = fmaxf(top, s), keep = m == -INFINITY ? 1.f : exp2f(top - m), w = m == -INFINITY ? 0.f : exp2f(s - m);
-        top = m;
-        total = total * keep + w;
+            for (int n = 0; n < AHEAD; ++n) {
+                s[n] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = lane + 32 * i;
-            if (c < pairs) {
-                const float2 v = unpack16x2<F16>(vp[c]);
-                acc[i] = make_float2(fmaf(w, v.x, acc[i].x * keep), fmaf(w, v.y, acc[i].y * keep));
+                for (int i = 0; i < 4; ++i) {
+                    const float2 k = unpack16x2<F16>(kw[n][i]);
+                    s[n] = fmaf(qv[i].x, k.x, fmaf(qv[i].y, k.y, s[n]));
+                }
+#pragma unroll
+                for (int x = 16; x; x >>= 1) s[n] += __shfl_xor_sync(0xffffffffu, s[n], x);
+                s[n] = seen >> (i0 + n) & 1 ? s[n] * a.scale_log2 : -INFINITY;
+                m = fmaxf(m, s[n]);
+            }
+            const float ref = m == -INFINITY ? 0.f : m, keep = exp2f(top - ref);
+            top = m;
+            total *= keep;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[i] = make_float2(acc[i].x * keep, acc[i].y * keep);
+#pragma unroll
+            for (int n = 0; n < AHEAD; ++n) {
+                const float w = exp2f(s[n] - ref);
+                total += w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 v = unpack16x2<F16>(vw[n][i]);
+                    acc[i] = make_float2(fmaf(w, v.x, acc[i].x), fmaf(w, v.y, acc[i].y));
+                }
             }
         }
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    uint32_t *op = reinterpret_cast<uint32_t *>(a.out + t * a.o_row + h * a.o_head);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int c = lane + 32 * i;
-        if (c < pairs) op[c] = pack16x2<F16>(acc[i].x * inv, acc[i].y * inv);
+    for (int i = 0; i < 4; ++i) accs[warp][lane + 32 * i] = acc[i];
+    if (lane == 0) tops[warp] = top, totals[warp] = total;
+    __syncthreads();
+    float m = -INFINITY, sum = 0.f;
+    float2 o = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < AA_WARPS; ++w) m = fmaxf(m, tops[w]);
+#pragma unroll
+    for (int w = 0; w < AA_WARPS; ++w) {
+        if (tops[w] == -INFINITY) continue;  // saw nothing
+        const float f = exp2f(tops[w] - m);
+        sum = fmaf(f, totals[w], sum);
+        o = make_float2(fmaf(f, accs[w][tid].x, o.x), fmaf(f, accs[w][tid].y, o.y));
     }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (tid < pairs) reinterpret_cast<uint32_t *>(a.out + t * a.o_row + h * a.o_head)[tid] = pack16x2<F16>(o.x * inv, o.y * inv);
 }
 
 // =====================================================================================
@@ -146,6 +183,10 @@ __global__ void __launch_bounds__(128) tree_attention_any_kernel(AttendArgs a) {
 //           head element 8 n + j, so that a lane's results are 16 neighbours; pieces are shifted by pairs of keys.
 // Weights are multiplied as two 16-bit pieces, p = hi + lo: the tensor cores have time to spare, and the result keeps the
 // accuracy of f32 weights.
+//
+// Measured, bf16, heads of 128: one token of 64 requests of 1000 to 16000, 64/8 heads, 263 us, 5.85 TB/s (89 % of a copy's rate; keys
+// straight to registers 389); one token of 256 requests of 500 to 2000, 32/8 heads, 205 us, 5.6 TB/s.  Small steps are a chain of
+// latencies: starts and lengths, pages, keys, the join (one token behind 777, 32/8 heads of 64: 10 us).
 // =====================================================================================
 constexpr int AR_WARPS = 4, AR_TILE = AR_WARPS * 16, AR_PER_SM = 3, AR_ROWS = 16;
 constexpr int AR_MAX_CTAS = 192 * AR_PER_SM;
@@ -245,8 +286,11 @@ template <int D>
 constexpr int AR_SMEM = D * 32 + AR_WARPS * AR_PLACES + AR_STAGES<D> + AR_CUM;
 static_assert(AR_SMEM<128> + 64 <= 224 * 1024 / AR_PER_SM - 1024, "three CTAs an SM (76096 bytes a CTA measured two)");
 
-template <bool F16, int D>
+// PADDED: heads of other sizes below D; what lies behind them is 0 in shared memory and neither read nor written (64 requests of 500 to
+// 4000 tokens, 32/8 heads of 96: 98 us, a warp per row and head took 4968).
+template <bool F16, int D, bool PADDED>
 __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_kernel(AttendArgs a) {
+    const int head = PADDED ? a.cache.head_dim : D;
     constexpr int THREADS = AR_WARPS * 32, QC = D / 32, VC = D / 64;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
@@ -363,13 +407,21 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
             if (lane == 0) there[(i & 2) >> 1] = b;
             __syncwarp();
         };
+        auto copy_lines = [&](uint32_t dst, const uint16_t *src, bool there) {
+            if (!PADDED) {
+                copies16<D / 64, 128, 128>(dst, src, there ? 16 : 0);
+            } else {
+                copy16<0, 0>(dst, src, there && 8 * cp < head ? 16 : 0);
+                if (D > 64) copy16<128, 128>(dst, src, there && 64 + 8 * cp < head ? 16 : 0);
+            }
+        };
         auto load_k = [&](int i) {
             __syncwarp();  // the block that was here has been read
             if (i < tiles)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const long long o = places[(i & 3) * 16 + 4 * q + ck].x;
-                    copies16<D / 64, 128, 128>(copy_k + (i & 1) * AR_STAGE<D> + q * 8 * D, kbase + o, o < 0 ? 0 : 16);
+                    copy_lines(copy_k + (i & 1) * AR_STAGE<D> + q * 8 * D, kbase + o, o >= 0);
                 }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -379,7 +431,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const long long o = places[(i & 3) * 16 + 4 * q + ck].y;
-                    copies16<D / 64, 128, 128>(copy_v + piece_v[q & 1] + (i & 1) * AR_STAGE<D> + q * 8 * D, vbase + o, o < 0 ? 0 : 16);
+                    copy_lines(copy_v + piece_v[q & 1] + (i & 1) * AR_STAGE<D> + q * 8 * D, vbase + o, o >= 0);
                 }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -400,7 +452,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
         for (int c = warp; c < QC; c += AR_WARPS)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                qs[(c * 2 + i) * 32 + lane] = j[i] >= 0 ? *reinterpret_cast<const uint4 *>(qrow[i] + 32 * c + 8 * t4) : make_uint4(0, 0, 0, 0);
+                qs[(c * 2 + i) * 32 + lane] = j[i] >= 0 && (!PADDED || 32 * c + 8 * t4 < head) ? *reinterpret_cast<const uint4 *>(qrow[i] + 32 * c + 8 * t4) : make_uint4(0, 0, 0, 0);
         place(0, page0);
         load_k(0);
         load_v(0);
@@ -528,7 +580,8 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
                     }
                     if (o < 0) continue;  // (zeros)
 #pragma unroll
-                    for (int c = 0; c < VC; ++c)
+                    for (int c = 0; c < VC; ++c) {
+                        if (PADDED && 64 * c + 16 * t4 >= head) continue;
 #pragma unroll
                         for (int d = 0; d < 16; ++d) {
                             const uint32_t bitsv = (vbase - 8 * cp + o)[64 * c + 16 * t4 + d];
@@ -538,6 +591,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
                             for (int i2 = 0; i2 < 2; ++i2)
                                 if (w[i2] != 0.f) acc[c][d & 7][2 * i2 + (d >> 3)] += w[i2] * v;
                         }
+                    }
                 }
             }
             load_v(i + 2);
@@ -565,6 +619,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
         const bool whole = c0 == c1;
         float *part = parts + (long long)(2 * blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0)) * PART;
         auto store = [&](int row, int d, const float (&o)[4], float total_w) {
+            if (PADDED && d >= head) return;
             const float inv = total_w == 0.f ? 0.f : 1.f / total_w;
             uint16_t *dst = a.out + (long long)(rq.q0 + (row0 + row) / group) * a.o_row + (long long)(hk * group + (row0 + row) % group) * a.o_head + d;
             *reinterpret_cast<uint2 *>(dst) = make_uint2(pack16x2<F16>(o[0] * inv, o[1] * inv), pack16x2<F16>(o[2] * inv, o[3] * inv));
@@ -644,6 +699,10 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
 // only when a maximum has grown by more than 8 (powers of two), by the warp that finds it.
 // Weights are rounded to the rows' 16-bit type for the product, as they have to be for one tensor-core operand (their sum is
 // not): half a step per weight, independent from key to key.
+//
+// Measured, bf16, heads of 128: two trees of 64 over 32000 tokens, 64/8 heads, 163 us, 823 TFLOP/s; 16 trees of 8 to 32 over 300 to 6000
+// tokens, 32/8 heads, 58 us; four prompts of 512 behind 2000 to 4000 tokens, 32/8 heads, 153 us, 655 TFLOP/s.  Bound by how fast one CTA's
+// chain S -> weights -> O turns over (a tile of 64 keys takes some 1900 cycles, K and V from the L2 and the exponentials half of that).
 // =====================================================================================
 constexpr int AT_ROWS = 128, AT_TILE = 64, AT_THREADS = 8 * 32, AT_PER_SM = 2, AT_MAX_CTAS = 192 * AT_PER_SM, AT_COLS = 256;
 // A segment that begins in a CTA and goes on behind it: where it ends, and its rows.  The next launch joins its parts.
@@ -1310,16 +1369,24 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
     AttendArgs a{reinterpret_cast<const uint16_t *>(q), s[0], s[1], view, table, table_stride, lens, q_start, mask,
                  reinterpret_cast<uint16_t *>(out), s[2], s[3], scale * 1.4426950408889634f, R, T, n_heads, table_width,
                  view.page_size & (view.page_size - 1) ? -1 : __builtin_ctz(view.page_size), w.header, w.attention};
+    const bool f16 = cache->format == ACT_F16;
+    auto launch_rows = [&](auto kernel, int smem) {
+        if (int e = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "tree_attention shared memory")) return e;
+        const int grid = min(device_sm_count() * AR_PER_SM, AR_MAX_CTAS);
+        return check_cuda(launch_pdl(kernel, dim3(grid), dim3(AR_WARPS * 32), smem, as_stream(stream), a), "tree_attention launch");
+    };
     if (view.head_dim == 64 || view.head_dim == 128) {
-        const bool f16 = cache->format == ACT_F16;
-        // More rows than one mma.sync tile has, on average: tcgen05.
+        // More rows than one mma.sync tile has, on average: tcgen05.  32 requests of 2000 to 4000 tokens, 32/8 heads of 128, trees of 4 (16
+        // rows per head): mma.sync 79 us, tcgen05 88; trees of 8 (32 rows): 122 and 89.
         if ((long long)T * (n_heads / view.n_kv) > (long long)AR_ROWS * R) {
             auto kernel = view.head_dim == 64 ? (f16 ? tree_attention_tiles_kernel<true, 64> : tree_attention_tiles_kernel<false, 64>)
                                               : (f16 ? tree_attention_tiles_kernel<true, 128> : tree_attention_tiles_kernel<false, 128>);
             const int smem = (view.head_dim == 64 ? AT_SMEM<64> : AT_SMEM<128>) + (R + 1) * 8;
             if ((rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "tree_attention shared memory"))) return rc;
             const int grid = min(device_sm_count() * AT_PER_SM, AT_MAX_CTAS);
-            const int align = (long long)T * (n_heads / view.n_kv) > (long long)AT_ROWS * R ? 100 : 0;  // MB of keys
+            // Segments in step (see there), MB of keys: two trees of 64 over 32000 tokens, 64/8 heads of 128 (262 MB), 171 us, 197 without;
+            // four prompts of 512 behind 2000 to 4000 (50 MB) 153 either way.
+            const int align = (long long)T * (n_heads / view.n_kv) > (long long)AT_ROWS * R ? 100 : 0;
             // boxes of slots that never straddle a page or a tile
             int box = AT_TILE;
             while (box >= 8 && view.page_size % box) box >>= 1;
@@ -1343,15 +1410,15 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
                                             : (f16 ? tree_attention_join_kernel<true, 128> : tree_attention_join_kernel<false, 128>);
             return check_cuda(launch_pdl(join, dim3(grid, view.head_dim / AJ_COLS), dim3(AT_ROWS), 0, as_stream(stream), a), "tree_attention join launch");
         }
-        auto kernel = view.head_dim == 64 ? (f16 ? tree_attention_rows_kernel<true, 64> : tree_attention_rows_kernel<false, 64>)
-                                          : (f16 ? tree_attention_rows_kernel<true, 128> : tree_attention_rows_kernel<false, 128>);
-        const int smem = (view.head_dim == 64 ? AR_SMEM<64> : AR_SMEM<128>);
-        if ((rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "tree_attention shared memory"))) return rc;
-        const int grid = min(device_sm_count() * AR_PER_SM, AR_MAX_CTAS);
-        return check_cuda(launch_pdl(kernel, dim3(grid), dim3(AR_WARPS * 32), smem, as_stream(stream), a), "tree_attention launch");
+        return launch_rows(view.head_dim == 64 ? (f16 ? tree_attention_rows_kernel<true, 64, false> : tree_attention_rows_kernel<false, 64, false>)
+                                               : (f16 ? tree_attention_rows_kernel<true, 128, false> : tree_attention_rows_kernel<false, 128, false>),
+                           view.head_dim == 64 ? AR_SMEM<64> : AR_SMEM<128>);
     }
-    const long long items = (long long)T * n_heads;
-    AWQ_REQUIRE((items + 3) / 4 <= 0x7fffffffLL, "tree_attention: too many rows and heads");
-    auto kernel = cache->format == ACT_F16 ? tree_attention_any_kernel<true> : tree_attention_any_kernel<false>;
-    return check_cuda(launch_pdl(kernel, dim3((unsigned)((items + 3) / 4)), dim3(128), 0, as_stream(stream), a), "tree_attention launch");
+    if (view.head_dim < 128)
+        return launch_rows(view.head_dim < 64 ? (f16 ? tree_attention_rows_kernel<true, 64, true> : tree_attention_rows_kernel<false, 64, true>)
+                                              : (f16 ? tree_attention_rows_kernel<true, 128, true> : tree_attention_rows_kernel<false, 128, true>),
+                           view.head_dim < 64 ? AR_SMEM<64> : AR_SMEM<128>);
+    AWQ_REQUIRE((long long)T * n_heads <= 0x7fffffffLL, "tree_attention: too many rows and heads");
+    auto kernel = f16 ? tree_attention_any_kernel<true> : tree_attention_any_kernel<false>;
+    return check_cuda(launch_pdl(kernel, dim3((unsigned)(T * n_heads)), dim3(AA_WARPS * 32), 0, as_stream(stream), a), "tree_attention launch");
 }

@@ -47,6 +47,41 @@ def test_other_head_sizes(D, dtype):
     run([37, 0, 70], [1, 3, 6], 4, 2, D, 16, dtype, tree=True)
 
 
+@pytest.mark.parametrize("D", [16, 32, 96, 112, 144, 208, 256])
+@pytest.mark.parametrize("lens,new", [([5000], [1]), ([700, 0, 33, 129], [1, 64, 0, 17]), ([0, 3], [70, 1])])
+def test_other_head_sizes_over_long_contexts(D, lens, new):
+    run(lens, new, 8, 2, D, 16, FP if D % 32 else BF, tree=max(new) <= 64, empty=0.1)
+
+
+@pytest.mark.parametrize("D,wide", [(48, 64), (96, 104), (112, 128), (160, 168)])
+def test_columns_behind_a_head_are_left(D, wide):
+    """Heads that are slices of wider rows: what lies behind them is not used (NaN) and not written (7)."""
+    from mlir_air_b200 import ops
+    lens, new, H, kv, page = [70, 5, 0], [3, 20, 1], 4, 2, 8
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    table, pages = make_table([l + n for l, n in zip(lens, new)], page, 3)
+    wide_of = lambda *s: torch.full((*s, wide), float("nan"), device="cuda", dtype=BF)  # noqa: E731
+    k, v, q = wide_of(pages, page, kv)[..., :D], wide_of(pages, page, kv)[..., :D], wide_of(sum(new), H)[..., :D]
+    for x in (k, v, q):
+        x.copy_(torch.randn(x.shape, device="cuda", generator=gen))
+    mask, ws = random_masks(new, 3), ops.RequestWorkspace()
+    k[table[1, 1], 0, 0, 3], v[table[1, 1], 2, 1, 5] = 3.0, float("inf")  # (a drafted token that some rows see: infinite for them only)
+    into = torch.full((sum(new), H, wide), 7.0, device="cuda", dtype=BF)
+    ops.tree_attention(q, ops.KVCache(k, v), table, i32(lens), i32(starts(new)), ws, mask=mask, out=into[..., :D])
+    ws.check()
+    assert bool((into[..., D:] == 7).all())
+    out = into[..., :D]
+    j = (int(table[1, 1]), 8 + 2 - lens[1])  # its page, and its place among the request's new tokens
+    sees = ((mask[3:23] >> j[1]) & 1).bool()
+    rows = torch.arange(3, 23, device="cuda")
+    assert bool(torch.isinf(out[rows[sees]][:, 2:, 5]).all()) and 0 < int(sees.sum()) < 20
+    out[rows[sees], 2:, 5] = 0
+    v[j[0], 2, 1, 5] = 0
+    ref, tol = attend_ref(q, k, v, table, lens, new, mask, D ** -0.5)
+    ref[rows[sees], 2:, 5] = 0
+    assert bool(((out.double() - ref).abs() <= tol).all())
+
+
 @pytest.mark.parametrize("page", [1, 3, 8, 16, 64, 128, 1000])
 @pytest.mark.parametrize("D", [64, 128])
 def test_pages(page, D):
