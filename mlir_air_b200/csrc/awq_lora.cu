@@ -140,6 +140,11 @@ __device__ __forceinline__ void lora_store(const LoraArgs &a, long long at, cons
 // first pieces are on their way before the sums meet.  Every CTA puts the rows in order for itself (a few hundred comparisons a
 // thread), which is cheaper than a launch in front.  How many tiles there are only the device knows: as many clusters as run at
 // once go through them, and where the tiles are few, several share a tile's columns and each forms x A^T for itself.
+//
+// Measured: 4 rows on adapters of rank 16, K = N = 2048, 5.5 us, most of it the launch and two passes of latency; 64 rows on 64 adapters of
+// rank 16, K = N = 4096, 18 us; 64 on 64 of rank 64, K = N = 8192, 40 us (134 MB of adapters, 3.4 TB/s).
+// LORA_FEW, one launch against three, K = N = 4096, in us: 128 rows on 8 adapters of rank 16 9.9 and 11.5, on 64 20.8 and 26.2; 256 rows on 8 adapters
+// 14.6 and 12.5, on 64 27.9 and 27.0.
 // =====================================================================================
 constexpr int LORA_FEW = 128, LF_WARPS = 8, LF_CLUSTER = 8;
 
@@ -278,6 +283,10 @@ __global__ void __cluster_dims__(LF_CLUSTER, 1, 1) __launch_bounds__(LF_WARPS * 
 // Many rows, three launches: rows by adapter into tiles of 64; x A^T of a tile by a cluster of eight CTAs (an eighth of K each,
 // the sums meeting in distributed shared memory); and the columns of B, 64 rows x 256 columns a CTA, which is where the bytes
 // of base and out go by.
+//
+// Measured, 9 prompts of 3583 rows together, K 4096, N 14336, 7 adapters of rank 8 to 64: 79 us (3.1 TB/s; 37 us for the bytes alone).  The
+// columns of B take most of it, and in there the instructions of a row: unpacking base, two products per 16 ranks, rounding, 16-byte stores.
+// Base by asynchronous copies with 16 warps (102 us) and through shared memory in whole lines (89) were slower.
 // =====================================================================================
 constexpr int LM_ROWS = 64, LM_MT = LM_ROWS / 16, LG_THREADS = 1024, LD_WARPS = 8, LU_WARPS = 4;
 constexpr int LORA_MAX_TILES = (LORA_MAX_ROWS + LM_ROWS - 1) / LM_ROWS + LORA_MAX_ADAPTERS + 1;
