@@ -483,7 +483,7 @@ int awq_b200_page_plan(const int32_t *lens, const int32_t *fresh, int32_t *table
 
 /* Half-split RoPE (as awq_b200_rope_halfsplit_bf16) of Q and K by row positions[t] of lut bf16 [n_positions, head_dim], K and V
  * into slot slots[t] of the cache (-1: the row is left out).  A slot that several rows name keeps the last of them.
- * q_out may be q.  Rows and cache share one format. */
+ * q_out may be q (same strides), but not overlap it otherwise.  Rows and cache share one format. */
 int awq_b200_rope_append(const void *q, long long q_row_stride, long long q_head_stride, const void *k, long long k_row_stride,
                          long long k_head_stride, const void *v, long long v_row_stride, long long v_head_stride, const uint16_t *lut,
                          int n_positions, const int32_t *positions, const int32_t *slots, void *q_out, long long q_out_row_stride,
@@ -493,7 +493,7 @@ int awq_b200_rope_append(const void *q, long long q_row_stride, long long q_head
 /* out[t, h] = softmax over the keys row t sees of scale q[t, h] . k, times v; heads in groups of n_heads / n_kv_heads share a cache
  * head.  A row sees its request's lens[r] cached tokens and of the step's tokens of its request token j if bit j of mask[t] is set
  * (int64 [T], up to 64 tokens per request), or, without `mask`, those up to itself (any number).  A row that sees nothing is 0;
- * rows behind the last request are left as they are. */
+ * rows behind the last request are left as they are.  out may be q (same strides), but not overlap it otherwise. */
 int awq_b200_tree_attention(const void *q, long long q_row_stride, long long q_head_stride, const awq_b200_kv_cache_t *cache,
                             const int32_t *table, long long table_stride, int table_width, const int32_t *lens, const int32_t *q_start,
                             const long long *mask, float scale, void *out, long long out_row_stride, long long out_head_stride, int R, int T,
@@ -514,7 +514,7 @@ int awq_b200_page_keep(void *kv, long long layer_stride, long long kv_stride, lo
 /* out bf16 [T, N] = bf16(base + scales[a] (x A[a]^T) B[a]^T (+ residual)), a = idx[t] per row (-1: base alone): low-rank adapters
  * beside a shared projection, whose f32 sums (awq_b200_gemv_f32 and the like) or bf16 output `base` is.  A bf16 [n, rank_max, K],
  * B bf16 [n, N, rank_max], of which adapter a uses ranks[a] rows / columns (NULL: all); rank_max a multiple of 8 up to 128, K and N
- * multiples of 8, T <= 65535.  out may be a bf16 base; base and residual are [T, N]. */
+ * multiples of 8, T <= 65535.  base and residual are [T, N]; out may be a bf16 base or the residual, other overlaps are refused. */
 int awq_b200_lora_bf16(const uint16_t *x, long long x_row_stride, const uint16_t *A, const uint16_t *B, const float *scales,
                        const int32_t *ranks, int n_adapters, int rank_max, const int32_t *idx, const void *base, int base_is_f32,
                        const uint16_t *residual, uint16_t *out, int T, int K, int N, void *workspace, size_t workspace_bytes,

@@ -620,6 +620,16 @@ extern "C" int awq_b200_lora_bf16(const uint16_t *x, long long x_row_stride, con
     AWQ_REQUIRE(aligned16(x) && aligned16(A) && aligned16(B) && aligned16(base) && aligned16(residual) && aligned16(out),
                 "lora: pointers must be 16-byte aligned");
     AWQ_REQUIRE_REQUEST_WORKSPACE("lora", workspace, workspace_bytes);
+    // CTAs read all of x, A and B, and each the base and residual of the elements that it writes.
+    auto apart = [&](const void *p, long long elements, int size) {
+        const uintptr_t from = reinterpret_cast<uintptr_t>(p), to = reinterpret_cast<uintptr_t>(out);
+        return !p || from + (uintptr_t)elements * size <= to || to + 2 * (uintptr_t)T * N <= from;
+    };
+    const long long whole = (long long)T * N;
+    AWQ_REQUIRE(apart(x, (T - 1) * x_row_stride + K, 2) && apart(A, (long long)n_adapters * rank_max * K, 2) && apart(B, (long long)n_adapters * rank_max * N, 2),
+                "lora: out must not overlap x or the adapters");
+    AWQ_REQUIRE((!base_is_f32 && base == out) || apart(base, whole, base_is_f32 ? 4 : 2), "lora: out may be a bf16 base, but not overlap base otherwise");
+    AWQ_REQUIRE(residual == out || apart(residual, whole, 2), "lora: out may be the residual, but not overlap it otherwise");
     const RequestWorkspaceView w = request_workspace(workspace);
     LoraArgs a{};
     a.x = x, a.A = A, a.B = B, a.scales = scales, a.ranks = ranks, a.idx = idx, a.base = base, a.residual = residual, a.out = out;

@@ -668,7 +668,7 @@ def tree_attention(q, cache: KVCache, table, lens, q_start, ws: RequestWorkspace
     """out [T, n_heads, head_dim]: the step's rows q against their requests' cached tokens and the step's own (whose K and V
     are in the cache already: `rope_append`).  Row t of request r sees its lens[r] cached tokens and token j of the step if bit
     j of mask[t] (int64) is set, or without `mask` the tokens up to itself.  A row that sees nothing is 0.  Rows behind
-    q_start[R] are left as they are in a given `out`, 0 in a new one.  scale: head_dim ** -0.5 unless given."""
+    q_start[R] are left as they are in a given `out` (which may be q), 0 in a new one.  scale: head_dim ** -0.5 unless given."""
     dev = cache.device
     if ws.device != dev:
         raise _lib.AwqBackendError("tree_attention: workspace and cache must be on one device")
@@ -749,7 +749,7 @@ class LoraAdapters:
 
 def lora(x, adapters: LoraAdapters, idx, base, ws: RequestWorkspace, out=None, residual=None):
     """out bf16 [T, N] = bf16(base + scale (x A^T) B^T (+ residual)) with adapter idx[t] for row t of x bf16 [T, K], -1: none.  base is
-    the shared projection's output, f32 sums (`gemv(..., f32_out=True)`) or bf16; out may be a bf16 base."""
+    the shared projection's output, f32 sums (`gemv(..., f32_out=True)`) or bf16; out may be a bf16 base or the residual, not x."""
     dev = ws.device
     if adapters.device != dev:
         raise _lib.AwqBackendError("lora: workspace and adapters must be on one device")

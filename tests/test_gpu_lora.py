@@ -88,6 +88,19 @@ def test_in_place_and_strides():
     ws.check()
 
 
+@pytest.mark.parametrize("T", [5, 140])
+def test_the_residual_may_be_overwritten(T):
+    from mlir_air_b200 import ops
+    x, A, B, s, rk, base = make(T, 512, 512, 3, 16, [16, 3, 8])
+    res, ws = torch.randn((T, 512), device="cuda").to(BF), ops.RequestWorkspace()
+    args = (x, ops.LoraAdapters(A, B, s, rk), i32([t % 4 - 1 for t in range(T)]), base, ws)
+    want = ops.lora(*args, residual=res)
+    assert ops.lora(*args, residual=res, out=res) is res and torch.equal(res, want)
+    with pytest.raises(Exception, match="overlap"):
+        ops.lora(*args, out=x)
+    ws.check()
+
+
 def test_beside_an_int4_projection():
     """gemv's f32 sums, then the adapters and the residual with one rounding: what a decode layer with adapters computes."""
     import numpy as np

@@ -207,6 +207,19 @@ def test_rows_behind_the_last_request_are_left():
     ws.check()
 
 
+@pytest.mark.parametrize("D,new,lens", [(64, (1, 3), (2000, 9)), (128, (40, 64), (900, 30)), (96, (5, 1), (700, 3)), (160, (4, 1), (300, 3))])
+def test_the_rows_may_be_overwritten(D, new, lens):
+    from mlir_air_b200 import ops
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    table, pages = make_table([l + n for l, n in zip(lens, new)], 16, 5)
+    k, v = (torch.randn((pages, 16, 2, D), device="cuda", generator=gen).to(BF) for _ in range(2))
+    q = torch.randn((sum(new), 8, D), device="cuda", generator=gen).to(BF)
+    args, ws = (ops.KVCache(k, v), table, i32(lens), i32(starts(new))), ops.RequestWorkspace()
+    want = ops.tree_attention(q, *args, ws)
+    assert ops.tree_attention(q, *args, ws, out=q) is q and torch.equal(q, want)
+    ws.check()
+
+
 def test_the_same_bits_every_time():
     from mlir_air_b200 import ops
     for new, lens in (((1,) * 5, (3000, 10, 700, 64, 9000)), ((64, 20), (5000, 800))):

@@ -123,6 +123,15 @@ def test_lora():
     assert lora(T=0) == 0 and lora(N=0) == 0
 
 
+def test_lora_refuses_outputs_over_inputs():
+    at = lambda n: ctypes.c_void_p(4096 + n)  # noqa: E731
+    far, x, out = 1 << 24, 4 * 512 * 2 + 512 * 2, 5 * 256 * 2  # bytes of x and out
+    apart = dict(x=at(far), A=at(2 * far), B=at(3 * far), base=at(4 * far), res=at(5 * far), out=at(6 * far))
+    for bad in (dict(out=at(far)), dict(out=at(far + x - 16)), dict(out=at(far - out + 16)), dict(out=at(2 * far + 3 * 16 * 512 * 2 - 16)), dict(out=at(3 * far)),
+                dict(out=at(4 * far)), dict(out=at(4 * far + 2 * out - 16)), dict(f32=0, out=at(4 * far + 16)), dict(out=at(5 * far + 16))):
+        err(lora(**{**apart, **bad}), text="overlap")
+
+
 def test_handles_refuse_host_tensors():
     torch = pytest.importorskip("torch")
     from mlir_air_b200 import ops
