@@ -218,6 +218,13 @@ __device__ __forceinline__ bool not_finite16x2(uint32_t v) {
     return (v & e) == e || ((v >> 16) & e) == e;
 }
 
+// acc + 0 v for two 16-bit values: not a number once v was infinite or none.
+template <bool F16>
+__device__ __forceinline__ uint32_t at_zero_fma(uint32_t v, uint32_t acc) {
+    if (F16) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0u));
+    else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0u));
+    return acc;
+}
 // Of the block's threads before this one, and of all.
 template <int THREADS>
 __device__ __forceinline__ long long exclusive_sum(long long mine, long long &total) {
@@ -543,8 +550,16 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
             __syncwarp();
             bool odd = false;
             if (partly) {  // a value that some rows do not see must not reach them as 0 times infinity or NaN
+                uint32_t zeros[4] = {};
+#pragma unroll
+                for (int w = 0; w < 4 * VC; ++w) {  // (the pieces this lane reads below)
+                    const uint4 u = *reinterpret_cast<const uint4 *>(vs + (w & 1) * 2 * D + (w >> 1 & 1) * 16 * D + (w >> 2) * 128);
+                    zeros[0] = at_zero_fma<F16>(u.x, zeros[0]), zeros[1] = at_zero_fma<F16>(u.y, zeros[1]);
+                    zeros[2] = at_zero_fma<F16>(u.z, zeros[2]), zeros[3] = at_zero_fma<F16>(u.w, zeros[3]);
+                }
+                const bool any = not_finite16x2<F16>(zeros[0]) || not_finite16x2<F16>(zeros[1]) || not_finite16x2<F16>(zeros[2]) || not_finite16x2<F16>(zeros[3]);
 #pragma unroll 1
-                for (int w = 0; w < 16 * VC; ++w) {  // (the pieces this lane reads below)
+                for (int w = 0; any && w < 16 * VC; ++w) {
                     uint32_t &u = reinterpret_cast<uint32_t *>(const_cast<uint8_t *>(vs) + (w >> 2 & 1) * 2 * D + (w >> 3 & 1) * 16 * D + (w >> 4) * 128)[w & 3];
                     if (!not_finite16x2<F16>(u)) continue;
                     odd = true;
@@ -849,13 +864,6 @@ __device__ __forceinline__ void at_copy_keys(uint32_t dst0, uint32_t dst1, const
     }
 }
 
-// acc + 0 v for two 16-bit values: not a number once v was infinite or none.
-template <bool F16>
-__device__ __forceinline__ uint32_t at_zero_fma(uint32_t v, uint32_t acc) {
-    if (F16) asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0u));
-    else asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(v), "r"(0u));
-    return acc;
-}
 template <bool F16, int D>
 __device__ __noinline__ void at_clean_values(uint8_t *mine, int from, int row, int *odd) {
 #pragma unroll 1
