@@ -184,9 +184,9 @@ __global__ void __launch_bounds__(AA_WARPS * 32) tree_attention_any_kernel(Atten
 // Weights are multiplied as two 16-bit pieces, p = hi + lo: the tensor cores have time to spare, and the result keeps the
 // accuracy of f32 weights.
 //
-// Measured, bf16, heads of 128: one token of 64 requests of 1000 to 16000, 64/8 heads, 263 us, 5.85 TB/s (89 % of a copy's rate; keys
-// straight to registers 389); one token of 256 requests of 500 to 2000, 32/8 heads, 205 us, 5.6 TB/s.  Small steps are a chain of
-// latencies: starts and lengths, pages, keys, the join (one token behind 777, 32/8 heads of 64: 10 us).
+// Measured, bf16, heads of 128: one token of 64 requests of 1000 to 16000, 64/8 heads, 261 us, 5.9 TB/s (90 % of a copy's rate; keys
+// straight to registers 389); one token of 256 requests of 500 to 2000, 32/8 heads, 196 us, 5.9 TB/s.  Small steps are a chain of
+// latencies: starts and lengths, pages, keys, the join (one token behind 777, 32/8 heads of 64: 9.6 us).
 // =====================================================================================
 constexpr int AR_WARPS = 4, AR_TILE = AR_WARPS * 16, AR_PER_SM = 3, AR_ROWS = 16;
 constexpr int AR_MAX_CTAS = 192 * AR_PER_SM;
@@ -294,7 +294,7 @@ constexpr int AR_SMEM = D * 32 + AR_WARPS * AR_PLACES + AR_STAGES<D> + AR_CUM;
 static_assert(AR_SMEM<128> + 64 <= 224 * 1024 / AR_PER_SM - 1024, "three CTAs an SM (76096 bytes a CTA measured two)");
 
 // PADDED: heads of other sizes below D; what lies behind them is 0 in shared memory and neither read nor written (64 requests of 500 to
-// 4000 tokens, 32/8 heads of 96: 98 us, a warp per row and head took 4968).
+// 4000 tokens, 32/8 heads of 96: 92 us, a warp per row and head took 4968).
 template <bool F16, int D, bool PADDED>
 __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_kernel(AttendArgs a) {
     const int head = PADDED ? a.cache.head_dim : D;
@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
 // Weights are rounded to the rows' 16-bit type for the product, as they have to be for one tensor-core operand (their sum is
 // not): half a step per weight, independent from key to key.
 //
-// Measured, bf16, heads of 128: two trees of 64 over 32000 tokens, 64/8 heads, 163 us, 823 TFLOP/s; 16 trees of 8 to 32 over 300 to 6000
+// Measured, bf16, heads of 128: two trees of 64 over 32000 tokens, 64/8 heads, 163 to 174 us, 770 to 820 TFLOP/s; 16 trees of 8 to 32 over 300 to 6000
 // tokens, 32/8 heads, 58 us; four prompts of 512 behind 2000 to 4000 tokens, 32/8 heads, 153 us, 655 TFLOP/s.  Bound by how fast one CTA's
 // chain S -> weights -> O turns over (a tile of 64 keys takes some 1900 cycles, K and V from the L2 and the exponentials half of that).
 // =====================================================================================
@@ -1385,7 +1385,7 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
     };
     if (view.head_dim == 64 || view.head_dim == 128) {
         // More rows than one mma.sync tile has, on average: tcgen05.  32 requests of 2000 to 4000 tokens, 32/8 heads of 128, trees of 4 (16
-        // rows per head): mma.sync 79 us, tcgen05 88; trees of 8 (32 rows): 122 and 89.
+        // rows per head): mma.sync 79 us, tcgen05 89; trees of 8 (32 rows): 118 and 90.
         if ((long long)T * (n_heads / view.n_kv) > (long long)AR_ROWS * R) {
             auto kernel = view.head_dim == 64 ? (f16 ? tree_attention_tiles_kernel<true, 64> : tree_attention_tiles_kernel<false, 64>)
                                               : (f16 ? tree_attention_tiles_kernel<true, 128> : tree_attention_tiles_kernel<false, 128>);
