@@ -463,7 +463,7 @@ size_t awq_b200_request_workspace_bytes(void);
 int awq_b200_request_check(void *workspace, awq_stream_t stream);
 
 /* K and V of one layer: [n_pages, page_size, n_kv_heads, head_dim], bf16 or fp16 (AWQ_ACT_*), any strides that are
- * multiples of 8 elements, the head_dim values of a head side by side. */
+ * multiples of 8 elements (0 for a dimension of one only), the head_dim values of a head side by side. */
 typedef struct {
     const void *k, *v;
     long long k_page_stride, k_slot_stride, k_head_stride, v_page_stride, v_slot_stride, v_head_stride;

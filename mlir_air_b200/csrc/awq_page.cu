@@ -16,6 +16,9 @@ int check_kv_cache(const char *who, const awq_b200_kv_cache_t *c, KvCacheView *o
     AWQ_REQUIRE(aligned16(c->k) && aligned16(c->v), "%s: the cache must be 16-byte aligned", who);
     const long long s[6] = {c->k_page_stride, c->k_slot_stride, c->k_head_stride, c->v_page_stride, c->v_slot_stride, c->v_head_stride};
     for (long long v : s) AWQ_REQUIRE(v >= 0 && v % 8 == 0, "%s: cache strides must be multiples of 8 elements", who);
+    // (the stride of a dimension of one is never used; a box of a tensor map cannot have one of 0)
+    const int n[3] = {c->n_pages, c->page_size, c->n_kv_heads};
+    for (int i = 0; i < 6; ++i) AWQ_REQUIRE(s[i] > 0 || n[i % 3] == 1, "%s: a cache stride of 0 needs a dimension of one", who);
     *out = KvCacheView{reinterpret_cast<const uint16_t *>(c->k), reinterpret_cast<const uint16_t *>(c->v), s[0], s[1], s[2], s[3], s[4], s[5],
                        c->n_pages, c->page_size, c->n_kv_heads, c->head_dim};
     return AWQ_OK;

@@ -77,6 +77,18 @@ def test_rope_append():
     assert append(c, T=0) == 0
 
 
+def test_cache_strides_of_zero():
+    """A dimension of one may come with any stride, 0 among them; a longer one may not repeat the same values: what brings whole boxes of the
+    cache would read them from elsewhere."""
+    for bad in (dict(k_head_stride=0), dict(v_head_stride=0), dict(k_slot_stride=0), dict(v_slot_stride=0), dict(k_page_stride=0), dict(v_page_stride=0)):
+        b, keep2 = cache(**bad)
+        err(attend(b), text="stride")
+        err(append(b), text="stride")
+    ones = dict(n_pages=1, page_size=1, n_kv_heads=1, k_page_stride=0, v_page_stride=0, k_slot_stride=0, v_slot_stride=0, k_head_stride=0, v_head_stride=0)
+    b, keep2 = cache(**ones)
+    assert attend(b, R=0) == 0 and append(b, T=0) == 0
+
+
 def plan(**change):
     a = dict(lens=P, new=P, table=P, stride=4, width=4, free=P, pool=10, count=P, count_out=P, parents=None, page=16, start=P, slots=P, pos=P, mask=None,
              R=2, T=5, ws=P, nbytes=BIG, stream=None)
