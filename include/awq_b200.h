@@ -451,7 +451,8 @@ int awq_b200_rope_halfsplit_bf16(const uint16_t *x, size_t x_stride, const uint1
  * A step works on T rows: the new tokens of R requests, one request after another, request r's rows being
  * q_start[r] .. q_start[r + 1].  Its K and V lie in pages of page_size slots; token p of request r is in slot
  * table[r][p / page_size] * page_size + p % page_size.  `lens` counts the tokens a request had before the step; the
- * step's own tokens follow them.  R <= 4096, T <= 2^20, a cache has less than 2^31 slots; strides are in elements.
+ * step's own tokens follow them.  R <= 4096, T <= 2^20, a cache has less than 2^31 slots; strides are in elements, those
+ * of what is written 0 for a dimension of one only.
  *
  * Lengths, pages, slots and adapters live on the device, where the host cannot check them: a kernel that meets one
  * outside its buffers skips the access and sets a bit in the workspace's error word, which awq_b200_request_check

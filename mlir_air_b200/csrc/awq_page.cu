@@ -454,6 +454,7 @@ extern "C" int awq_b200_rope_append(const void *q, long long q_row_stride, long 
     const long long s[8] = {q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride, q_out_row_stride, q_out_head_stride};
     for (long long x : s) AWQ_REQUIRE(x >= 0 && x % 8 == 0, "rope_append: strides must be multiples of 8 elements");
     if (T == 0) return AWQ_OK;
+    AWQ_REQUIRE((T == 1 || q_out_row_stride > 0) && (n_heads <= 1 || q_out_head_stride > 0), "rope_append: an output stride of 0 needs a dimension of one");
     AWQ_REQUIRE(q && k && v && lut && positions && slots && q_out, "rope_append: null pointer");
     AWQ_REQUIRE(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(lut) && aligned16(q_out), "rope_append: pointers must be 16-byte aligned");
     AWQ_REQUIRE_REQUEST_WORKSPACE("rope_append", workspace, workspace_bytes);
@@ -481,6 +482,8 @@ extern "C" int awq_b200_page_keep(void *kv, long long layer_stride, long long kv
     AWQ_REQUIRE(free_count && free_count_out, "page_keep: null pointer");
     AWQ_REQUIRE(R == 0 || (table && lens && lens_out && q_start && kept && free_pages), "page_keep: null pointer");
     AWQ_REQUIRE(!path || kv, "page_keep: a path needs the cache");
+    const int n[5] = {layers, 2, n_pages, page_size, n_kv_heads};
+    for (int i = 0; path && i < 5; ++i) AWQ_REQUIRE(s[i] > 0 || n[i] <= 1, "page_keep: a stride of 0 needs a dimension of one");
     AWQ_REQUIRE(aligned16(kv), "page_keep: the cache must be 16-byte aligned");
     AWQ_REQUIRE_REQUEST_WORKSPACE("page_keep", workspace, workspace_bytes);
     KeepArgs a{reinterpret_cast<uint16_t *>(kv), s[0], s[1], s[2], s[3], s[4], table, table_stride, lens, q_start, kept, path, lens_out, free_pages,

@@ -1370,6 +1370,7 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
     const long long s[4] = {q_row_stride, q_head_stride, out_row_stride, out_head_stride};
     for (long long x : s) AWQ_REQUIRE(x >= 0 && x % 8 == 0, "tree_attention: strides must be multiples of 8 elements");
     if (R == 0 || T == 0) return AWQ_OK;
+    AWQ_REQUIRE((T == 1 || out_row_stride > 0) && (n_heads == 1 || out_head_stride > 0), "tree_attention: an output stride of 0 needs a dimension of one");
     AWQ_REQUIRE(q && out && table && lens && q_start, "tree_attention: null pointer");
     AWQ_REQUIRE(aligned16(q) && aligned16(out), "tree_attention: pointers must be 16-byte aligned");
     AWQ_REQUIRE_REQUEST_WORKSPACE("tree_attention", workspace, workspace_bytes);

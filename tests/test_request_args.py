@@ -153,3 +153,16 @@ def test_handles_refuse_host_tensors():
         ops.LoraAdapters(torch.zeros(1, 8, 64, dtype=torch.bfloat16), torch.zeros(1, 64, 8, dtype=torch.bfloat16), torch.ones(1))
     with pytest.raises(_lib.AwqBackendError):
         ops.RequestWorkspace(device="cpu")
+
+
+def test_written_strides_of_zero():
+    """Rows, heads or layers that are written must not lie on top of one another: which of them stays would be chance."""
+    c, keep2 = cache()
+    err(attend(c, orow=0), text="stride")
+    err(attend(c, oh=0), text="stride")
+    err(append(c, orow=0), text="stride")
+    err(append(c, oh=0), text="stride")
+    assert attend(c, orow=0, T=0) == 0 and append(c, orow=0, T=0) == 0
+    for bad in ("s0", "s1", "s2", "s3", "s4"):
+        err(keep(**{bad: 0}), text="stride")
+    err(keep(s1=0, layers=1), text="stride")
