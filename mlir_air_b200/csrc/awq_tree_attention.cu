@@ -734,7 +734,7 @@ struct AttendTilesShared {
     // not ready for the product yet.
     uint64_t k_full[2], v_full[2], scored[2], added[4], weighed[2], q_full, q_free, summed, v_landed;
     uint32_t tmem;
-    int odd[2], pad;
+    int odd[4], pad;                       // a segment's: values that are not finite were taken out of V
     uint64_t found[4];                     // mbarriers: a segment's description is there
     AttendSegment segments[4];             // (no tiles: the last one is over)
     unsigned long long bits[2][AT_ROWS];   // of a segment's rows: their tokens' masks
@@ -933,7 +933,6 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
         mbar_init(smem_u32(&sh.v_landed), 1);
         for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&sh.found[i]), 1);
         mbar_fence_init();
-        sh.odd[0] = sh.odd[1] = 0;
     }
     pdl_wait();
     pdl_launch_dependents();
@@ -1039,7 +1038,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
                     // A weight of 0 must not meet infinity or NaN: slots without a token become 0, and of new tokens, which some rows do
                     // not see, what is not finite; it is added where it is seen, at the end.
                     if (!(ok = mbar_wait_bounded_warp(landed, cleaned++ & 1, limit))) break;
-                    at_clean<F16, D>(vs + (n & 1) * AT_OPERAND<D>, valid, seen_by_all(g) - key0, lane, &sh.odd[seg & 1]);
+                    at_clean<F16, D>(vs + (n & 1) * AT_OPERAND<D>, valid, seen_by_all(g) - key0, lane, &sh.odd[seg & 3]);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar_of(v_full, n));
@@ -1079,7 +1078,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 __syncwarp();
                 if (is_v && (key0 + AT_TILE > seen_by_all(g) || (valid[0] & valid[1]) != 0xffffffffu))
-                    at_clean<F16, D>(vs + (n & 1) * AT_OPERAND<D>, valid, seen_by_all(g) - key0, lane, &sh.odd[seg & 1]);
+                    at_clean<F16, D>(vs + (n & 1) * AT_OPERAND<D>, valid, seen_by_all(g) - key0, lane, &sh.odd[seg & 3]);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_of(is_v ? v_full : k_full, n));
@@ -1092,8 +1091,10 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
         for (int seg = 0; ok; ++seg) {
             const bool more = walk.next(g, per);
             if (!more) g.tiles = 0;
-            // (its place was that of segment seg - 4; the scores of seg - 2 are there, so that everybody is behind seg - 3)
+            // (Its place was that of segment seg - 4.  The scores of seg - 2 are there, so that all of seg - 3 has been weighed: everybody has its
+            // description, and nobody is still with seg - 4.)
             if (lane == 0) {
+                sh.odd[seg & 3] = 0;  // (read for seg - 4 before anything of seg - 3 was weighed)
                 sh.segments[seg & 3] = g;
                 mbar_arrive(smem_u32(&sh.found[seg & 3]));
             }
@@ -1245,7 +1246,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
             // ---- the segment's sums: out, or to the CTA that joins them ----
             const int c0 = g.c0, c1 = g.c1;
             const bool whole = c0 == c1;
-            const bool odd = *reinterpret_cast<volatile int *>(&sh.odd[seg & 1]) != 0;
+            const bool odd = *reinterpret_cast<volatile int *>(&sh.odd[seg & 3]) != 0;
             float *part = parts + (long long)(2 * blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0)) * PART;  // [D + 2][128]
             uint16_t *out = a.out + (long long)(g.q0 + j) * a.o_row + (long long)head * a.o_head;
             auto store32 = [&](int c, const float (&o)[32], float total) {
@@ -1289,7 +1290,6 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
             dg_fence_before();
             named_bar_sync(1, 128);
             if (tid == 0) {
-                sh.odd[seg & 1] = 0;
                 // what begins here and goes on is this CTA's last segment
                 if (!whole && (int)blockIdx.x == c0) joins[blockIdx.x] = AttendJoin{c1, g.q0, g.n, g.hk, g.m}, joined = true;
             }

@@ -21,7 +21,9 @@ class Bar:
         return self.phase % 2 != parity
 
 
-def run(segments, seed, rescale=0.5, tma=False):
+def run(segments, seed, rescale=0.5, tma=False, odd=0.0):
+    """odd: the share of tiles whose V holds what is not finite.  The warp that brings V takes it out and raises the segment's flag; the softmax
+    warps put it back where it is seen, which takes them a while, if they find the flag when the segment's sums are there."""
     rng = random.Random(seed)
     total = sum(segments)
     k_full, v_full, scored, weighed = ([Bar(1), Bar(1)] for _ in range(4))
@@ -29,6 +31,12 @@ def run(segments, seed, rescale=0.5, tma=False):
     segment_of = [i for i, t in enumerate(segments) for _ in range(t)]
     K, V, S, valid = [None] * 2, [None] * 2, [None] * 2, [None] * 4  # what each place holds
     queue, state = [], dict(q=None, o=None, weights={}, done=0)
+    flags, draw = [False] * 4, random.Random(-1 - seed)
+    raised = [odd > 0 and draw.random() < odd for _ in segment_of]  # by a tile
+
+    def clean(n):
+        if raised[n]:
+            flags[segment_of[n] % 4] = True
 
     def phase(t):
         return t >> 1 & 1
@@ -49,6 +57,8 @@ def run(segments, seed, rescale=0.5, tma=False):
                     valid[n % 4] = (n, "there")
                 yield None
                 place[n % 2] = (n, "there")
+                if is_v:
+                    clean(n)
                 (v_full if is_v else k_full)[n % 2].arrive()
                 n += 1
 
@@ -64,6 +74,7 @@ def run(segments, seed, rescale=0.5, tma=False):
         for seg in range(len(segments)):
             assert ring[seg % 4] is None or ring[seg % 4][1] == 4
             ring[seg % 4] = [seg, 0]
+            flags[seg % 4] = False
             found[seg % 4].arrive()
             yield None
             if seg:
@@ -88,9 +99,10 @@ def run(segments, seed, rescale=0.5, tma=False):
                 if not is_v:
                     assert valid[n % 4] is None or valid[n % 4][1] == "read"
                     valid[n % 4] = (n, "there")
-                if is_v and rng.random() < 0.3:
+                if is_v and (rng.random() < 0.3 or raised[n]):
                     yield None
                     place[n % 2] = (n, "there")
+                    clean(n)
                     v_full[n % 2].arrive()
                 else:
                     landing.append((place, n, v_full if is_v else k_full))
@@ -176,6 +188,9 @@ def run(segments, seed, rescale=0.5, tma=False):
                 n += 1
             yield summed, seg % 2
             assert state["o"] == n - 1
+            for _ in range(8 if odd else 0):  # (four warps, each in its time)
+                assert flags[seg % 4] == any(raised[n - tiles:n]), "a segment's flag lost, or another one's"
+                yield None
             yield None
             state["o"] = None
 
@@ -207,3 +222,11 @@ def run(segments, seed, rescale=0.5, tma=False):
 def test_no_schedule_deadlocks_or_overwrites(segments, tma):
     for seed in range(60):
         run(segments, seed, rescale=(0.0, 0.5, 1.0)[seed % 3], tma=tma)
+
+
+@pytest.mark.parametrize("tma", [False, True])
+@pytest.mark.parametrize("segments", [[1, 1, 1, 1, 1], [5, 9, 1, 6], [2, 1, 3, 1, 1, 4], [1] * 12, [1, 1, 2] * 4, [3] * 6, [40]])
+def test_every_segment_keeps_its_flag(segments, tma):
+    """Values that are not finite, in some tiles: whoever raises, reads and clears the flags, a segment's is there for all its readers."""
+    for seed in range(100):
+        run(segments, seed, rescale=(0.0, 0.5, 1.0)[seed % 3], tma=tma, odd=(0.2, 0.5)[seed % 2])

@@ -328,3 +328,56 @@ def test_arguments_that_do_not_fit_are_refused():
             ops.KVCache(*bad)
     ops.tree_attention(**ok)
     ws.check()
+
+
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("R,H,kv,D,n,length,page", [(64, 64, 8, 128, 60, 0, 16), (40, 32, 8, 64, 64, 0, 1), (150, 32, 8, 64, 20, 40, 16), (30, 24, 4, 64, 60, 70, 3)])
+def test_values_that_are_not_finite_in_many_short_segments(R, H, kv, D, n, length, page, dtype, tree):
+    """Infinities and NaN in new tokens of many requests, several segments of one tile or two to a CTA: a row that sees one has it in its result, all
+    others are as near to 64 bits as without them."""
+    from mlir_air_b200 import ops
+    gen = torch.Generator(device="cuda").manual_seed(R)
+    rnd = lambda *s: torch.randn(s, device="cuda", generator=gen)  # noqa: E731
+    total = length + n
+    table, pages = make_table([total] * R, page, R)
+    k, v = (rnd(pages, page, kv, D).to(dtype) for _ in range(2))
+    q = rnd(R * n, H, D).to(dtype)
+    p = torch.arange(total, device="cuda")
+    at = table[:, p // page].long(), (p % page)[None, :].expand(R, -1)
+    mask = random_masks([n] * R, R) if tree else None
+    new_seen = (mask.view(R, n, 1) >> torch.arange(n, device="cuda") & 1).bool() if tree else torch.ones((n, n), device="cuda").tril().bool().expand(R, n, n)
+    seen = torch.cat([torch.ones((R, n, length), dtype=torch.bool, device="cuda"), new_seen], 2)
+    # 64 bits, a cache head at a time
+    ref, tol, u = [], [], torch.finfo(dtype).eps / 2
+    for g in range(kv):
+        kr, vr = k[at][:, :, g].double(), v[at][:, :, g].double()
+        qr = q.view(R, n, kv, H // kv, D)[:, :, g].double()
+        s = torch.einsum("rnhd,rpd->rhnp", qr, kr) * D ** -0.5
+        w = torch.softmax(s.masked_fill(~seen[:, None], -torch.inf), -1)
+        o, mag = torch.einsum("rhnp,rpd->rnhd", w, vr), torch.einsum("rhnp,rpd->rnhd", w, vr.abs())
+        # (see attend_ref; the scores' part of the bound by the largest of all)
+        d = D * 2.0 ** -24 * float(torch.einsum("rnhd,rpd->rhnp", qr.abs(), kr.abs()).max()) * D ** -0.5 + 2.0 ** -20
+        ref.append(o)
+        tol.append(u * o.abs() + (u + 2 * d) * mag + torch.finfo(dtype).smallest_normal * 2 * u)
+    ref, tol = torch.stack(ref, 2), torch.stack(tol, 2) * 1.001  # [R, n, kv, H / kv, D]
+    # one in three requests, some of its heads: a value of a token near the front, and of any
+    extra = torch.zeros((R, n, kv, 1, D), dtype=torch.float64, device="cuda")
+    host = torch.Generator().manual_seed(R)
+    pick = lambda hi: int(torch.randint(0, hi, (1,), generator=host))  # noqa: E731
+    planted = {}
+    for r in range(0, R, 3):
+        for what in (float("inf"), -float("inf"), float("nan"), float("inf")):
+            j, g, e = (pick(4) if pick(2) else pick(n)), pick(kv), pick(D)
+            v[at[0][r, length + j], at[1][r, length + j], g, e] = what
+            planted[r, j, g, e] = what  # (a place drawn twice keeps the last)
+    for (r, j, g, e), what in planted.items():
+        extra[r, new_seen[r, :, j], g, 0, e] += what
+    ws = ops.RequestWorkspace()
+    args = (ops.KVCache(k, v), table, i32([length] * R), i32([n * r for r in range(R + 1)]), ws)
+    for _ in range(3):
+        out = ops.tree_attention(q, *args, mask=mask).view(R, n, kv, H // kv, D).double()
+        ws.check()
+        plain = (extra == 0).expand_as(out)
+        assert bool(((out - ref).abs() <= tol)[plain].all())
+        assert torch.equal(out[~plain].nan_to_num(nan=7.0, posinf=8.0, neginf=9.0), extra.expand_as(out)[~plain].nan_to_num(nan=7.0, posinf=8.0, neginf=9.0))
