@@ -1288,11 +1288,8 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
                 if (!whole) part[D * AT_ROWS + tid] = top, part[(D + 1) * AT_ROWS + tid] = sum;
             }
             dg_fence_before();
-            named_bar_sync(1, 128);
-            if (tid == 0) {
-                // what begins here and goes on is this CTA's last segment
-                if (!whole && (int)blockIdx.x == c0) joins[blockIdx.x] = AttendJoin{c1, g.q0, g.n, g.hk, g.m}, joined = true;
-            }
+            // what begins here and goes on is this CTA's last segment
+            if (tid == 0 && !whole && (int)blockIdx.x == c0) joins[blockIdx.x] = AttendJoin{c1, g.q0, g.n, g.hk, g.m}, joined = true;
         }
         if (tid == 0 && !joined) joins[blockIdx.x].last = -1;
     }

@@ -1,7 +1,9 @@
 """The barriers of tree_attention's tcgen05 kernel, modelled on the host: its warp roles as coroutines under random schedules, with
 waits that, like an mbarrier's, tell a phase from its neighbour only.  No schedule may deadlock, and nothing may be written while it is
 still to be read: the stages of K and V, the scores, the sums, the words that say which keys there are."""
+import os
 import random
+import re
 
 import pytest
 
@@ -21,12 +23,12 @@ class Bar:
         return self.phase % 2 != parity
 
 
-def run(segments, seed, rescale=0.5, tma=False, odd=0.0):
-    """odd: the share of tiles whose V holds what is not finite.  The warp that brings V takes it out and raises the segment's flag; the softmax
+def run(segments, seed, rescale=0.5, tma=False, odd=0.0, warps=1):
+    """warps: the softmax warps, each on its own (1: as one role).  odd: the share of tiles whose V holds what is not finite.  The warp that brings V takes it out and raises the segment's flag; the softmax
     warps put it back where it is seen, which takes them a while, if they find the flag when the segment's sums are there."""
     rng = random.Random(seed)
     total = sum(segments)
-    k_full, v_full, scored, weighed = ([Bar(1), Bar(1)] for _ in range(4))
+    k_full, v_full, scored, weighed = ([Bar(n), Bar(n)] for n in (1, 1, 1, warps))
     added, q_full, q_free, summed = [Bar(1) for _ in range(4)], Bar(1), Bar(1), Bar(1)
     segment_of = [i for i, t in enumerate(segments) for _ in range(t)]
     K, V, S, valid = [None] * 2, [None] * 2, [None] * 2, [None] * 4  # what each place holds
@@ -72,7 +74,7 @@ def run(segments, seed, rescale=0.5, tma=False, odd=0.0):
 
     def q_loader():
         for seg in range(len(segments)):
-            assert ring[seg % 4] is None or ring[seg % 4][1] == 4
+            assert ring[seg % 4] is None or ring[seg % 4][1] == 3 + warps
             ring[seg % 4] = [seg, 0]
             flags[seg % 4] = False
             found[seg % 4].arrive()
@@ -167,6 +169,8 @@ def run(segments, seed, rescale=0.5, tma=False, odd=0.0):
                     summed.arrive()
             state["done"] += 1
 
+    at, took = {}, {}  # softmax warps that have weighed a tile, or taken a segment's sums
+
     def softmax():
         n = 0
         for seg, tiles in enumerate(segments):
@@ -175,29 +179,33 @@ def run(segments, seed, rescale=0.5, tma=False, odd=0.0):
                 yield scored[n % 2], phase(n)
                 assert S[n % 2] == (n, "scores") and valid[n % 4] == (n, "there")
                 yield None
-                valid[n % 4] = (n, "read")
                 if i > 0 and rng.random() < rescale:
                     yield added[(n - 1) % 4], (n - 1) >> 2 & 1
-                    assert state["o"] == n - 1, "sums rescaled before the last product is in them"
-                    state["o"] = "busy"
+                    assert state["o"] in (n - 1, "busy"), "sums rescaled before the last product is in them"
+                    state["o"] = "busy" if warps == 1 else n - 1
                     yield None
                     state["o"] = n - 1
-                assert S[n % 2] == (n, "scores")
-                S[n % 2] = (n, "weights")
+                assert S[n % 2] == (n, "scores") and valid[n % 4] == (n, "there")
+                at[n] = at.get(n, 0) + 1
+                if at[n] == warps:
+                    valid[n % 4], S[n % 2] = (n, "read"), (n, "weights")
                 weighed[n % 2].arrive()
                 n += 1
             yield summed, seg % 2
             assert state["o"] == n - 1
-            for _ in range(8 if odd else 0):  # (four warps, each in its time)
+            for _ in range(8 if odd else 0):  # (a warp takes its time)
                 assert flags[seg % 4] == any(raised[n - tiles:n]), "a segment's flag lost, or another one's"
                 yield None
             yield None
-            state["o"] = None
+            took[seg] = took.get(seg, 0) + 1
+            if took[seg] == warps:
+                state["o"] = None
 
     landing = []
     loaders = [("k", tma_loader(0, landing)), ("v", tma_loader(1, landing)), ("memory", memory(landing))] if tma else \
         [("k", loader(0)), ("v", loader(1))]
-    roles = {name: [r, None] for name, r in [("mma", products()), ("tc", tensor_cores()), ("softmax", softmax()), ("q", q_loader())] + loaders}
+    roles = {name: [r, None] for name, r in [("mma", products()), ("tc", tensor_cores()), ("softmax", softmax()), ("q", q_loader())] + loaders +
+             [(f"softmax {i}", softmax()) for i in range(1, warps)]}
     speed = {name: rng.choice([1, 1, 3, 30]) for name in roles}  # some roles far behind the others
     idle = 0
     while roles:
@@ -229,4 +237,23 @@ def test_no_schedule_deadlocks_or_overwrites(segments, tma):
 def test_every_segment_keeps_its_flag(segments, tma):
     """Values that are not finite, in some tiles: whoever raises, reads and clears the flags, a segment's is there for all its readers."""
     for seed in range(100):
-        run(segments, seed, rescale=(0.0, 0.5, 1.0)[seed % 3], tma=tma, odd=(0.2, 0.5)[seed % 2])
+        run(segments, seed, rescale=(0.0, 0.5, 1.0)[seed % 3], tma=tma, odd=(0.2, 0.5)[seed % 2], warps=(1, 4)[seed // 2 % 2])
+
+
+@pytest.mark.parametrize("tma", [False, True])
+@pytest.mark.parametrize("segments", [[1], [3], [1, 1, 1, 1, 1], [2, 1, 3, 1, 1, 4], [5, 9, 1, 6], [20]])
+def test_softmax_warps_need_not_stay_together(segments, tma):
+    for seed in range(60):
+        run(segments, seed, rescale=(0.0, 0.5, 1.0)[seed % 3], tma=tma, warps=4)
+
+
+def test_every_wait_between_the_roles_has_a_limit():
+    """A warp whose wait gives up leaves for the kernel's end.  A barrier that it will not come to any more would hold the others for good, so
+    between the first role and the end there is none: the roles wait at mbarriers, each time with a limit."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mlir_air_b200", "csrc", "awq_tree_attention.cu")
+    text = open(path).read()
+    kernel = text[text.index("tree_attention_tiles_kernel("):text.index("tree_attention_join_kernel(")]
+    roles = kernel[kernel.index("---- TMA: warp 4 K"):kernel.index("req_error(&a.header->error, REQ_ERR_TIMEOUT)")]
+    assert len(re.findall(r"mbar_wait_bounded_warp\(", roles)) > 10
+    assert not re.findall(r"named_bar\w*|__syncthreads\w*|bar\.sync|barrier\.|mbar_wait\(|while \(", roles)
+    assert kernel.count("__syncthreads()") - kernel[:kernel.index("---- TMA: warp 4 K")].count("__syncthreads()") == 1  # where they all end
