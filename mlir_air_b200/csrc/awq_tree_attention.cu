@@ -732,7 +732,7 @@ struct AttendSegment {
 struct AttendTilesShared {
     // mbarriers, of even and odd tiles: K, V there; QK^T, PV (of every fourth) done; P there.  Of a segment: Q there, Q done with, O done.  V that is
     // not ready for the product yet.
-    uint64_t k_full[2], v_full[2], scored[2], added[4], weighed[2], q_full, q_free, summed, v_landed;
+    uint64_t k_full[2], v_full[2], scored[2], added[4], weighed[2], q_full, q_free, summed, v_landed, drained;
     uint32_t tmem;
     int odd[4], pad;                       // a segment's: values that are not finite were taken out of V
     uint64_t found[4];                     // mbarriers: a segment's description is there
@@ -931,6 +931,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
         mbar_init(q_free, 1);
         mbar_init(summed, 1);
         mbar_init(smem_u32(&sh.v_landed), 1);
+        mbar_init(smem_u32(&sh.drained), 1);
         for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&sh.found[i]), 1);
         mbar_fence_init();
     }
@@ -979,6 +980,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
     AttendSegment g;
     bool ok = true;
     int n = 0;  // tiles so far: tile n has place n % 2 of everything that is held twice, in phase n / 2 % 2
+    int cleaned = 0;  // of the warp that brings V: tiles that were put right before the product had them
     auto bar_of = [](uint32_t bar, int t) { return bar + 8 * (t & 1); };
     // keys that all rows of a segment see, from the front on
     auto seen_by_all = [&](const AttendSegment &s) { return s.len + (a.mask ? 0 : s.m * AT_ROWS / group + 1); };
@@ -998,7 +1000,6 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
         const CUtensorMap *map = is_v ? &v_map : &k_map;
         const int boxes = AT_TILE / box;
         const uint32_t landed = smem_u32(&sh.v_landed);
-        int cleaned = 0;  // tiles that went through `landed`
         if (lane == 0) tma_prefetch_desc(map);
         for (int seg = 0; ok && next(seg); ++seg) {
             const int total = g.len + g.n;
@@ -1293,7 +1294,19 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
         }
         if (tid == 0 && !joined) joins[blockIdx.x].last = -1;
     }
-    if (!ok && lane == 0) req_error(&a.header->error, REQ_ERR_TIMEOUT);
+    if (!ok) {
+        // A wait gave up, here or, as its consequence, in other warps one after another: the roles wait for each other at mbarriers alone, all
+        // with a limit.  What this warp has on its way into shared or tensor memory must be there before the CTA gives these back.
+        if (lane == 0) req_error(&a.header->error, REQ_ERR_TIMEOUT);
+        if (box && (warp == 4 || warp == 5)) {
+            for (int t = max(n - 2, 0); t < n; ++t) mbar_wait_bounded_warp(bar_of(warp == 5 ? v_full : k_full, t), phase_of(t), WAIT_LIMIT_DEFAULT);
+            if (warp == 5 && cleaned > 0) mbar_wait_bounded_warp(smem_u32(&sh.v_landed), (cleaned - 1) & 1, WAIT_LIMIT_DEFAULT);
+        } else if (warp == 7) {
+            if (elect_one()) dg_umma_commit(smem_u32(&sh.drained));
+            __syncwarp();
+            mbar_wait_bounded_warp(smem_u32(&sh.drained), 0, WAIT_LIMIT_DEFAULT);
+        }
+    }
     dg_fence_before();
     __syncthreads();
     dg_fence_after();

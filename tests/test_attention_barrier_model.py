@@ -257,3 +257,21 @@ def test_every_wait_between_the_roles_has_a_limit():
     assert len(re.findall(r"mbar_wait_bounded_warp\(", roles)) > 10
     assert not re.findall(r"named_bar\w*|__syncthreads\w*|bar\.sync|barrier\.|mbar_wait\(|while \(", roles)
     assert kernel.count("__syncthreads()") - kernel[:kernel.index("---- TMA: warp 4 K")].count("__syncthreads()") == 1  # where they all end
+
+
+def test_a_warp_that_gave_up_waits_for_its_copies_and_products():
+    """Whoever leaves early must not leave copies or products behind that still write to shared or tensor memory when the CTA gives it back: all
+    that is in flight when a wait of its warp gives up is waited for, with a limit, at the kernel's end.  Which tiles that are, for any number
+    of tiles issued: the last two, and all before them have been waited for already."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mlir_air_b200", "csrc", "awq_tree_attention.cu")
+    text = open(path).read()
+    kernel = text[text.index("tree_attention_tiles_kernel("):text.index("tree_attention_join_kernel(")]
+    end = kernel[kernel.index("req_error(&a.header->error, REQ_ERR_TIMEOUT)"):]
+    end = end[:end.index("__syncthreads()")]
+    for what in ("v_full : k_full, t", "v_landed", "dg_umma_commit(smem_u32(&sh.drained))", "smem_u32(&sh.drained), 0"):
+        assert what in end, what
+    assert end.count("WAIT_LIMIT_DEFAULT") == 3  # (not the call's own limit, which may be a short one)
+    # K's and V's warp issue tile n once tile n - 2 has been scored or added, so that its copies have landed
+    for n in range(12):
+        landed = {t for t in range(n) if t + 2 < n}
+        assert landed | set(range(max(n - 2, 0), n)) == set(range(n))
