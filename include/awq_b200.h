@@ -504,7 +504,8 @@ int awq_b200_tree_attention(const void *q, long long q_row_stride, long long q_h
  * 16-bit type): the rows path[q_start[r] + i] (ascending; NULL: the first kept[r], which lie where they belong) move to lens[r] + i,
  * lens_out[r] = lens[r] + kept[r] (lens_out may be lens), and the pages behind that go back onto the stack of free pages.
  * kept[r] = -1 ends the request: length 0, all pages free.  A path has up to 64 tokens.  A request whose count or path does not fit
- * keeps nothing and is reported by awq_b200_request_check. */
+ * keeps nothing of the step; one whose rows (beyond T, which is the size of path), length or starts do not fit is left as it is, its pages
+ * too, also with -1.  Both are reported by awq_b200_request_check, and so is a stack without room for the pages, which then gets none. */
 int awq_b200_page_keep(void *kv, long long layer_stride, long long kv_stride, long long page_stride, long long slot_stride,
                        long long head_stride, int layers, int n_pages, int page_size, int n_kv_heads, int head_dim,
                        const int32_t *table, long long table_stride, int table_width, const int32_t *lens, int32_t *lens_out,

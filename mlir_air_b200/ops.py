@@ -696,7 +696,8 @@ def page_keep(kv, table, lens, q_start, kept, free_pages, free_count, ws: Reques
     """After a step: keep kept[r] of request r's tokens.  In every layer of kv [layers, 2, n_pages, page_size, n_kv_heads, head_dim] the
     rows path[q_start[r] + i] (indices in its tree, ascending; without `path` the first kept[r]) move to lens[r] + i; lens grows
     by kept and the pages behind it go back to `free_pages` (in place unless lens_out / free_count_out are given).
-    kept[r] = -1 ends the request: length 0, all its pages free."""
+    kept[r] = -1 ends the request: length 0, all its pages free.  `path` has a place for every row of the step; a request with rows
+    behind its end is left as it is, and ws.check() says so."""
     dev, R = ws.device, lens.numel()
     if kv.dim() != 6 or kv.shape[1] != 2 or kv.element_size() != 2 or kv.get_device() != dev or kv.numel() == 0:
         raise _lib.AwqBackendError(f"kv must be [layers, 2, n_pages, page_size, n_kv_heads, head_dim] of 16-bit values on cuda:{dev}, got "

@@ -312,6 +312,52 @@ def test_keep_reports_what_does_not_fit():
         ops.page_keep(kv, table, i32(lens), i32([0, 8]), i32([2, 1]), i32([0] * used), i32([0]), ws)
 
 
+@pytest.mark.parametrize("what", ["short path", "starts beyond the path", "start below zero", "start behind the next", "length beyond the table", "length below zero"])
+@pytest.mark.parametrize("ends", [False, True])
+def test_a_request_whose_range_does_not_fit_keeps_its_state(what, ends):
+    """Its length, its rows and its pages stay as they are, also if it was to end; the other requests are served."""
+    from mlir_air_b200 import ops
+    from mlir_air_b200._lib import AwqBackendError
+    ws = ops.RequestWorkspace()
+    lens, new, start = [10, 40, 17], [8, 4, 20], [0, 8, 12, 32]
+    kept, bad, path = [2, 1, 5], [2], [0, 3] + [0] * 6 + [2, 0, 0, 0] + [1, 4, 5, 8, 9] + [0] * 15
+    table, used = make_table([18, 44, 37], 16, 0, width=4)
+    if what == "short path":
+        path = path[:17]
+    elif what == "starts beyond the path":
+        start[2:], bad = [40, 60], [1, 2]
+    elif what == "start below zero":
+        start[0], bad = -1, [0]
+    elif what == "start behind the next":
+        start[1], bad = 20, [0, 1]
+        start[0] = 21
+    elif what == "length beyond the table":
+        lens[2] = 64
+    else:
+        lens[1], bad = -3, [1]
+    if ends:
+        kept = [-1 if r in bad else k for r, k in enumerate(kept)]
+    kv = torch.randn((2, 2, used, 16, 2, 64), device="cuda").to(BF)
+    before, stack, count, lens_t = kv.clone(), i32([-5] * used), i32([0]), i32(lens)
+    ops.page_keep(kv, table, lens_t, i32(start), i32(kept), stack, count, ws, path=i32(path))
+    with pytest.raises(AwqBackendError, match="count or path"):
+        ws.check()
+    assert lens_t.tolist() == [l if r in bad else l + kept[r] for r, l in enumerate(lens)]
+    host, free, want = table.tolist(), [], before.clone()
+    for r in range(3):
+        if r in bad:
+            continue
+        slot = lambda p: (host[r][p // 16], p % 16)  # noqa: B023, E731
+        for i in range(kept[r]):
+            a, b = slot(lens[r] + path[start[r] + i]), slot(lens[r] + i)
+            want[:, :, b[0], b[1]] = before[:, :, a[0], a[1]]
+        free += host[r][-(-(lens[r] + kept[r]) // 16):-(-(lens[r] + start[r + 1] - start[r]) // 16)]
+    assert torch.equal(kv, want)
+    assert count.tolist() == [len(free)] and stack.tolist() == free + [-5] * (used - len(free))
+    ops.page_keep(kv, table, i32([10, 40, 17]), i32([0, 0, 0, 0]), i32([0, 0, 0]), stack, count, ws)
+    ws.check()
+
+
 # ---- together -----------------------------------------------------------------------------------------------------
 def test_steps_of_a_serving_loop():
     """Prompts, drafted trees, acceptance, requests that end and new ones in their place: after every step the cache holds, for
