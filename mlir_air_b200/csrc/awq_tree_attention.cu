@@ -54,6 +54,12 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2 units in the last pl
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Weights that are multiplied as 16-bit values are 2^WEIGHT_LIFT times exp(score - maximum); their f32 sum is as many times too large, so that
+// the factor goes with the division.  fp16 ends at 2^-24, and a long context's small weights count together: 32000 keys 16 nats behind one were
+// off by 6 %, 17.5 nats behind were nothing.  Seven up, and with a maximum that may lie 8 behind, the largest is 2^15; what a weight may lose
+// is 2^-32 of the largest.  bf16 has f32's exponents.
+template <bool F16>
+constexpr float WEIGHT_LIFT = F16 ? 7.f : 0.f;
 __device__ __forceinline__ int page_index(const AttendArgs &a, int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / a.cache.page_size; }
 
 // Head sizes above 128: a CTA per row and head, a warp per 32 keys, four of them at a time; f32 throughout.  Rows of a group do not share
@@ -181,8 +187,8 @@ __global__ void __launch_bounds__(AA_WARPS * 32) tree_attention_any_kernel(Atten
 //           rows of Q are taken in the same order; odd keys have the halves of their lines swapped;
 //   output: a lane has 16 bytes of four keys (its k-indices) and pairs them up with byte permutes; column n of block j is then
 //           head element 8 n + j, so that a lane's results are 16 neighbours; pieces are shifted by pairs of keys.
-// Weights are multiplied as two 16-bit pieces, p = hi + lo: the tensor cores have time to spare, and the result keeps the
-// accuracy of f32 weights.
+// Weights are multiplied as two 16-bit pieces, p = hi + lo: the tensor cores have time to spare, and the result keeps 16 (bf16) or 22 bits
+// of a weight; in fp16 those below 2^-21 of the largest keep what lies above 2^-32 of it (WEIGHT_LIFT).
 //
 // Measured, bf16, heads of 128: one token of 64 requests of 1000 to 16000, 64/8 heads, 261 us, 5.9 TB/s (90 % of a copy's rate; keys
 // straight to registers 389); one token of 256 requests of 500 to 2000, 32/8 heads, 196 us, 5.9 TB/s.  Small steps are a chain of
@@ -514,7 +520,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
                         if (!seen) s[b][e] = -INFINITY;
                     }
             }
-            // The weights refer to a maximum that may lie 8 behind: they stay below 2^8, and the sums are rarely rescaled.
+            // The weights refer to a maximum that may lie 8 behind: they stay below 2^8 (and the lift), and the sums are rarely rescaled.
             float p[2][4];
 #pragma unroll
             for (int i2 = 0; i2 < 2; ++i2) {
@@ -530,7 +536,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
 #pragma unroll
                         for (int b = 0; b < 8; ++b) acc[c][b][2 * i2] *= keep, acc[c][b][2 * i2 + 1] *= keep;
                 }
-                const float ref = top[i2] == -INFINITY ? 0.f : top[i2];
+                const float ref = (top[i2] == -INFINITY ? 0.f : top[i2]) - WEIGHT_LIFT<F16>;
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -713,7 +719,8 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
 // cores during its softmax, the exponentials during its products) is the other one's.  O stays in tensor memory; it is rescaled
 // only when a maximum has grown by more than 8 (powers of two), by the warp that finds it.
 // Weights are rounded to the rows' 16-bit type for the product, as they have to be for one tensor-core operand (their sum is
-// not): half a step per weight, independent from key to key.
+// not): half a step per weight, independent from key to key; in fp16 for weights from 2^-21 of the largest on, smaller ones to 2^-32 of
+// it (WEIGHT_LIFT).
 //
 // Measured, bf16, heads of 128: two trees of 64 over 32000 tokens, 64/8 heads, 163 to 174 us, 770 to 820 TFLOP/s; 16 trees of 8 to 32 over 300 to 6000
 // tokens, 32/8 heads, 58 us; four prompts of 512 behind 2000 to 4000 tokens, 32/8 heads, 153 us, 655 TFLOP/s.  Bound by how fast one CTA's
@@ -1220,7 +1227,7 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
                             }
                         }
                     }
-                    const float ref = top == -INFINITY ? 0.f : top;
+                    const float ref = (top == -INFINITY ? 0.f : top) - WEIGHT_LIFT<F16>;
                     uint64_t sums[2] = {0, 0};
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {

@@ -1,4 +1,6 @@
 """tree_attention against 64 bits: head layouts, page and tile borders, masks, strides, values that no row sees."""
+import math
+
 import pytest
 import torch
 
@@ -381,3 +383,34 @@ def test_values_that_are_not_finite_in_many_short_segments(R, H, kv, D, n, lengt
         plain = (extra == 0).expand_as(out)
         assert bool(((out - ref).abs() <= tol)[plain].all())
         assert torch.equal(out[~plain].nan_to_num(nan=7.0, posinf=8.0, neginf=9.0), extra.expand_as(out)[~plain].nan_to_num(nan=7.0, posinf=8.0, neginf=9.0))
+
+
+@pytest.mark.parametrize("gap", [4.0, 14.0, 16.0, 17.5, 20.0])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("D,n,per_sm", [(64, 1, 3), (96, 1, 3), (128, 20, 2), (64, 20, 2), (160, 1, 1)])
+def test_many_small_weights_behind_a_large_one(D, n, per_sm, dtype, gap):
+    """Keys that hold all the weight and no value, and 32000 others `gap` nats below: what these add up to is the result.  As many requests over
+    the same pages as CTAs run at once, so that a CTA, and each of its warps, has such a key and all of a request's others.
+
+    With a = exp(-gap), m large keys and N others of value 1 the result is N a / (m + N a).  A weight is rounded by u, half a step, relative to
+    itself, or in fp16, below 2^-21 of the largest, by half of 2^-31 of the largest: together N 2^-32 / m.  The rest as in attend_ref."""
+    from mlir_air_b200 import ops
+    R, group, page, length = (torch.cuda.get_device_properties(0).multi_processor_count * per_sm if D < 160 else 3), 4, 16, 32000
+    k, v = torch.zeros((length // page + 2 * R, page, 1, D), dtype=dtype, device="cuda"), torch.ones((length // page + 2 * R, page, 1, D), dtype=dtype, device="cuda")
+    for key in (0, 16, 32, 48):
+        k[key // page, key % page, 0, 5], v[key // page, key % page] = gap, 0
+    q = torch.zeros((R * n, group, D), dtype=dtype, device="cuda")
+    q[..., 5] = 1
+    blocks = length // page
+    table = torch.arange(blocks + 2, dtype=torch.int32, device="cuda").repeat(R, 1)
+    table[:, blocks:] = blocks + torch.arange(2 * R, dtype=torch.int32, device="cuda").view(R, 2)
+    ws = ops.RequestWorkspace()
+    out = ops.tree_attention(q, ops.KVCache(k, v), table, i32([length] * R), i32([n * r for r in range(R + 1)]), ws, scale=1.0)
+    ws.check()
+    a, m, u = math.exp(-gap), 4, torch.finfo(dtype).eps / 2
+    others = length - m + 1 + torch.arange(n, dtype=torch.float64, device="cuda").repeat(R)
+    want = (others * a / (m + others * a)).view(-1, 1, 1)
+    d = D * 2.0 ** -24 * gap + 2.0 ** -20
+    tol = u * want + (u + 2 * d) * want + (others.max() * 2.0 ** -32 / m if dtype == FP else 0) + torch.finfo(dtype).smallest_normal * 2 * u
+    err = (out.double() - want).abs()
+    assert bool((err <= tol * 1.001).all()), (float((err / want).max()), float((tol / want).max()))
