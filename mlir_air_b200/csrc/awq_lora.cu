@@ -9,7 +9,8 @@
 // depend on its tile or its place in it.  Operands go from global memory to registers in 16-byte pieces: the order of the
 // products along K (or the rank) is free as long as both operands have the same one, so eight neighbours of a row are a lane's
 // operands of two k-steps.  x A^T stays at f32's accuracy between the products: it is summed in f32 and multiplied as two
-// bf16 pieces (hi + lo, 2^-17).
+// bf16 pieces (hi + lo, 2^-17; of an infinite sum hi is the largest finite value, so that lo is what is infinite and no difference of
+// infinities arises).
 #include "awq_request.cuh"
 
 #include <cooperative_groups.h>
@@ -78,6 +79,14 @@ __device__ __forceinline__ void lora_down(float (&acc)[MT][NB][4], const uint16_
     }
 }
 
+// Two sums as pieces.  Of those at `left` and behind, which are ranks that an adapter has not, nothing is left: x may be infinite there and A 0.
+__device__ __forceinline__ void lora_pieces(float x, float y, int left, uint32_t &hi, uint32_t &lo) {
+    constexpr float MOST = 3.38953139e38f;  // bf16's largest
+    if (left < 1) x = 0.f;
+    if (left < 2) y = 0.f;
+    hi = pack16x2<false>(fminf(fmaxf(x, -MOST), MOST), fminf(fmaxf(y, -MOST), MOST));
+    lo = pack16x2<false>(x - bf16x2_lo(hi), y - bf16x2_hi(hi));
+}
 // The first `left` of eight columns of B, the others zero, whatever is stored there.
 __device__ __forceinline__ uint4 lora_mask_rank(uint4 v, int left) {
     uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -241,7 +250,8 @@ __global__ void __cluster_dims__(LF_CLUSTER, 1, 1) __launch_bounds__(LF_WARPS * 
                     s.x += v.x, s.y += v.y;
                 }
                 s.x *= scale, s.y *= scale;
-                const uint32_t hi = pack16x2<false>(s.x, s.y), lo = pack16x2<false>(s.x - bf16x2_lo(hi), s.y - bf16x2_hi(hi));
+                uint32_t hi, lo;
+                lora_pieces(s.x, s.y, rank - r, hi, lo);
                 // element r of the row: chunk, the lane's eight, the word in it
                 const int c = r / 32, l = (row % 8) * 4 + r % 32 / 8, w = r % 8 / 2;
                 reinterpret_cast<uint32_t *>(&frag[c][0][row / 8][l])[w] = hi;
@@ -436,8 +446,9 @@ __global__ void __launch_bounds__(LD_WARPS * 32, 2) lora_down_kernel(LoraArgs a)
                 s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
             }
             s.x *= scale, s.y *= scale, s.z *= scale, s.w *= scale;
-            const uint2 hi = make_uint2(pack16x2<false>(s.x, s.y), pack16x2<false>(s.z, s.w));
-            const uint2 lo = make_uint2(pack16x2<false>(s.x - bf16x2_lo(hi.x), s.y - bf16x2_hi(hi.x)), pack16x2<false>(s.z - bf16x2_lo(hi.y), s.w - bf16x2_hi(hi.y)));
+            uint2 hi, lo;
+            lora_pieces(s.x, s.y, rank - r0 - r, hi.x, lo.x);
+            lora_pieces(s.z, s.w, rank - r0 - r - 2, hi.y, lo.y);
             uint16_t *d = a.low + (long long)(w.y + row) * 2 * wide + r0 + r;
             *reinterpret_cast<uint2 *>(d) = hi;
             *reinterpret_cast<uint2 *>(d + wide) = lo;

@@ -190,3 +190,41 @@ def test_streams_and_graphs():
         graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want2)
+
+
+@pytest.mark.parametrize("T", [1, 20, 128, 200])
+@pytest.mark.parametrize("rank_max,ranks", [(8, [1, 2, 8]), (16, [1, 3, 5]), (64, [1, 2, 33])])
+def test_infinite_and_missing_numbers_stay_what_they_are(T, rank_max, ranks):
+    """An infinite x gives what the formula gives, infinities where they do not meet their opposites; NaN gives NaN; other rows are as they were."""
+    from mlir_air_b200 import ops
+    x, A, B, s, rk, base = make(T, 512, 264, 3, rank_max, ranks)
+    idx, ws, ad = i32([t % 4 - 1 for t in range(T)]), ops.RequestWorkspace(), ops.LoraAdapters(A, B, s, rk)
+    if T == 1:
+        idx[0] = 0
+    was = ops.lora(x, ad, idx, base, ws)
+    rows = list(range(0, T, 3))
+    for i, t in enumerate(rows):
+        x[t, (37 * t) % 512] = (float("inf"), -float("inf"), float("nan"))[i % 3]
+    got = ops.lora(x, ad, idx, base, ws)
+    ws.check()
+    want, _ = lora_ref(x, A, B, s, ranks, idx.cpu(), base)
+    odd = torch.zeros(T, dtype=torch.bool, device="cuda")
+    odd[rows] = True
+    odd &= idx >= 0
+    assert torch.equal(got[~odd], was[~odd])
+    same = lambda t: t[odd].double().nan_to_num(nan=7.0, posinf=8.0, neginf=9.0)  # noqa: E731
+    assert torch.equal(same(got), same(want)) and bool(torch.isinf(got).any())
+
+
+@pytest.mark.parametrize("T", [3, 150])
+def test_a_sum_between_the_largest_numbers_of_two_formats(T):
+    """x A^T beyond bf16's largest number, but not f32's: the product with a small B is finite."""
+    from mlir_air_b200 import ops
+    x, A, B = torch.zeros((T, 64), dtype=BF, device="cuda"), torch.zeros((1, 8, 64), dtype=BF, device="cuda"), torch.zeros((1, 64, 8), dtype=BF, device="cuda")
+    x[:, 3], x[:, 9], A[0, 0, 3], A[0, 0, 9], B[0, :, 0] = torch.finfo(BF).max, 1.5 * 2.0 ** 119, 1, 1, 2.0 ** -10
+    ws, base = ops.RequestWorkspace(), torch.zeros((T, 64), device="cuda")
+    args = (x, A, B, torch.ones(1, device="cuda"), None)
+    got = ops.lora(x, ops.LoraAdapters(*args[1:4]), i32([0] * T), base, ws)
+    ws.check()
+    ref, tol = lora_ref(*args, torch.zeros(T, dtype=torch.int64), base)
+    assert bool(torch.isfinite(ref).all()) and bool(((got.double() - ref).abs() <= tol).all())
