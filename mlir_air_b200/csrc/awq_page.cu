@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(RA_THREADS) rope_append_kernel(AppendArgs a) {
         return;
     }
     bool later = false;
-    for (int i = t + 1 + threadIdx.x; i < a.T; i += RA_THREADS) later |= a.slots[i] == slot;
+    for (int i = t + 1 + threadIdx.x; i < a.T; i += RA_THREADS)  // (a row that is left out for its position takes no slot from others)
+        later |= a.slots[i] == slot && (unsigned)a.positions[i] < (unsigned)a.n_positions;
     later = __syncthreads_or(later);
     const int D = a.cache.head_dim, half = D >> 1, chunks = half >> 3;
     const int page = slot / a.cache.page_size, off = slot - page * a.cache.page_size;

@@ -217,6 +217,22 @@ def test_append_reports_slots_and_positions():
         ops.rope_append(x.half(), x, x, lut, i32([0, 0]), i32([0, 1]), cache, ws)
 
 
+def test_a_row_that_is_left_out_takes_no_slot_from_others():
+    """Of two rows that name one slot the last that has a position stays there."""
+    from mlir_air_b200 import ops
+    from mlir_air_b200._lib import AwqBackendError
+    D = 64
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    k, v = (torch.randn((4, 2, D), device="cuda", generator=gen).to(BF) for _ in range(2))
+    lut = torch.cat([torch.ones(10, D // 2), torch.zeros(10, D // 2)], 1).to(BF).cuda()
+    for bad in (10, -1, 2 ** 31 - 1):
+        cache, ws = ops.KVCache(*torch.zeros((2, 3, 16, 2, D), dtype=BF, device="cuda")), ops.RequestWorkspace()
+        ops.rope_append(torch.zeros((4, 2, D), dtype=BF, device="cuda"), k, v, lut, i32([0, 1, 2, bad]), i32([5, 7, 5, 5]), cache, ws)
+        with pytest.raises(AwqBackendError, match="slot outside"):
+            ws.check()
+        assert torch.equal(cache.k[0, 5], k[2]) and torch.equal(cache.v[0, 5], v[2]) and torch.equal(cache.k[0, 7], k[1])
+
+
 # ---- page_keep ----------------------------------------------------------------------------------------------------
 def keep_ref(kv, table, lens, new, kept, path, free, page):
     """The definition on a clone of kv and host lists: (kv, lens, free)."""
