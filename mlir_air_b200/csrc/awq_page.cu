@@ -24,6 +24,9 @@ int check_kv_cache(const char *who, const awq_b200_kv_cache_t *c, KvCacheView *o
     return AWQ_OK;
 }
 
+// Pages of `tokens` tokens: both below 2^31, their sum need not be.
+__device__ __forceinline__ int pages_of(int tokens, int page) { return (int)(((unsigned)tokens + (unsigned)page - 1u) / (unsigned)page); }
+
 // Exclusive sums of a pair over the block's threads (256), and the totals.
 __device__ __forceinline__ void block_scan_pair(long long &a, long long &b, long long &total_a, long long &total_b) {
     __shared__ long long sa[8], sb[8];
@@ -89,7 +92,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(PlanArgs a) {
             continue;
         }
         rows += n;
-        need += ((long long)len + n + a.page - 1) / a.page - ((long long)len + a.page - 1) / a.page;
+        need += pages_of(len + n, a.page) - pages_of(len, a.page);
     }
     long long all_rows, all_need;
     block_scan_pair(rows, need, all_rows, all_need);
@@ -103,7 +106,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(PlanArgs a) {
             start[r] = (int)rows;
             first[r] = (int)need;
             rows += n;
-            need += (len + n + a.page - 1) / a.page - (len + a.page - 1) / a.page;
+            need += pages_of(len + n, a.page) - pages_of(len, a.page);
         }
         if (tid == 0) start[a.R] = (int)all_rows, first[a.R] = (int)all_need;
     } else {
@@ -120,7 +123,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(PlanArgs a) {
             req_error(&a.header->error, REQ_ERR_PAGE);
             page = -1;
         }
-        a.table[r * a.table_stride + (a.lens[r] + a.page - 1) / a.page + k - first[r]] = page;
+        a.table[r * a.table_stride + pages_of(a.lens[r], a.page) + k - first[r]] = page;
     }
     for (int t = me; t < a.T; t += step) {
         if (t >= (int)all_rows) {  // rows behind the last request
@@ -130,7 +133,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(PlanArgs a) {
             continue;
         }
         const int r = request_of_row(start, a.R, t), j = t - start[r], len = a.lens[r];
-        const int at = len + j, block = at / a.page, held = (len + a.page - 1) / a.page;
+        const int at = len + j, block = at / a.page, held = pages_of(len, a.page);
         // a new page is not read from the table, which another CTA may not have written yet
         int page = block < held ? a.table[r * a.table_stride + block] : a.free_pages[count - 1 - (first[r] + block - held)];
         if ((unsigned)page >= (unsigned)a.max_pages) {
@@ -367,7 +370,7 @@ __global__ void __launch_bounds__(KEEP_THREADS) page_keep_kernel(KeepArgs a) {
         }
         if (q.bad) req_error(&a.header->error, REQ_ERR_KEPT);
         after[r] = q.unknown ? q.len : q.ends ? 0 : q.len + (q.bad ? 0 : q.kept);
-        first[r] = q.unknown ? 0 : (q.len + q.fresh + a.page - 1) / a.page - (after[r] + a.page - 1) / a.page;
+        first[r] = q.unknown ? 0 : pages_of(q.len + q.fresh, a.page) - pages_of(after[r], a.page);
         gone += first[r];
     }
     block_scan_pair(gone, unused, all_gone, all_unused);
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(KEEP_THREADS) page_keep_kernel(KeepArgs a) {
     __syncthreads();
     for (int k = tid; fits && k < (int)all_gone; k += KEEP_THREADS) {
         const int r = request_of_row(first, a.R, k);
-        a.free_pages[count + k] = a.table[r * a.table_stride + (after[r] + a.page - 1) / a.page + k - first[r]];
+        a.free_pages[count + k] = a.table[r * a.table_stride + pages_of(after[r], a.page) + k - first[r]];
     }
     for (int r = r0; r < r1; ++r) a.lens_out[r] = after[r];
     if (tid == 0) {

@@ -123,6 +123,30 @@ def test_plan_reports_parents_and_pages_it_cannot_use():
             ws.check()
 
 
+def test_lengths_near_the_end_of_32_bits():
+    """A table as wide as slots can be numbered, pages whose size is no power of two, a request that ends in its last page."""
+    from mlir_air_b200 import ops
+    page, width, ws = 1000, 2147483, ops.RequestWorkspace()
+    table = torch.full((2, width), -1, dtype=torch.int32, device="cuda")
+    table[0, -1], table[1, 0] = 7, 3
+    lens, new, stack, count = i32([2147482990, 1999]), i32([9, 3]), i32([5, 4, 6, -5, -5, -5]), i32([3])
+    table[1, 1] = 8
+    p = ops.page_plan(lens, new, table, stack, count, page, 12, ws)
+    ws.check()
+    assert p.q_start.tolist() == [0, 9, 12] and count.tolist() == [2] and int(table[1, 2]) == 6
+    assert p.slots.tolist() == [7990 + j for j in range(9)] + [8999, 6000, 6001]
+    assert p.positions.tolist() == [2147482990 + j for j in range(9)] + [1999, 2000, 2001]
+    kv = torch.zeros((1, 2, 10, page, 1, 16), dtype=BF, device="cuda")
+    kv[0, 0, 7, 990:999, 0, 0] = torch.arange(9, device="cuda")
+    ops.page_keep(kv, table, lens, p.q_start, i32([3, 1]), stack, count, ws, path=i32([2, 5, 8] + [0] * 6 + [0, 0, 0]))
+    ws.check()
+    assert lens.tolist() == [2147482993, 2000] and count.tolist() == [3] and stack.tolist() == [5, 4, 6, -5, -5, -5]
+    assert kv[0, 0, 7, 990:993, 0, 0].tolist() == [2, 5, 8]
+    ops.page_keep(kv, table, lens, i32([0, 0, 0]), i32([0, -1]), stack, count, ws)
+    ws.check()
+    assert lens.tolist() == [2147482993, 0] and count.tolist() == [5] and stack.tolist() == [5, 4, 6, 3, 8, -5]
+
+
 # ---- rope_append --------------------------------------------------------------------------------------------------
 def rotate(x, row):
     half = x.shape[-1] // 2
