@@ -731,6 +731,7 @@ constexpr int AT_ROWS = 128, AT_TILE = 64, AT_THREADS = 8 * 32, AT_PER_SM = 2, A
 struct AttendJoin {
     int last, q0, n, hk, m;
 };
+constexpr long long AT_STEP_BYTES = 100LL << 20;  // of keys and values, from which on segments begin at CTAs of their own
 constexpr int AT_JOINS = 4 * AR_MAX_CTAS;  // their place in the scratch, behind the other kernel's counters
 // A piece of a segment that one CTA works on: keys from tile0 on, `tiles` of its n_tiles.
 struct AttendSegment {
@@ -910,8 +911,7 @@ __device__ __forceinline__ void at_clean(uint8_t *tile, const uint32_t (&valid)[
 
 template <bool F16, int D>
 __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_kernel(AttendArgs a, const __grid_constant__ CUtensorMap k_map,
-                                                                                            const __grid_constant__ CUtensorMap v_map, int box,
-                                                                                            int min_units, int align, long long limit) {
+                                                                                            const __grid_constant__ CUtensorMap v_map, int box, long long limit) {
     constexpr uint32_t IDESC = (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(AT_ROWS >> 4) << 24);
     constexpr uint32_t IDESC_QK = IDESC | ((uint32_t)(AT_TILE >> 3) << 17), IDESC_PV = IDESC | (1u << 16) | ((uint32_t)(D >> 3) << 17);
     constexpr int HALF = AT_TILE * 128, Q_HALF = AT_ROWS * 128;  // bytes of 64 columns of an operand
@@ -970,10 +970,13 @@ __global__ void __launch_bounds__(AT_THREADS, AT_PER_SM) tree_attention_tiles_ke
             return tiles * a.cache.n_kv;
         });
     };
-    long long units = all_units(1), per = max((units + gridDim.x - 1) / gridDim.x, (long long)min_units), pad = 1;
+    long long units = all_units(1), per = max((units + gridDim.x - 1) / gridDim.x, 1LL), pad = 1;
     // Segments of the same keys (a request's rows beyond 128) should run in step, so that the keys come from memory once.  They do if
-    // every segment begins at a CTA of its own; that takes longer parts, so it is done where the keys do not stay in the L2 anyway.
-    if (align && units * (AT_TILE * D * 4LL) > (long long)align << 20) {
+    // every segment begins at a CTA of its own; that takes longer parts, so it is done where the keys, counted once per segment, do not stay in
+    // the L2 anyway: two trees of 64 over 32000 tokens, 64/8 heads of 128 (262 MB), 171 us, 197 without; four prompts of 512 behind 2000 to 4000 (50 MB)
+    // 153 either way.  Whether any two segments do share keys is not looked at: steps where none do pay for the search, some passes over the
+    // requests' lengths, too.
+    if (units * (AT_TILE * D * 4LL) > AT_STEP_BYTES) {
         if (all_units(per) <= (per + per / 4) * gridDim.x)
             for (long long p = per; pad == 1 && p <= per + per / 4; p += max(per / 32, 1LL))
                 if (all_units(p) <= p * gridDim.x) pad = p;
@@ -1410,9 +1413,6 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
             const int smem = (view.head_dim == 64 ? AT_SMEM<64> : AT_SMEM<128>) + (R + 1) * 8;
             if ((rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "tree_attention shared memory"))) return rc;
             const int grid = min(device_sm_count() * AT_PER_SM, AT_MAX_CTAS);
-            // Segments in step (see there), MB of keys: two trees of 64 over 32000 tokens, 64/8 heads of 128 (262 MB), 171 us, 197 without;
-            // four prompts of 512 behind 2000 to 4000 (50 MB) 153 either way.
-            const int align = (long long)T * (n_heads / view.n_kv) > (long long)AT_ROWS * R ? 100 : 0;
             // boxes of slots that never straddle a page or a tile
             int box = AT_TILE;
             while (box >= 8 && view.page_size % box) box >>= 1;
@@ -1429,7 +1429,7 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
                                                {64u, 1u, (uint32_t)box, 1u}, CU_TENSOR_MAP_SWIZZLE_128B)))
                     return rc;
             }
-            if ((rc = check_cuda(launch_pdl(kernel, dim3(grid), dim3(AT_THREADS), smem, as_stream(stream), a, maps[0], maps[1], box, 1, align, wait_limit_cycles()),
+            if ((rc = check_cuda(launch_pdl(kernel, dim3(grid), dim3(AT_THREADS), smem, as_stream(stream), a, maps[0], maps[1], box, wait_limit_cycles()),
                                  "tree_attention launch")))
                 return rc;
             auto join = view.head_dim == 64 ? (f16 ? tree_attention_join_kernel<true, 64> : tree_attention_join_kernel<false, 64>)
