@@ -600,6 +600,12 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
                         w[i2] = key < 8 ? (key & 1 ? w1 : w0) : (key & 1 ? w3 : w2);
                     }
                     if (o < 0) continue;  // (zeros)
+                    const int d0 = key0 + key - rq.len;
+#pragma unroll
+                    for (int i2 = 0; i2 < 2; ++i2) {  // a weight that came out as 0 leaves infinity infinity; one that is not seen is none
+                        const bool seen = j[i2] >= 0 && (d0 < 0 || (a.mask ? d0 < 64 && (bits[i2] >> d0 & 1) : d0 <= j[i2]));
+                        w[i2] = !seen ? 0.f : w[i2] == 0.f ? 1.f : w[i2];
+                    }
 #pragma unroll
                     for (int c = 0; c < VC; ++c) {
                         if (PADDED && 64 * c + 16 * t4 >= head) continue;
@@ -654,7 +660,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
             for (int w = 0; w < AR_WARPS; ++w) {
                 const float mm = mw[w * 16 + row], f = mm == -INFINITY ? 0.f : exp2_fast(mm - m);
                 l += f * lw[w * 16 + row];
-                if (f == 0.f) continue;
+                if (mm == -INFINITY) continue;  // saw nothing.  (A warp whose weights come out as 0 goes on: 0 times NaN is NaN)
                 const float4 u = *reinterpret_cast<const float4 *>(ow + (w * 16 + row) * D + d);
                 o[0] += f * u.x, o[1] += f * u.y, o[2] += f * u.z, o[3] += f * u.w;
             }
@@ -693,7 +699,7 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
                                 l = l * f + lc[k] * fc;
                                 const float add[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) o[e] = (f == 0.f ? 0.f : o[e] * f) + (fc == 0.f ? 0.f : add[e] * fc);
+                                for (int e = 0; e < 4; ++e) o[e] = o[e] * f + (mc[k] == -INFINITY ? 0.f : add[e] * fc);
                             }
                     }
                     store(row, d, o, l);
@@ -1351,9 +1357,10 @@ __global__ void __launch_bounds__(AT_ROWS) tree_attention_join_kernel(AttendArgs
         for (int k = 0; k < 4; ++k) {
             const float to = fmaxf(top, m[k]), ref = to == -INFINITY ? 0.f : to, keep = exp2_fast(top - ref), f = exp2_fast(m[k] - ref);
             top = to;
-            total = total * keep + (f == 0.f ? 0.f : l[k] * f);
+            total = total * keep + (c + k <= s.last ? l[k] * f : 0.f);
+            // (a part that saw nothing has no sums; of one whose weights come out as 0, NaN stays NaN)
 #pragma unroll
-            for (int e = 0; e < AJ_COLS; ++e) o[e] = (keep == 0.f ? 0.f : o[e] * keep) + (f == 0.f ? 0.f : v[k][e] * f);
+            for (int e = 0; e < AJ_COLS; ++e) o[e] = o[e] * keep + (m[k] == -INFINITY ? 0.f : v[k][e] * f);
         }
     }
     const float inv = total == 0.f ? 0.f : 1.f / total;

@@ -414,3 +414,38 @@ def test_many_small_weights_behind_a_large_one(D, n, per_sm, dtype, gap):
     tol = u * want + (u + 2 * d) * want + (others.max() * 2.0 ** -32 / m if dtype == FP else 0) + torch.finfo(dtype).smallest_normal * 2 * u
     err = (out.double() - want).abs()
     assert bool((err <= tol * 1.001).all()), (float((err / want).max()), float((tol / want).max()))
+
+
+@pytest.mark.parametrize("where", ["first keys", "last keys", "new token"])
+@pytest.mark.parametrize("what", ["V nan", "V inf", "K nan"])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("D,n", [(64, 1), (128, 1), (96, 1), (160, 1), (64, 33), (128, 33)])
+def test_what_a_row_sees_reaches_it_whatever_its_weight(D, n, dtype, what, where):
+    """NaN or infinity in a key that a row sees, but whose score lies so far below that its weight is 0 in 32 bits, alone or with all keys of its
+    tile, its warp and its CTA: the result is not finite there (0 times infinity), and as it was elsewhere."""
+    from mlir_air_b200 import ops
+    length, page, group, kv, gap = 40000, 16, 2, 2, 200.0
+    total = length + n
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    table, pages = make_table([total], page, 1)
+    k, v = torch.zeros((pages, page, kv, D), dtype=dtype, device="cuda"), torch.randn((pages, page, kv, D), device="cuda", generator=gen).to(dtype)
+    at = lambda p: (int(table[0, p // page]), p % page)  # noqa: E731
+    flat = table[0].long()[torch.arange(total, device="cuda") // page] * page + torch.arange(total, device="cuda") % page
+    low = slice(0, length // 2) if where == "first keys" else slice(length // 2, length) if where == "last keys" else slice(length, length + 1)
+    k.flatten(0, 1)[flat[low], :, 3] = -gap
+    q = torch.zeros((n, kv * group, D), dtype=dtype, device="cuda")
+    q[..., 3] = 1
+    args = (table, i32([length]), i32([0, n]), ops.RequestWorkspace())
+    was = ops.tree_attention(q, ops.KVCache(k, v), *args, scale=1.0)
+    assert bool(torch.isfinite(was).all())
+    page_at = at({"first keys": 777, "last keys": length - 333, "new token": length}[where])
+    bad = torch.zeros(was.shape, dtype=torch.bool, device="cuda")
+    if what == "K nan":
+        k[page_at][1, 3] = float("nan")
+        bad[:, group:] = True
+    else:
+        v[page_at][1, 17] = float(what[2:])
+        bad[:, group:, 17] = True
+    got = ops.tree_attention(q, ops.KVCache(k, v), *args, scale=1.0)
+    args[-1].check()
+    assert not bool(torch.isfinite(got[bad]).any()) and torch.equal(got[~bad], was[~bad])
