@@ -494,7 +494,11 @@ int awq_b200_rope_append(const void *q, long long q_row_stride, long long q_head
 /* out[t, h] = softmax over the keys row t sees of scale q[t, h] . k, times v; heads in groups of n_heads / n_kv_heads share a cache
  * head.  A row sees its request's lens[r] cached tokens and of the step's tokens of its request token j if bit j of mask[t] is set
  * (int64 [T], up to 64 tokens per request), or, without `mask`, those up to itself (any number).  A row that sees nothing is 0;
- * rows behind the last request are left as they are.  out may be q (same strides), but not overlap it otherwise. */
+ * rows behind the last request are left as they are.  out may be q (same strides), but not overlap it otherwise.
+ * Scores and sums are f32.  Heads of 64 and 128 whose step has more than 16 rows per request and cache head on average run on a kernel that
+ * rounds the weights exp(score - maximum) to the rows' 16-bit type for the product with V (half a step each; not for their sum); the
+ * others keep 16 bits of them or more.  So a row's last bits may depend on how many rows the other requests bring.  NaN and infinities in
+ * what a row sees reach it, also where the weight is 0. */
 int awq_b200_tree_attention(const void *q, long long q_row_stride, long long q_head_stride, const awq_b200_kv_cache_t *cache,
                             const int32_t *table, long long table_stride, int table_width, const int32_t *lens, const int32_t *q_start,
                             const long long *mask, float scale, void *out, long long out_row_stride, long long out_head_stride, int R, int T,

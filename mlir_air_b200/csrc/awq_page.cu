@@ -59,7 +59,7 @@ __device__ __forceinline__ void block_scan_pair(long long &a, long long &b, long
 //
 // Every CTA scans all requests (two sums over at most 4096 pairs) and then works on its share of the rows and of the new
 // pages: a second launch or a wait between CTAs would cost more than the scan.  The step goes through whole or not at all.
-// Measured: 4 requests 3.4 us, 512 requests with trees 6 us: launch, lengths, scan.
+// Measured: 4 requests 3.8 us, 512 requests with trees 6 us: launch, lengths, scan.
 // =====================================================================================
 constexpr int PLAN_THREADS = 256;
 struct PlanArgs {
@@ -177,8 +177,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) page_plan_kernel(PlanArgs a) {
 // and sums in f32, one rounding, as in rope_halfsplit), K and V written to its slot.  A row whose slot is -1 is left out.
 // A slot that several rows name keeps the last of them, whatever order the CTAs run in: each row looks through the
 // slots behind its own.
-// Measured: one row 2.1 us; 8 prompts of 333 to 1999 tokens, 32/8 heads of 128 (227 MB read and written), 44 us, 5.2 TB/s (34.5 us at a
-// copy's rate).
+// Measured: one row 2.5 us; 8 prompts of 333 to 1999 tokens, 32/8 heads of 128 (227 MB read and written), 44 us, 5.1 TB/s (34.5 us at a
+// copy's rate).  The look through later slots is quadratic: 16000 rows take 78 us (60 for the bytes), 32000 179 (120), 64000 498 (240).
 // =====================================================================================
 constexpr int RA_THREADS = 128;
 struct AppendArgs {

@@ -63,7 +63,7 @@ constexpr float WEIGHT_LIFT = F16 ? 7.f : 0.f;
 __device__ __forceinline__ int page_index(const AttendArgs &a, int key) { return a.page_shift >= 0 ? key >> a.page_shift : key / a.cache.page_size; }
 
 // Head sizes above 128: a CTA per row and head, a warp per 32 keys, four of them at a time; f32 throughout.  Rows of a group do not share
-// their loads.  Bound by instructions (64 requests of 500 to 4000 tokens, 8/4 heads of 256: 767 us, 0.6 TB/s).
+// their loads.  Bound by instructions (64 requests of 500 to 4000 tokens, 8/4 heads of 256: 752 us, 0.75 TB/s).
 constexpr int AA_WARPS = 4;
 template <bool F16>
 __global__ void __launch_bounds__(AA_WARPS * 32) tree_attention_any_kernel(AttendArgs a) {
@@ -181,8 +181,8 @@ __global__ void __launch_bounds__(AA_WARPS * 32) tree_attention_any_kernel(Atten
 //
 // Inside a tile every warp has 16 keys of its own and keeps its own running maximum and sum.  K and V come in by asynchronous
 // copies into shared memory of the warp's own, two blocks ahead, so that 12 warps an SM have up to 190 KB on their way.  Eight
-// lanes fetch 128 bytes of a key at once: requests of half a line, which a lane's own pieces would be, are what the L2's tags
-// run out of first.  In shared memory the pieces lie where mma.sync's lanes find them without bank conflicts:
+// lanes fetch 128 bytes of a key at once: with requests of half a line, which a lane's own pieces would be, 64 long requests took 343 us, not
+// 269.  In shared memory the pieces lie where mma.sync's lanes find them without bank conflicts:
 //   scores: the order of the products over the head is free, so 16 bytes of a key are a lane's operands of two k-steps if the
 //           rows of Q are taken in the same order; odd keys have the halves of their lines swapped;
 //   output: a lane has 16 bytes of four keys (its k-indices) and pairs them up with byte permutes; column n of block j is then
@@ -190,9 +190,9 @@ __global__ void __launch_bounds__(AA_WARPS * 32) tree_attention_any_kernel(Atten
 // Weights are multiplied as two 16-bit pieces, p = hi + lo: the tensor cores have time to spare, and the result keeps 16 (bf16) or 22 bits
 // of a weight; in fp16 those below 2^-21 of the largest keep what lies above 2^-32 of it (WEIGHT_LIFT).
 //
-// Measured, bf16, heads of 128: one token of 64 requests of 1000 to 16000, 64/8 heads, 261 us, 5.9 TB/s (90 % of a copy's rate; keys
-// straight to registers 389); one token of 256 requests of 500 to 2000, 32/8 heads, 196 us, 5.9 TB/s.  Small steps are a chain of
-// latencies: starts and lengths, pages, keys, the join (one token behind 777, 32/8 heads of 64: 9.6 us).
+// Measured, bf16, heads of 128: one token of 64 requests of 1000 to 16000, 64/8 heads, 262 to 278 us, 5.5 to 5.9 TB/s (85 to 90 % of a copy's
+// rate; keys straight to registers 389); one token of 256 requests of 500 to 2000, 32/8 heads, 226 us, 5.9 TB/s.  Small steps are a chain of
+// latencies: starts and lengths, pages, keys, the join (one token behind 777, 32/8 heads of 64: 9.8 us).
 // =====================================================================================
 constexpr int AR_WARPS = 4, AR_TILE = AR_WARPS * 16, AR_PER_SM = 3, AR_ROWS = 16;
 constexpr int AR_MAX_CTAS = 192 * AR_PER_SM;
@@ -300,7 +300,7 @@ constexpr int AR_SMEM = D * 32 + AR_WARPS * AR_PLACES + AR_STAGES<D> + AR_CUM;
 static_assert(AR_SMEM<128> + 64 <= 224 * 1024 / AR_PER_SM - 1024, "three CTAs an SM (76096 bytes a CTA measured two)");
 
 // PADDED: heads of other sizes below D; what lies behind them is 0 in shared memory and neither read nor written (64 requests of 500 to
-// 4000 tokens, 32/8 heads of 96: 92 us, a warp per row and head took 4968).
+// 4000 tokens, 32/8 heads of 96: 100 us, a warp per row and head took 4968).
 template <bool F16, int D, bool PADDED>
 __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_kernel(AttendArgs a) {
     const int head = PADDED ? a.cache.head_dim : D;
@@ -728,9 +728,10 @@ __global__ void __launch_bounds__(AR_WARPS * 32, AR_PER_SM) tree_attention_rows_
 // not): half a step per weight, independent from key to key; in fp16 for weights from 2^-21 of the largest on, smaller ones to 2^-32 of
 // it (WEIGHT_LIFT).
 //
-// Measured, bf16, heads of 128: two trees of 64 over 32000 tokens, 64/8 heads, 163 to 174 us, 770 to 820 TFLOP/s; 16 trees of 8 to 32 over 300 to 6000
-// tokens, 32/8 heads, 58 us; four prompts of 512 behind 2000 to 4000 tokens, 32/8 heads, 153 us, 655 TFLOP/s.  Bound by how fast one CTA's
-// chain S -> weights -> O turns over (a tile of 64 keys takes some 1900 cycles, K and V from the L2 and the exponentials half of that).
+// Measured, bf16, heads of 128: two trees of 64 over 32000 tokens, 64/8 heads, 166 us (810 TFLOP/s) in ten replayed calls, 188 to 193 (700) in
+// calls one after another for some time, when the SMs run slower; 16 trees of 8 to 32 over 300 to 6000 tokens, 32/8 heads, 59 to 62 us; four prompts of
+// 512 behind 2000 to 4000 tokens, 32/8 heads, 151 us, 690 TFLOP/s.  Bound by how fast one CTA's chain S -> weights -> O turns over: a tile of 64 keys
+// takes some 2300 cycles, while the tensor pipe is active for 37 % of them, instructions issue in 41 %, and DRAM is at 18 %.
 // =====================================================================================
 constexpr int AT_ROWS = 128, AT_TILE = 64, AT_THREADS = 8 * 32, AT_PER_SM = 2, AT_MAX_CTAS = 192 * AT_PER_SM, AT_COLS = 256;
 // A segment that begins in a CTA and goes on behind it: where it ends, and its rows.  The next launch joins its parts.
@@ -1413,7 +1414,9 @@ extern "C" int awq_b200_tree_attention(const void *q, long long q_row_stride, lo
     };
     if (view.head_dim == 64 || view.head_dim == 128) {
         // More rows than one mma.sync tile has, on average: tcgen05.  32 requests of 2000 to 4000 tokens, 32/8 heads of 128, trees of 4 (16
-        // rows per head): mma.sync 79 us, tcgen05 89; trees of 8 (32 rows): 118 and 90.
+        // rows per head): mma.sync 79 us, tcgen05 89; trees of 8 (32 rows): 118 and 92.  The host knows the average alone, over all R requests, those
+        // that bring no rows too, and one kernel takes the whole step: a prompt's chunk of 1000 rows beside 63 single tokens takes 177 us, the two
+        // apart 77 and 66; 8 trees of 32 among 64 requests 64 us, without the idle ones 40.
         if ((long long)T * (n_heads / view.n_kv) > (long long)AR_ROWS * R) {
             auto kernel = view.head_dim == 64 ? (f16 ? tree_attention_tiles_kernel<true, 64> : tree_attention_tiles_kernel<false, 64>)
                                               : (f16 ? tree_attention_tiles_kernel<true, 128> : tree_attention_tiles_kernel<false, 128>);

@@ -104,7 +104,8 @@ class DecoderStack:
         self.gemm_ws = ops.GemmDecodeWorkspace(widest, device=device, batch=self.MAX_DECODE_ROWS, K=deepest)
 
     def _project(self, x, w: AwqWeight, adapters, idx, residual=None):
-        """bf16(x W (+ adapters) (+ residual)): one rounding on the decode path, where the adapters take the projection's f32 sums."""
+        """bf16(x W (+ adapters) (+ residual)): one rounding on the decode path, where the adapters take the projection's f32 sums; more rows go
+        through the prefill GEMM, which rounds the weights to bf16, and adapters are added to its bf16 output."""
         if x.shape[0] > self.MAX_DECODE_ROWS:
             if adapters is None or idx is None:
                 return ops.gemm(x, w, residual=residual)

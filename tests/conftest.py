@@ -12,9 +12,9 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (B200)")
 
 
-# Draws its inputs anew each time, and its bound does not allow for what the path rounds on more than 64 rows: 13 of 30 draws missed it
-# (test_gpu_decoder_rounding.py has the same steps against what the path does).  Last, so that a run that ends at the first failure has
-# been through everything else.
+# Takes its inputs from the global generator, wherever that stands by then, and its bound does not allow for what the path rounds on more than
+# 64 rows: 13 of 30 draws missed it (test_gpu_decoder_rounding.py has such steps against what the path does).  Last, so that a run that
+# ends at the first failure has been through everything else.
 LAST = "test_gpu_decoder.py::test_prompts_trees_and_single_tokens[True]"
 
 
